@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define NVFP4B200_API_VERSION 4
+#define NVFP4B200_API_VERSION 5
 
 enum nvfp4b200_status {
   NVFP4B200_OK = 0,
@@ -41,7 +41,8 @@ enum nvfp4b200_status {
   NVFP4B200_ERR_CUDA = 7              /* another CUDA runtime/driver call failed         */
 };
 
-enum nvfp4b200_dtype { NVFP4B200_BF16 = 0, NVFP4B200_F32 = 1 };
+/* F16 is taken by the entry points that say so. */
+enum nvfp4b200_dtype { NVFP4B200_BF16 = 0, NVFP4B200_F32 = 1, NVFP4B200_F16 = 2 };
 enum nvfp4b200_epilogue { NVFP4B200_EPI_NONE = 0, NVFP4B200_EPI_RELU = 1, NVFP4B200_EPI_RELU2 = 2 };
 
 /* Library / device information. */
@@ -213,6 +214,99 @@ int nvfp4b200_gemm(const void* a, const void* b, const void* sfa, const void* sf
                    int64_t m, int64_t n, int64_t k, int64_t ldd, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* MXFP4 operands and their product (the reference has the product only)    */
+/* ------------------------------------------------------------------------ */
+
+/* MXFP4 quantizer: E2M1 with one UE8M0 scale per block of 32, in either or
+ * both orientations from one read of x.  y = (x * row_scale[r]) * gamma[c]
+ * (both factors optional, each product rounded once in fp32);
+ *   code = max(exponent field of the block's amax as fp32 - 2, 0)
+ *   q    = e2m1(y * 2^(127 - code)), nearest, ties to even, saturated to 6.
+ * A block with an infinity or a NaN gets code 0xFF (NaN) and unspecified
+ * nibbles.  x: [rows, cols] of x_dtype (bf16, f16 or f32), row stride ldx
+ * (ldx % 8 == 0); row_scale fp32 [rows]; gamma bf16 [cols].
+ * Rows: q u8 [rows, cols/2], s the 128x4-atom layout of
+ * [round_up(rows,128), round_up(cols/32,4)] bytes; cols % 32 == 0.
+ * Transposed: with prows = round_up(rows, 32), the rows past the last taken
+ * as zeros, qt u8 [cols, prows/2], st for [round_up(cols,128),
+ * round_up(prows/32,4)]; cols % 8 == 0.  q and s, qt and st are NULL together
+ * where that orientation is not wanted.  Every byte of the outputs is written
+ * (padding codes are 0) unless rows == 0, when nothing is. */
+int nvfp4b200_mx_quant(const void* x, int x_dtype, const float* row_scale, const void* gamma, void* q, void* s,
+                       void* qt, void* st, int64_t rows, int64_t cols, int64_t ldx, void* stream);
+
+/* The values of an MXFP4 matrix: y[r, c] = e2m1 * 2^(code - 127), exact in
+ * bf16 and fp32 while it is in their range; a code of 0xFF gives NaN.  q u8
+ * [rows, k/2], s as nvfp4b200_mx_quant writes it, y bf16 or f32 [rows, k];
+ * k % 32 == 0. */
+int nvfp4b200_mx_dequant(const void* q, const void* s, void* y, int y_dtype, int64_t rows, int64_t k, void* stream);
+
+/* nvfp4b200_mxfp4_mm in the general form of nvfp4b200_gemm (without operand
+ * scales, which MXFP4 has none of): v = epilogue(A . B^T + bias) + residual;
+ * d_dtype BF16 stores bf16(v), F32 stores v or, with accumulate, adds it. */
+int nvfp4b200_mx_gemm(const void* a, const void* b, const void* sfa, const void* sfb, const void* bias,
+                      const void* residual, void* d, int d_dtype, int accumulate, int epilogue, int64_t m, int64_t n,
+                      int64_t k, int64_t ldd, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Global gradient norm and clipping (no reference counterpart)             */
+/* ------------------------------------------------------------------------ */
+
+/* Doubles of workspace that nvfp4b200_grad_norm needs for `count` tensors. */
+#define NVFP4B200_GRAD_WS_DOUBLES(count) (1024 * (1 + (int64_t)(count) / 112))
+
+/* norm = |grad_scale| * sqrt(sum of all g^2) (norm_type 2) or
+ * |grad_scale| * max |g| (norm_type 0); coef = min(1, max_norm / (norm +
+ * 1e-6)).  The lists are host arrays of `count` device pointers, dtypes (bf16,
+ * f16 or f32) and lengths; they are read before the call returns.  norm, coef
+ * (fp32) and total (fp64: the bare sum of squares or maximum, for a sum over
+ * ranks) are optional outputs.  With outs, out_i = round(g_i * (grad_scale *
+ * coef)) in out_dtypes; an output may be its own gradient (then nothing is
+ * written when the factor is 1) and overlaps no other tensor of the call
+ * (NVFP4B200_ERR_INVALID_ARG).  A NaN among the gradients makes norm and coef
+ * NaN; an infinite norm makes coef 0.  ws: NVFP4B200_GRAD_WS_DOUBLES(count)
+ * doubles, contents irrelevant.  The result does not depend on timing. */
+int nvfp4b200_grad_norm(const void* const* grads, const int* grad_dtypes, void* const* outs, const int* out_dtypes,
+                        const int64_t* numels, int count, int norm_type, float grad_scale, float max_norm,
+                        double* ws, int64_t ws_doubles, float* norm, float* coef, double* total, void* stream);
+
+/* norm and coef as above from n totals (fp64, of this rank or summed over
+ * ranks); n <= 2^20. */
+int nvfp4b200_grad_norm_finish(const double* partials, int64_t n, int norm_type, float grad_scale, float max_norm,
+                               float* norm, float* coef, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Norms after and before a block, with gate and residual scale (no         */
+/* reference counterpart)                                                   */
+/* ------------------------------------------------------------------------ */
+
+/* y = residual_scale * x + branch_scale * gate[g] * (b * inv_b * gamma_post),
+ * inv_b = rsqrt(mean(b^2) + eps); and, when n is given, n = y * inv_y *
+ * gamma_pre with inv_y = rsqrt(mean(y^2) + eps) of y as stored.  b, x, y, n:
+ * [rows, d] of dtype (bf16, f16 or f32), b and x with row strides ldb, ldx;
+ * gamma_post, gamma_pre [d] and gate [groups, d] of the same dtype, each
+ * optional (1); row r takes gate row r / (rows / groups); groups = 0 without
+ * a gate, rows % groups == 0.  n and inv_y are NULL together.  d <= 16384. */
+int nvfp4b200_sandwich_norm(const void* b, const void* x, const void* gamma_post, const void* gate,
+                            const void* gamma_pre, void* y, void* n, float* inv_b, float* inv_y, int dtype,
+                            int64_t rows, int64_t d, int64_t groups, int64_t ldb, int64_t ldx, float residual_scale,
+                            float branch_scale, float eps, void* stream);
+
+/* *floats = fp32 words of workspace that the backward needs on this device. */
+int nvfp4b200_sandwich_norm_bwd_ws(int64_t rows, int64_t d, int64_t groups, int64_t* floats);
+
+/* Backward of nvfp4b200_sandwich_norm given dy and, when n was taken, dn (then
+ * with y and inv_y; one of dy and dn may be NULL, a gradient of zeros): dx and db [rows, d] of dtype; dgamma_post and dgamma_pre
+ * fp32 [d], dgate fp32 [groups, d], each optional and written, not added to.
+ * Column sums are added up in a fixed order.  ws: contents irrelevant. */
+int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, const void* y, const float* inv_b,
+                                const float* inv_y, const void* gamma_post, const void* gate, const void* gamma_pre,
+                                void* dx, void* db, float* dgamma_post, float* dgate, float* dgamma_pre, float* ws,
+                                int64_t ws_floats, int dtype, int64_t rows, int64_t d, int64_t groups, int64_t ld_dy,
+                                int64_t ld_dn, int64_t ldb, int64_t ldy, float residual_scale, float branch_scale,
+                                void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Training-step element-wise kernels (no reference counterpart: the        */
 /* reference's backward is bf16, float4utils.py:653-683)                     */
 /* ------------------------------------------------------------------------ */
@@ -270,6 +364,17 @@ int nvfp4b200_adamw_master_step(void* param, float* master, const void* grad, in
                                 int64_t n, float one_minus_lr_wd, float one_minus_beta1, float beta2,
                                 float one_minus_beta2, float eps, float step_size, float bias_corr2_sqrt,
                                 float grad_scale, uint32_t* amax_bits, void* stream);
+
+/* The two AdamW steps with one more factor on the gradient, a device scalar
+ * (NULL = 1): g = grad * (grad_scale * *clip).  It is the coef of
+ * nvfp4b200_grad_norm, so clipping costs no pass of its own and no host read. */
+int nvfp4b200_adamw_step_clipped(void* param, const void* grad, int grad_dtype, float* m, float* v, int64_t n, float lr,
+                                 float beta1, float beta2, float eps, float weight_decay, float bias_corr1,
+                                 float bias_corr2, float grad_scale, const float* clip, void* stream);
+int nvfp4b200_adamw_master_step_clipped(void* param, float* master, const void* grad, int grad_dtype, float* m,
+                                        float* v, int64_t n, float one_minus_lr_wd, float one_minus_beta1, float beta2,
+                                        float one_minus_beta2, float eps, float step_size, float bias_corr2_sqrt,
+                                        float grad_scale, const float* clip, uint32_t* amax_bits, void* stream);
 
 /* Global scales from amaxes (no reference counterpart): for i < n,
  * global_scale_out[i] = amax_i/(6*448), amax_i = float bits amax_bits[i],

@@ -1460,6 +1460,13 @@ int nvfp4b200_mxfp4_mm(const void* a, const void* b, const void* sfa, const void
                    n, (cudaStream_t)stream, nullptr, nullptr, /*mx=*/1);
 }
 
+int nvfp4b200_mx_gemm(const void* a, const void* b, const void* sfa, const void* sfb, const void* bias,
+                      const void* residual, void* d, int d_dtype, int accumulate, int epilogue, int64_t m, int64_t n,
+                      int64_t k, int64_t ldd, void* stream) {
+  return gemm::run(a, b, sfa, sfb, nullptr, nullptr, bias, residual, d, d_dtype, accumulate, epilogue, m, n, k, ldd,
+                   (cudaStream_t)stream, nullptr, nullptr, /*mx=*/1);
+}
+
 int nvfp4b200_nvfp4_mm_relu(const void* a, const void* b, const void* sfa, const void* sfb, const float* output_scale,
                             const void* bias, void* d, int64_t m, int64_t n, int64_t k, void* stream) {
   return gemm::run(a, b, sfa, sfb, output_scale, nullptr, bias, nullptr, d, NVFP4B200_BF16, 0, NVFP4B200_EPI_RELU, m,

@@ -1,0 +1,524 @@
+// The RMSNorms after and before a block, fused with the block's gate and the
+// residual's scale (B200, sm_100a).
+//
+//     y = alpha * x + s * gate[g] * (b * inv_b * gamma_post),   inv_b = rsqrt(mean(b^2) + eps)
+//     n = y * inv_y * gamma_pre,                                inv_y = rsqrt(mean(y^2) + eps)
+//
+// b is the block's output, x the residual stream, gate [G, D] belongs to G
+// equal runs of rows (G = 1: a channel gate, G = sequences: a gate of their
+// own), n the next block's input.  n is the norm of y as stored: y is rounded
+// to its type first, so n and inv_y are what the separate norm of the stored
+// y gives, and what the backward, which only has the stored y, assumes.
+//
+// Backward, given dy (the gradient that reaches y from behind) and dn:
+//     yh = y * inv_y;  v = dn * gamma_pre
+//     t  = dy + inv_y * (v - yh * mean(v * yh))
+//     dx = alpha * t
+//     bh = b * inv_b;  u = s * t * gate * gamma_post
+//     db = inv_b * (u - bh * mean(u * bh))
+//     S_g = sum over the rows of g of s * t * bh
+//     dgate[g] = gamma_post * S_g;  dgamma_post = sum_g gate[g] * S_g
+//     dgamma_pre = sum over rows of dn * yh
+// so one column sum per group carries both the gate's and the norm weight's
+// gradient.  All statistics and sums are fp32; column sums are added up in a
+// fixed order (rows in a CTA, CTAs in a second kernel), never by atomics.
+//
+// Bound: HBM, one read of each input and one write of each output.
+#include "vec.cuh"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace nvfp4b200 {
+namespace norm {
+
+constexpr int VPT = 2;            // 8-element vectors per thread and row
+constexpr int CPT = 8 * VPT;      // columns per thread
+constexpr int MAX_D = 1024 * CPT;
+
+// Column of a thread's element j: vectors of 8 (VEC), or strided single
+// elements for widths and strides that no 16-byte vector fits.
+template <bool VEC, int TPR>
+__device__ __forceinline__ int column(int t, int j) {
+  return VEC ? (j >> 3) * (TPR * 8) + 8 * t + (j & 7) : j * TPR + t;
+}
+
+// One row's elements of a tensor as raw vectors (VEC) or floats.
+template <int DT, bool VEC, int TPR>
+struct Row {
+  typename Elem<DT>::Vec8 v[VEC ? VPT : 1];
+  float f[VEC ? 1 : CPT];
+
+  __device__ __forceinline__ void load(const typename Elem<DT>::Raw* p, int t, int d) {
+    if (VEC) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int c = column<true, TPR>(t, 8 * i);
+        v[i] = Elem<DT>::zero();
+        if (c < d) v[i] = Elem<DT>::load(p + c);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) {
+        const int c = column<false, TPR>(t, j);
+        f[j] = c < d ? Elem<DT>::get(p + c) : 0.0f;
+      }
+    }
+  }
+  __device__ __forceinline__ void values(float (&o)[CPT]) const {
+    if (VEC) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float t[8];
+        Elem<DT>::unpack(v[i], t);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[8 * i + j] = t[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) o[j] = f[j];
+    }
+  }
+};
+
+// Rounds the values to the stored type and writes them; `o` becomes what was stored.
+template <int DT, bool VEC, int TPR>
+__device__ __forceinline__ void store_row(typename Elem<DT>::Raw* p, int t, int d, float (&o)[CPT]) {
+  if (VEC) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = column<true, TPR>(t, 8 * i);
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = o[8 * i + j];
+      const auto v = Elem<DT>::pack(f);
+      if (c < d) Elem<DT>::store(p + c, v);
+      Elem<DT>::unpack(v, f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[8 * i + j] = f[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < CPT; ++j) {
+      const int c = column<false, TPR>(t, j);
+      const auto b = Elem<DT>::bits(o[j]);
+      if (c < d) p[c] = b;
+      o[j] = Elem<DT>::value(b);
+    }
+  }
+}
+
+// Sum over the TPR threads of a row; the same bits in every thread.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float s, float* red, int group) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (TPR == 32) return s;
+  constexpr int W = TPR / 32;
+  const int w = (threadIdx.x % TPR) >> 5;
+  if ((threadIdx.x & 31) == 0) red[group * W + w] = s;
+  if (TPR == 1024 || TPR == (int)blockDim.x) __syncthreads();
+  else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(TPR) : "memory");
+  s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) s += red[group * W + i];
+  return s;
+}
+
+struct FwdArgs {
+  const void *b, *x, *gamma_post, *gate, *gamma_pre;
+  void *y, *n;
+  float *inv_b, *inv_y;
+  int64_t rows, ldb, ldx, rows_per_gate;
+  int d;
+  float alpha, s, eps;
+  int pre;
+};
+
+template <int DT, bool VEC, int TPR>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) sandwich_fwd_kernel(const FwdArgs a) {
+  using Raw = typename Elem<DT>::Raw;
+  constexpr int GROUPS = TPR < 256 ? 256 / TPR : 1;
+  __shared__ float red[4][GROUPS * (TPR / 32)];
+  const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  const Raw *B = static_cast<const Raw*>(a.b), *X = static_cast<const Raw*>(a.x);
+  const float inv_d = 1.0f / (float)a.d;
+  int buf = 0;
+  for (int64_t r = (int64_t)blockIdx.x * GROUPS + group; r < a.rows; r += (int64_t)gridDim.x * GROUPS) {
+    Row<DT, VEC, TPR> rb, rx, rw;
+    float b[CPT], o[CPT], w[CPT];
+    rb.load(B + r * a.ldb, t, a.d);
+    rx.load(X + r * a.ldx, t, a.d);
+    rb.values(b);
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < CPT; ++j) ss = fmaf(b[j], b[j], ss);
+    const float inv_b = rsqrtf(row_sum<TPR>(ss, red[buf], group) * inv_d + a.eps);
+#pragma unroll
+    for (int j = 0; j < CPT; ++j) b[j] *= inv_b;
+    if (a.gamma_post) {
+      rw.load(static_cast<const Raw*>(a.gamma_post), t, a.d);
+      rw.values(w);
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) b[j] *= w[j];
+    }
+    if (a.gate) {
+      rw.load(static_cast<const Raw*>(a.gate) + (r / a.rows_per_gate) * a.d, t, a.d);
+      rw.values(w);
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) b[j] *= w[j];
+    }
+    rx.values(o);
+#pragma unroll
+    for (int j = 0; j < CPT; ++j) o[j] = fmaf(a.s, b[j], a.alpha * o[j]);
+    store_row<DT, VEC, TPR>(static_cast<Raw*>(a.y) + r * a.d, t, a.d, o);
+    if (t == 0) a.inv_b[r] = inv_b;
+    if (a.pre) {
+      ss = 0.0f;
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) ss = fmaf(o[j], o[j], ss);
+      const float inv_y = rsqrtf(row_sum<TPR>(ss, red[buf + 1], group) * inv_d + a.eps);
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) o[j] *= inv_y;
+      if (a.gamma_pre) {
+        rw.load(static_cast<const Raw*>(a.gamma_pre), t, a.d);
+        rw.values(w);
+#pragma unroll
+        for (int j = 0; j < CPT; ++j) o[j] *= w[j];
+      }
+      store_row<DT, VEC, TPR>(static_cast<Raw*>(a.n) + r * a.d, t, a.d, o);
+      if (t == 0) a.inv_y[r] = inv_y;
+    }
+    buf ^= 2;   // a row's two sums use two slots; a slot is written again two rows later, past two barriers
+  }
+}
+
+struct BwdArgs {
+  const void *dy, *dn, *b, *y, *gamma_post, *gate, *gamma_pre;
+  const float *inv_b, *inv_y;
+  void *dx, *db;
+  float* part;              // [2][ctas][d]: gate-weighted S (dgamma_post), dgamma_pre
+  float* part_gate;         // [G * parts][d]: S of a part of a group's rows (parts > 1)
+  float* dgate;             // [G][d], written here when a CTA holds whole groups; or null
+  int64_t rows, ldb, ld_dy, ld_dn, ldy, rows_per_gate, rows_per_cta;
+  int d;
+  float alpha, s;
+};
+
+// A CTA walks rows_per_cta consecutive rows, one at a time.  rows_per_cta
+// divides rows_per_gate or is a multiple of it, so a CTA's rows lie in one
+// group or are whole groups.  (Groups of rows that end early are handled by
+// the host: parts of a group are cut at its end.)
+template <int DT, bool VEC, int TPR>
+__global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int64_t parts_per_group) {
+  using Raw = typename Elem<DT>::Raw;
+  __shared__ float red[4][TPR / 32];
+  const int t = threadIdx.x;
+  const float inv_d = 1.0f / (float)a.d;
+  // the CTA's rows: part p of group g, or a run of whole groups
+  int64_t r, end;
+  if (parts_per_group > 1) {
+    const int64_t g = blockIdx.x / parts_per_group, p = blockIdx.x % parts_per_group;
+    r = g * a.rows_per_gate + p * a.rows_per_cta;
+    end = imin64(r + a.rows_per_cta, (g + 1) * a.rows_per_gate);
+  } else {
+    r = (int64_t)blockIdx.x * a.rows_per_cta;
+    end = imin64(r + a.rows_per_cta, a.rows);
+  }
+  float S[CPT], post[CPT], pre[CPT];
+#pragma unroll
+  for (int j = 0; j < CPT; ++j) S[j] = post[j] = pre[j] = 0.0f;
+  int buf = 0;
+  for (; r < end; ++r) {
+    Row<DT, VEC, TPR> row, rb, rw;
+    float tt[CPT], z[CPT], w[CPT], v[CPT];
+    if (a.dy) row.load(static_cast<const Raw*>(a.dy) + r * a.ld_dy, t, a.d);
+    rb.load(static_cast<const Raw*>(a.b) + r * a.ldb, t, a.d);
+    if (a.dy) {
+      row.values(tt);
+    } else {
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) tt[j] = 0.0f;
+    }
+    if (a.dn) {
+      Row<DT, VEC, TPR> rn, ry;
+      rn.load(static_cast<const Raw*>(a.dn) + r * a.ld_dn, t, a.d);
+      ry.load(static_cast<const Raw*>(a.y) + r * a.ldy, t, a.d);
+      rn.values(v);
+      ry.values(z);
+      const float inv = __ldg(a.inv_y + r);
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) {
+        z[j] *= inv;
+        pre[j] = fmaf(v[j], z[j], pre[j]);
+      }
+      if (a.gamma_pre) {
+        rw.load(static_cast<const Raw*>(a.gamma_pre), t, a.d);
+        rw.values(w);
+#pragma unroll
+        for (int j = 0; j < CPT; ++j) v[j] *= w[j];
+      }
+      float dot = 0.0f;
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) dot = fmaf(v[j], z[j], dot);
+      const float mean = row_sum<TPR>(dot, red[buf], 0) * inv_d;
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) tt[j] = fmaf(inv, fmaf(-mean, z[j], v[j]), tt[j]);
+    }
+    const float inv = __ldg(a.inv_b + r);
+    rb.values(z);
+#pragma unroll
+    for (int j = 0; j < CPT; ++j) {
+      z[j] *= inv;
+      v[j] = a.s * tt[j];
+      S[j] = fmaf(v[j], z[j], S[j]);
+    }
+    if (a.gamma_post) {
+      rw.load(static_cast<const Raw*>(a.gamma_post), t, a.d);
+      rw.values(w);
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) v[j] *= w[j];
+    }
+    if (a.gate) {
+      rw.load(static_cast<const Raw*>(a.gate) + (r / a.rows_per_gate) * a.d, t, a.d);
+      rw.values(w);
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) v[j] *= w[j];
+    }
+    float dot = 0.0f;
+#pragma unroll
+    for (int j = 0; j < CPT; ++j) dot = fmaf(v[j], z[j], dot);
+    const float mean = row_sum<TPR>(dot, red[buf + 1], 0) * inv_d;
+#pragma unroll
+    for (int j = 0; j < CPT; ++j) z[j] = inv * fmaf(-mean, z[j], v[j]);
+    store_row<DT, VEC, TPR>(static_cast<Raw*>(a.db) + r * a.d, t, a.d, z);
+#pragma unroll
+    for (int j = 0; j < CPT; ++j) tt[j] *= a.alpha;
+    store_row<DT, VEC, TPR>(static_cast<Raw*>(a.dx) + r * a.d, t, a.d, tt);
+    buf ^= 2;
+    // the last row of a group (or of this CTA's part of it): hand S over
+    if (a.gate && (r + 1 == end || (r + 1) % a.rows_per_gate == 0)) {
+      const int64_t g = r / a.rows_per_gate;
+      rw.load(static_cast<const Raw*>(a.gate) + g * a.d, t, a.d);
+      rw.values(w);
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) post[j] = fmaf(w[j], S[j], post[j]);
+      float* out = parts_per_group > 1 ? a.part_gate + (int64_t)blockIdx.x * a.d : a.dgate ? a.dgate + g * a.d : nullptr;
+      if (parts_per_group == 1 && a.gamma_post) {
+        rw.load(static_cast<const Raw*>(a.gamma_post), t, a.d);
+        rw.values(w);
+#pragma unroll
+        for (int j = 0; j < CPT; ++j) S[j] *= w[j];
+      }
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) {
+        const int c = column<VEC, TPR>(t, j);
+        if (out && c < a.d) out[c] = S[j];
+        S[j] = 0.0f;
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < CPT; ++j) {
+    const int c = column<VEC, TPR>(t, j);
+    if (c < a.d) {
+      a.part[(int64_t)blockIdx.x * a.d + c] = a.gate ? post[j] : S[j];
+      a.part[((int64_t)gridDim.x + blockIdx.x) * a.d + c] = pre[j];
+    }
+  }
+}
+
+// Column sums of the partials, in CTA order.  Job 0 is dgamma_post, 1
+// dgamma_pre, 2 + g dgate of group g, each over blocks of 32 columns.  Eight threads share a column's run of
+// partials (each a contiguous eighth), their sums are added in order.
+struct FinishArgs {
+  const float *part, *part_gate;
+  const void* gamma_post;
+  float *dgamma_post, *dgamma_pre, *dgate;
+  int64_t ctas, parts_per_group;
+  int d;
+};
+
+template <int DT>
+__global__ void __launch_bounds__(256) sandwich_bwd_finish_kernel(const FinishArgs a) {
+  __shared__ float red[8][33];
+  const int col = threadIdx.x & 31, seg = threadIdx.x >> 5;
+  const int blocks = (a.d + 31) / 32;
+  const int c = (int)(blockIdx.x % blocks) * 32 + col;
+  const int64_t job = blockIdx.x / blocks;
+  const float* p;
+  float* out;
+  int64_t n;
+  if (job == 0) { p = a.part; out = a.dgamma_post; n = a.ctas; }
+  else if (job == 1) { p = a.part + a.ctas * a.d; out = a.dgamma_pre; n = a.ctas; }
+  else { p = a.part_gate + (job - 2) * a.parts_per_group * a.d; out = a.dgate + (job - 2) * a.d; n = a.parts_per_group; }
+  if ((job == 0 && !a.dgamma_post) || (job == 1 && !a.dgamma_pre)) return;
+  const int64_t per = (n + 7) / 8, lo = per * seg, hi = imin64(n, lo + per);
+  float s = 0.0f;
+  if (c < a.d)
+    for (int64_t i = lo; i < hi; ++i) s += p[i * a.d + c];
+  red[seg][col] = s;
+  __syncthreads();
+  if (seg == 0 && c < a.d) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += red[i][col];
+    if (job >= 2 && a.gamma_post) s *= Elem<DT>::get(static_cast<const typename Elem<DT>::Raw*>(a.gamma_post) + c);
+    out[c] = s;
+  }
+}
+
+template <typename F>
+static int by_width(int d, F f) {
+  if (d <= 32 * CPT) return f(std::integral_constant<int, 32>());
+  if (d <= 64 * CPT) return f(std::integral_constant<int, 64>());
+  if (d <= 128 * CPT) return f(std::integral_constant<int, 128>());
+  if (d <= 256 * CPT) return f(std::integral_constant<int, 256>());
+  if (d <= 512 * CPT) return f(std::integral_constant<int, 512>());
+  return f(std::integral_constant<int, 1024>());
+}
+
+template <typename F>
+static int by_type(int dt, bool vec, F f) {
+#define NORM_DT(D)                                                                         \
+  return vec ? f(std::integral_constant<int, D>(), std::true_type())                       \
+             : f(std::integral_constant<int, D>(), std::false_type())
+  if (dt == NVFP4B200_BF16) { NORM_DT(NVFP4B200_BF16); }
+  if (dt == NVFP4B200_F16) { NORM_DT(NVFP4B200_F16); }
+  NORM_DT(NVFP4B200_F32);
+#undef NORM_DT
+}
+
+// How the backward splits its rows over CTAs.  A function of the sizes alone.
+struct Split {
+  int64_t rows_per_cta, parts_per_group, ctas;
+};
+
+static Split split_rows(int64_t rows, int64_t groups, int64_t d, int sms) {
+  // 512 threads' worth of CTAs per SM (128 registers a thread), narrow rows in
+  // more, smaller CTAs
+  int64_t tpr = 32;
+  while (tpr * CPT < d) tpr *= 2;
+  const int64_t per = rows / groups, target = std::max<int64_t>(1, 512 / tpr) * sms;
+  Split s;
+  if (groups >= target || per == 1) {             // whole groups per CTA
+    const int64_t g = std::max<int64_t>(1, ceil_div(groups, target));
+    s.rows_per_cta = g * per;
+    s.parts_per_group = 1;
+    s.ctas = ceil_div(groups, g);
+  } else {
+    const int64_t parts = std::min(per, std::max<int64_t>(1, target / groups));
+    s.rows_per_cta = ceil_div(per, parts);
+    s.parts_per_group = ceil_div(per, s.rows_per_cta);
+    s.ctas = groups * s.parts_per_group;
+  }
+  return s;
+}
+
+}  // namespace norm
+}  // namespace nvfp4b200
+
+using namespace nvfp4b200;
+
+static bool vec_ok(const void* p, int64_t ld, int bytes) { return !p || (aligned(p, 16) && (ld * bytes) % 16 == 0); }
+
+extern "C" {
+
+int nvfp4b200_sandwich_norm(const void* b, const void* x, const void* gamma_post, const void* gate,
+                            const void* gamma_pre, void* y, void* n, float* inv_b, float* inv_y, int dtype,
+                            int64_t rows, int64_t d, int64_t groups, int64_t ldb, int64_t ldx, float residual_scale,
+                            float branch_scale, float eps, void* stream) {
+  if (!b || !x || !y || !inv_b || (n == nullptr) != (inv_y == nullptr) || (gamma_pre && !n) || !valid_dtype(dtype))
+    return NVFP4B200_ERR_INVALID_ARG;
+  if (rows < 0 || d <= 0 || d > norm::MAX_D || ldb < d || ldx < d || groups < 0 || (gate == nullptr) != (groups == 0) ||
+      (groups && rows % groups))
+    return NVFP4B200_ERR_BAD_SHAPE;
+  const int bytes = dtype_bytes(dtype);
+  for (const void* p : {b, x, gamma_post, gate, gamma_pre, (const void*)y, (const void*)n})
+    if (p && !aligned(p, bytes)) return NVFP4B200_ERR_MISALIGNED;
+  if (!aligned(inv_b, 4) || (inv_y && !aligned(inv_y, 4))) return NVFP4B200_ERR_MISALIGNED;
+  int rc = check_device();
+  if (rc) return rc;
+  if (rows == 0) return NVFP4B200_OK;
+  norm::FwdArgs a{b, x, gamma_post, gate, gamma_pre, y, n, inv_b, inv_y, rows, ldb, ldx, groups ? rows / groups : rows,
+                  (int)d, residual_scale, branch_scale, eps, n != nullptr};
+  const bool vec = (d * bytes) % 16 == 0 && d % 8 == 0 && vec_ok(b, ldb, bytes) && vec_ok(x, ldx, bytes) &&
+                   vec_ok(gamma_post, d, bytes) && vec_ok(gate, d, bytes) && vec_ok(gamma_pre, d, bytes) &&
+                   vec_ok(y, d, bytes) && vec_ok(n, d, bytes);
+  cudaStream_t st = (cudaStream_t)stream;
+  return norm::by_type(dtype, vec, [&](auto dt, auto v) {
+    return norm::by_width((int)d, [&](auto tpr) {
+      constexpr int T = decltype(tpr)::value, THREADS = T < 256 ? 256 : T, GROUPS = THREADS / T;
+      const int64_t want = ceil_div(rows, GROUPS);
+      const unsigned grid = (unsigned)std::min<int64_t>(want, (int64_t)sm_count_current() * (2048 / THREADS));
+      norm::sandwich_fwd_kernel<decltype(dt)::value, decltype(v)::value, T><<<grid, THREADS, 0, st>>>(a);
+      return launch_status();
+    });
+  });
+}
+
+int nvfp4b200_sandwich_norm_bwd_ws(int64_t rows, int64_t d, int64_t groups, int64_t* floats) {
+  if (!floats) return NVFP4B200_ERR_INVALID_ARG;
+  if (rows < 0 || d <= 0 || d > norm::MAX_D || groups < 0 || (groups && rows % groups)) return NVFP4B200_ERR_BAD_SHAPE;
+  *floats = 0;
+  if (rows == 0) return NVFP4B200_OK;
+  const norm::Split s = norm::split_rows(rows, groups ? groups : 1, d, sm_count_current());
+  *floats = (2 * s.ctas + (groups && s.parts_per_group > 1 ? s.ctas : 0)) * d;
+  return NVFP4B200_OK;
+}
+
+int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, const void* y, const float* inv_b,
+                                const float* inv_y, const void* gamma_post, const void* gate, const void* gamma_pre,
+                                void* dx, void* db, float* dgamma_post, float* dgate, float* dgamma_pre, float* ws,
+                                int64_t ws_floats, int dtype, int64_t rows, int64_t d, int64_t groups, int64_t ld_dy,
+                                int64_t ld_dn, int64_t ldb, int64_t ldy, float residual_scale, float branch_scale,
+                                void* stream) {
+  if ((!dy && !dn) || !b || !inv_b || !dx || !db || !ws || (dn == nullptr) != (y == nullptr) ||
+      (dn == nullptr) != (inv_y == nullptr) || (gamma_pre && !dn) || (dgamma_pre && !dn) || (dgate && !gate) ||
+      !valid_dtype(dtype))
+    return NVFP4B200_ERR_INVALID_ARG;
+  if (rows < 0 || d <= 0 || d > norm::MAX_D || (dy && ld_dy < d) || ldb < d || (dn && (ld_dn < d || ldy < d)) || groups < 0 ||
+      (gate == nullptr) != (groups == 0) || (groups && rows % groups))
+    return NVFP4B200_ERR_BAD_SHAPE;
+  const int bytes = dtype_bytes(dtype);
+  for (const void* p : {dy, dn, b, y, gamma_post, gate, gamma_pre, (const void*)dx, (const void*)db})
+    if (p && !aligned(p, bytes)) return NVFP4B200_ERR_MISALIGNED;
+  for (const void* p : {(const void*)inv_b, (const void*)inv_y, (const void*)dgamma_post, (const void*)dgate,
+                        (const void*)dgamma_pre, (const void*)ws})
+    if (p && !aligned(p, 4)) return NVFP4B200_ERR_MISALIGNED;
+  int rc = check_device();
+  if (rc) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (rows == 0) {
+    for (float* p : {dgamma_post, dgamma_pre})
+      if (p && cudaMemsetAsync(p, 0, d * sizeof(float), st) != cudaSuccess) return NVFP4B200_ERR_CUDA;
+    if (dgate && cudaMemsetAsync(dgate, 0, groups * d * sizeof(float), st) != cudaSuccess) return NVFP4B200_ERR_CUDA;
+    return NVFP4B200_OK;
+  }
+  const int64_t g = groups ? groups : 1;
+  const norm::Split sp = norm::split_rows(rows, g, d, sm_count_current());
+  int64_t need = 0;
+  nvfp4b200_sandwich_norm_bwd_ws(rows, d, groups, &need);
+  if (ws_floats < need) return NVFP4B200_ERR_BAD_SHAPE;
+  norm::BwdArgs a{dy, dn, b, y, gamma_post, gate, gamma_pre, inv_b, inv_y, dx, db, ws, ws + 2 * sp.ctas * d, dgate, rows, ldb,
+                  ld_dy, ld_dn, ldy, rows / g, sp.rows_per_cta, (int)d, residual_scale, branch_scale};
+  const bool vec = (d * bytes) % 16 == 0 && d % 8 == 0 && vec_ok(dy, ld_dy, bytes) && vec_ok(dn, ld_dn, bytes) &&
+                   vec_ok(b, ldb, bytes) && vec_ok(y, ldy, bytes) && vec_ok(gamma_post, d, bytes) &&
+                   vec_ok(gate, d, bytes) && vec_ok(gamma_pre, d, bytes) && vec_ok(dx, d, bytes) && vec_ok(db, d, bytes);
+  const norm::FinishArgs f{a.part, a.part_gate, gamma_post, dgamma_post, dgamma_pre, dgate, sp.ctas,
+                           sp.parts_per_group, (int)d};
+  return norm::by_type(dtype, vec, [&](auto dt, auto v) {
+    const int r = norm::by_width((int)d, [&](auto tpr) {
+      constexpr int T = decltype(tpr)::value;
+      norm::sandwich_bwd_kernel<decltype(dt)::value, decltype(v)::value, T>
+          <<<(unsigned)sp.ctas, T, 0, st>>>(a, sp.parts_per_group);
+      return launch_status();
+    });
+    if (r) return r;
+    if (!dgamma_post && !dgamma_pre && !dgate) return (int)NVFP4B200_OK;
+    const int64_t jobs = dgate && sp.parts_per_group > 1 ? groups + 2 : 2;
+    norm::sandwich_bwd_finish_kernel<decltype(dt)::value><<<(unsigned)(jobs * ceil_div(d, 32)), 256, 0, st>>>(f);
+    return launch_status();
+  });
+}
+
+}  // extern "C"

@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(256) add_bf16_kernel(const uint16_t* __restric
 
 struct AdamArgs {
   float lr, b1, b2, eps, wd, bc1, bc2, gscale;
+  const float* clip;   // device factor on the gradient, or null
 };
 
 // One AdamW element update on a bf16 parameter, every operation rounded
@@ -282,6 +283,7 @@ __device__ __forceinline__ float adam_one(float p, float g, float& m, float& v, 
 // The scalars lr*wd, lr/bc1 and sqrt(bc2) arrive precomputed (MasterArgs).
 struct MasterArgs {
   float one_minus_lr_wd, one_minus_b1, b2, one_minus_b2, eps, step_size, bc2_sqrt, gscale;
+  const float* clip;   // device factor on the gradient, or null
 };
 
 __device__ __forceinline__ float adam_master_one(float w, float g, float& m, float& v, const MasterArgs& a) {
@@ -329,6 +331,7 @@ template <bool GRAD_F32>
 __global__ void __launch_bounds__(256) adamw_kernel(uint16_t* __restrict__ p, const void* __restrict__ grad,
                                                     float* __restrict__ m, float* __restrict__ v, int64_t n,
                                                     AdamArgs a) {
+  if (a.clip) a.gscale = __fmul_rn(a.gscale, *a.clip);
   const int64_t nv = n / 8;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < nv; i += (int64_t)gridDim.x * blockDim.x) {
     const uint4 pv = reinterpret_cast<const uint4*>(p)[i];
@@ -369,6 +372,7 @@ __global__ void __launch_bounds__(256) adamw_master_kernel(uint16_t* __restrict_
                                                            const void* __restrict__ grad, float* __restrict__ m,
                                                            float* __restrict__ v, int64_t n, MasterArgs a,
                                                            uint32_t* __restrict__ amax_bits) {
+  if (a.clip) a.gscale = __fmul_rn(a.gscale, *a.clip);
   const int64_t nv = n / 8;
   uint32_t am = 0;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < nv; i += (int64_t)gridDim.x * blockDim.x) {
@@ -487,9 +491,10 @@ int nvfp4b200_add_bf16(const void* a, const void* b, void* y, int64_t n, void* s
   return launch_status();
 }
 
-int nvfp4b200_adamw_step(void* param, const void* grad, int grad_dtype, float* m, float* v, int64_t n, float lr,
-                         float beta1, float beta2, float eps, float weight_decay, float bias_corr1, float bias_corr2,
-                         float grad_scale, void* stream) {
+int nvfp4b200_adamw_step_clipped(void* param, const void* grad, int grad_dtype, float* m, float* v, int64_t n, float lr,
+                                 float beta1, float beta2, float eps, float weight_decay, float bias_corr1,
+                                 float bias_corr2, float grad_scale, const float* clip, void* stream) {
+  if (clip && !aligned(clip, 4)) return NVFP4B200_ERR_MISALIGNED;
   if (!param || !grad || !m || !v) return NVFP4B200_ERR_INVALID_ARG;
   if (grad_dtype != NVFP4B200_BF16 && grad_dtype != NVFP4B200_F32) return NVFP4B200_ERR_INVALID_ARG;
   if (n < 0) return NVFP4B200_ERR_BAD_SHAPE;
@@ -497,7 +502,7 @@ int nvfp4b200_adamw_step(void* param, const void* grad, int grad_dtype, float* m
   int rc = check_device();
   if (rc) return rc;
   if (n == 0) return NVFP4B200_OK;
-  AdamArgs a{lr, beta1, beta2, eps, weight_decay, bias_corr1, bias_corr2, grad_scale};
+  AdamArgs a{lr, beta1, beta2, eps, weight_decay, bias_corr1, bias_corr2, grad_scale, clip};
   const unsigned grid = grid_for(n / 8 + 1, 256);
   if (grad_dtype == NVFP4B200_F32)
     adamw_kernel<true><<<grid, 256, 0, (cudaStream_t)stream>>>(static_cast<uint16_t*>(param), grad, m, v, n, a);
@@ -506,10 +511,18 @@ int nvfp4b200_adamw_step(void* param, const void* grad, int grad_dtype, float* m
   return launch_status();
 }
 
-int nvfp4b200_adamw_master_step(void* param, float* master, const void* grad, int grad_dtype, float* m, float* v,
-                                int64_t n, float one_minus_lr_wd, float one_minus_beta1, float beta2,
-                                float one_minus_beta2, float eps, float step_size, float bias_corr2_sqrt,
-                                float grad_scale, uint32_t* amax_bits, void* stream) {
+int nvfp4b200_adamw_step(void* param, const void* grad, int grad_dtype, float* m, float* v, int64_t n, float lr,
+                         float beta1, float beta2, float eps, float weight_decay, float bias_corr1, float bias_corr2,
+                         float grad_scale, void* stream) {
+  return nvfp4b200_adamw_step_clipped(param, grad, grad_dtype, m, v, n, lr, beta1, beta2, eps, weight_decay,
+                                      bias_corr1, bias_corr2, grad_scale, nullptr, stream);
+}
+
+int nvfp4b200_adamw_master_step_clipped(void* param, float* master, const void* grad, int grad_dtype, float* m,
+                                        float* v, int64_t n, float one_minus_lr_wd, float one_minus_beta1, float beta2,
+                                        float one_minus_beta2, float eps, float step_size, float bias_corr2_sqrt,
+                                        float grad_scale, const float* clip, uint32_t* amax_bits, void* stream) {
+  if (clip && !aligned(clip, 4)) return NVFP4B200_ERR_MISALIGNED;
   if (!param || !master || !grad || !m || !v) return NVFP4B200_ERR_INVALID_ARG;
   if (amax_bits && !aligned(amax_bits, 4)) return NVFP4B200_ERR_MISALIGNED;
   if (grad_dtype != NVFP4B200_BF16 && grad_dtype != NVFP4B200_F32) return NVFP4B200_ERR_INVALID_ARG;
@@ -519,7 +532,8 @@ int nvfp4b200_adamw_master_step(void* param, float* master, const void* grad, in
   int rc = check_device();
   if (rc) return rc;
   if (n == 0) return NVFP4B200_OK;
-  MasterArgs a{one_minus_lr_wd, one_minus_beta1, beta2, one_minus_beta2, eps, step_size, bias_corr2_sqrt, grad_scale};
+  MasterArgs a{one_minus_lr_wd, one_minus_beta1, beta2, one_minus_beta2, eps, step_size, bias_corr2_sqrt, grad_scale,
+               clip};
   const unsigned grid = grid_for(n / 8 + 1, 256);
   auto P = static_cast<uint16_t*>(param);
   if (grad_dtype == NVFP4B200_F32)
@@ -527,6 +541,15 @@ int nvfp4b200_adamw_master_step(void* param, float* master, const void* grad, in
   else
     adamw_master_kernel<false><<<grid, 256, 0, (cudaStream_t)stream>>>(P, master, grad, m, v, n, a, amax_bits);
   return launch_status();
+}
+
+int nvfp4b200_adamw_master_step(void* param, float* master, const void* grad, int grad_dtype, float* m, float* v,
+                                int64_t n, float one_minus_lr_wd, float one_minus_beta1, float beta2,
+                                float one_minus_beta2, float eps, float step_size, float bias_corr2_sqrt,
+                                float grad_scale, uint32_t* amax_bits, void* stream) {
+  return nvfp4b200_adamw_master_step_clipped(param, master, grad, grad_dtype, m, v, n, one_minus_lr_wd,
+                                             one_minus_beta1, beta2, one_minus_beta2, eps, step_size, bias_corr2_sqrt,
+                                             grad_scale, nullptr, amax_bits, stream);
 }
 
 int nvfp4b200_global_scale_from_amax(const uint32_t* amax_bits, float* global_scale_out, int64_t n, void* stream) {

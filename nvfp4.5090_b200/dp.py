@@ -140,19 +140,29 @@ class ShardedBucketOptimizer:
         self.rs_works[key] = dist.reduce_scatter_tensor(self.grad_shard[key], grad_full, op=dist.ReduceOp.SUM,
                                                         group=self.pg, async_op=True)
 
+    def wait_grads(self, key: Hashable, timeout_s: Optional[float] = None) -> None:
+        """Make the current stream wait for the bucket's reduce-scatter, so that
+        ``grad_shard[key]`` can be read before ``update`` (e.g. for the global
+        gradient norm, which needs every bucket)."""
+        if key not in self.rs_works:
+            raise RuntimeError(f"bucket {key!r}: no reduce-scatter in flight")
+        w = self.rs_works[key]
+        if w is None:   # waited for already
+            return
+        if timeout_s is None:
+            w.wait()
+        else:
+            w.wait(timeout=datetime.timedelta(seconds=timeout_s))
+        self.rs_works[key] = None
+
     def update(self, key: Hashable, param_full: torch.Tensor, update_fn, timeout_s: Optional[float] = None,
                gather: bool = True) -> None:
         """Wait for the bucket's reduce-scatter and update this rank's shard;
         with ``gather`` also start the all-gather of the updated parameters
         (otherwise call ``gather`` later, e.g. in the order the next forward
         needs the buckets)."""
-        w = self.rs_works.pop(key, None)
-        if w is None:
-            raise RuntimeError(f"bucket {key!r}: no reduce-scatter in flight")
-        if timeout_s is None:
-            w.wait()
-        else:
-            w.wait(timeout=datetime.timedelta(seconds=timeout_s))
+        self.wait_grads(key, timeout_s)
+        del self.rs_works[key]
         if param_full.numel() != self.padded_len(key):
             raise RuntimeError(f"bucket {key!r}: parameters have {param_full.numel()} elements, "
                                f"expected the padded length {self.padded_len(key)}")

@@ -47,6 +47,7 @@ require(hasattr(torch, "float4_e2m1fn_x2"), "Your torch build lacks torch.float4
 require(hasattr(torch, "float8_e4m3fn"), "Your torch build lacks torch.float8_e4m3fn.")
 FP4_DTYPE = torch.float4_e2m1fn_x2
 FP8_SCALE_DTYPE = torch.float8_e4m3fn
+MX_SCALE_DTYPE = torch.float8_e8m0fnu
 
 
 def _flatten(x: torch.Tensor):
@@ -372,8 +373,137 @@ class NVFP4Linear(nn.Module):
         return NVFP4LinearFunction.apply(input, self.weight, self.bias, self.nvfp4_backward)
 
 
+# ============================================================
+# MXFP4 (one UE8M0 scale per 1x32 block; no counterpart in the reference's module)
+# ============================================================
+
+def quant_mxfp4_fused(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """bf16, fp16 or fp32 [..., K] -> (q float4_e2m1fn_x2 [..., K/2], s float8_e8m0fnu
+    [round_up(R,128), round_up(K/32,4)]), K % 32 == 0."""
+    x2, batch, r, k = _flatten(x)
+    q, s = ops.mx_quantize(x2)
+    return q.view(FP4_DTYPE).reshape(*batch, k // 2), s.view(MX_SCALE_DTYPE)
+
+
+@torch.no_grad()
+@torch._dynamo.disable
+def mxfp4mm(A: torch.Tensor, B: torch.Tensor, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Fully dynamic MXFP4 GEMM: C = A @ B^T (A [..., K], B [N, K] in bf16, fp16 or fp32; C bf16 or fp32)."""
+    require(A.is_cuda and B.is_cuda, "mxfp4mm requires CUDA tensors.")
+    require(B.dim() == 2, "B must be a 2-D [N, K] tensor")
+    a2, batch, r, k = _flatten(A)
+    require(k == B.shape[1], f"K mismatch: A has {k}, B has {B.shape[1]}")
+    qa, sa = ops.mx_quantize(a2)
+    qb, sb = ops.mx_quantize(B)
+    return ops.mx_gemm(qa, sa, qb, sb, out_dtype=out_dtype).reshape(*batch, B.shape[0])
+
+
+class MXFP4LinearFunction(torch.autograd.Function):
+    """X @ W^T + bias with MXFP4 operands in forward, dgrad and wgrad, each
+    quantized along its product's contraction dimension; quantization counts
+    as the identity in the backward.  Both orientations of an operand come from
+    one read of it, and what the backward needs of X and W is kept in MXFP4
+    (17/32 byte per element)."""
+
+    @staticmethod
+    def forward(ctx, input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
+        require(input.is_cuda and input.dtype in (torch.bfloat16, torch.float32),
+                "mxfp4_linear expects a CUDA bf16 or fp32 input.")
+        n, k = weight.shape
+        require(input.shape[-1] == k, f"K mismatch: input has {input.shape[-1]}, weight has {k}")
+        x = input.reshape(-1, k)
+        t = x.shape[0]
+        need_x, need_w = ctx.needs_input_grad[:2]
+        require(not (need_x or need_w) or n % 32 == 0, "training needs out_features divisible by 32")
+        qxt = sxt = qwt = swt = None
+        if need_w:
+            qx, sx, qxt, sxt = ops.mx_quantize_both(x)
+        else:
+            qx, sx = ops.mx_quantize(x)
+        if need_x:
+            qw, sw, qwt, swt = ops.mx_quantize_both(weight)
+        else:
+            qw, sw = ops.mx_quantize(weight)
+        y = ops.mx_gemm(qx, sx, qw, sw, bias=None if bias is None else bias.to(torch.bfloat16), out_dtype=input.dtype)
+        ctx.save_for_backward(qxt, sxt, qwt, swt)
+        ctx.shape, ctx.tokens, ctx.wdtype = input.shape, t, weight.dtype
+        ctx.bdtype = None if bias is None else bias.dtype
+        # not a view, so that users may change the result in place
+        return torch.ops.aten._unsafe_view(y, [*input.shape[:-1], n])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_output: torch.Tensor):
+        qxt, sxt, qwt, swt = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[:2]
+        dy = grad_output.reshape(-1, grad_output.shape[-1])
+        n, k = dy.shape[1], ctx.shape[-1]
+        dx = dw = db = qd = qdt = None
+        if need_x and need_w:
+            qd, sd, qdt, sdt = ops.mx_quantize_both(dy)
+        elif need_x:
+            qd, sd = ops.mx_quantize(dy)
+        elif need_w:
+            qdt, sdt = ops.mx_quantize_t(dy)
+        if need_x:
+            dx = ops.mx_gemm(qd, sd, qwt, swt, out_dtype=grad_output.dtype).reshape(ctx.shape)
+        if need_w:
+            out_dtype = torch.float32 if ctx.wdtype == torch.float32 else torch.bfloat16
+            if ctx.tokens:
+                dw = ops.mx_gemm(qdt, sdt, qxt, sxt, out_dtype=out_dtype).to(ctx.wdtype)
+            else:
+                dw = torch.zeros((n, k), device=dy.device, dtype=ctx.wdtype)
+        if ctx.bdtype is not None and ctx.needs_input_grad[2]:
+            db = dy.sum(dim=0, dtype=torch.float32).to(ctx.bdtype)
+        return dx, dw, db
+
+
+def mxfp4_linear(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """input [..., K] @ weight [N, K]^T + bias with MXFP4 products, differentiable in all three."""
+    return MXFP4LinearFunction.apply(input, weight, bias)
+
+
+class MXFP4Linear(NVFP4Linear):
+    """torch.nn.Linear with MXFP4 products in forward, dgrad and wgrad.
+
+    ``freeze()`` quantizes the weight once and drops into the serving form
+    (``ops.mx_linear``: bf16 inputs, no gradients; the weight is not read again
+    until ``thaw()``, a move or a loaded state, after which the layer is no
+    longer frozen); without it every call quantizes the current weight."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=torch.bfloat16):
+        super().__init__(in_features, out_features, bias, device, dtype)
+        self._held = None
+
+    def freeze(self) -> "MXFP4Linear":
+        with torch.no_grad():
+            bias = None if self.bias is None else self.bias.detach().to(torch.bfloat16, copy=True)
+            self._held = (*ops.mx_quantize(self.weight.detach()), bias)
+        return self
+
+    def thaw(self) -> "MXFP4Linear":
+        self._held = None
+        return self
+
+    def _apply(self, fn, recurse=True):
+        self._held = None
+        return super()._apply(fn, recurse)
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        self._held = None
+        return super()._load_from_state_dict(*args, **kwargs)
+
+    def forward(self, input: torch.Tensor) -> torch.Tensor:
+        if self._held is not None:
+            require(not (torch.is_grad_enabled() and input.requires_grad),
+                    "a frozen MXFP4Linear has no gradients: thaw() it, or call it under torch.no_grad()")
+            return ops.mx_linear(input, *self._held)
+        return mxfp4_linear(input, self.weight, self.bias)
+
+
 __all__ = ["round_up", "require", "FP4_DTYPE", "FP8_SCALE_DTYPE", "quant_nvfp4_fused",
            "rmsnorm_quant_nvfp4_fused", "nvfp4mm_torch", "nvfp4mm", "nvfp4mm_relu", "nvfp4mm_relu_2",
            "test_accuracy", "_bytes_nvfp4_quant_fused", "bench_quant_gbps", "bench_gemm_tflops",
            "NVFP4LinearFunction", "NVFP4Linear", "cutlass_nvfp4_mm", "cutlass_nvfp4_mm_relu",
-           "cutlass_nvfp4_mm_relu_2"]
+           "cutlass_nvfp4_mm_relu_2", "MX_SCALE_DTYPE", "quant_mxfp4_fused", "mxfp4mm", "MXFP4LinearFunction",
+           "mxfp4_linear", "MXFP4Linear"]

@@ -86,14 +86,28 @@ class Saved:
     gu: torch.Tensor
     h: torch.Tensor
     g_h: torch.Tensor
+    b: Optional[torch.Tensor] = None        # with a post-norm: the block's output before it
+    inv_b: Optional[torch.Tensor] = None
+
+
+@dataclass
+class PostNorm:
+    """What ends a block in place of the plain residual add:
+    y = residual_scale * x + branch_scale * gate * (b * inv_rms(b) * gamma),
+    with a gate [D] or [G, D] (one row per G-th of the tokens) or none."""
+    gamma: Optional[torch.Tensor] = None
+    gate: Optional[torch.Tensor] = None
+    residual_scale: float = 1.0
+    branch_scale: float = 1.0
 
 
 def block_forward(x: torch.Tensor, gamma: torch.Tensor, qw: QWeights, eps: float = 1e-6, save: bool = True,
-                  interleave: int = 0):
+                  interleave: int = 0, post: Optional[PostNorm] = None):
     """One RMSNorm+SwiGLU block on bf16 x [T, D] -> (y [T, D], saved activations).
 
     ``interleave=128``: W_gu rows alternate gate/up in blocks of 128 and the
-    gate/up GEMM computes h in its epilogue."""
+    gate/up GEMM computes h in its epilogue.  ``post``: a norm, gate and scales
+    between the block's output and the residual stream."""
     inv_rms, g_xn = ops.rmsnorm_stats(x, eps, gamma=gamma)
     q_xn, s_xn = ops.quantize(x, global_scale=g_xn, row_scale=inv_rms, gamma=gamma)
     if interleave:
@@ -104,9 +118,13 @@ def block_forward(x: torch.Tensor, gamma: torch.Tensor, qw: QWeights, eps: float
         del q_xn, s_xn
         h, g_h = ops.swiglu_fwd(gu, with_scale=True)
     q_h, s_h = ops.quantize(h, global_scale=g_h)
-    y = ops.gemm(q_h, s_h, qw.q_down, qw.s_down, scale_a=g_h, scale_b=qw.g_down, residual=x)
-    saved = Saved(x, inv_rms, g_xn, gu, h, g_h) if save else None
-    return y, saved
+    if post is None:
+        y = ops.gemm(q_h, s_h, qw.q_down, qw.s_down, scale_a=g_h, scale_b=qw.g_down, residual=x)
+        return y, Saved(x, inv_rms, g_xn, gu, h, g_h) if save else None
+    b = ops.gemm(q_h, s_h, qw.q_down, qw.s_down, scale_a=g_h, scale_b=qw.g_down)
+    y, _, inv_b, _ = ops.sandwich_norm(b, x, post.gamma, post.gate, residual_scale=post.residual_scale,
+                                       branch_scale=post.branch_scale, eps=eps)
+    return y, Saved(x, inv_rms, g_xn, gu, h, g_h, b, inv_b) if save else None
 
 
 def _wgrad(qa, sa, qb, sb, ga, gb, out: torch.Tensor, accumulate: bool) -> None:
@@ -125,7 +143,8 @@ def _wgrad(qa, sa, qb, sb, ga, gb, out: torch.Tensor, accumulate: bool) -> None:
 
 def block_backward(dy: torch.Tensor, gamma: torch.Tensor, qw: QWeights, sv: Saved,
                    grad_gamma: torch.Tensor, grad_gu: torch.Tensor, grad_down: torch.Tensor,
-                   accumulate: bool, interleave: int = 0, keep: Optional[dict] = None) -> torch.Tensor:
+                   accumulate: bool, interleave: int = 0, keep: Optional[dict] = None,
+                   post: Optional[PostNorm] = None, grad_post: Optional[dict] = None) -> torch.Tensor:
     """Backward of block_forward given dy [T, D].
 
     grad_gamma (fp32 [D]) is accumulated; grad_gu ([2F, D]) and grad_down
@@ -133,7 +152,16 @@ def block_backward(dy: torch.Tensor, gamma: torch.Tensor, qw: QWeights, sv: Save
     grad_gu / grad_down may also be [pieces, rows / pieces, cols] row-block
     views (see _wgrad).  Returns dx [T, D] (including the residual path).  ``keep`` (a dict)
     receives the intermediates dgu, dxn and the global scales g_dy, g_dgu,
-    for inspection; normally they are freed as soon as they are consumed."""
+    for inspection; normally they are freed as soon as they are consumed.
+    With ``post`` (as the forward had it) ``grad_post`` receives the fp32
+    gradients gamma [D] and gate [G, D] of its parameters."""
+    dres = dy
+    if post is not None:
+        g = ops.sandwich_norm_bwd(dy, sv.b, sv.inv_b, post.gamma, post.gate, residual_scale=post.residual_scale,
+                                  branch_scale=post.branch_scale)
+        dres, dy = g["dx"], g["db"]
+        if grad_post is not None:
+            grad_post.update(gamma=g["dgamma_post"], gate=g["dgate"])
     g_dy = ops.global_scale(dy)
     q_dy, s_dy = ops.quantize(dy, global_scale=g_dy)
     # interleaved gate/up with whole 256-column dh tiles: the SwiGLU backward
@@ -163,8 +191,51 @@ def block_backward(dy: torch.Tensor, gamma: torch.Tensor, qw: QWeights, sv: Save
     q_xnt, s_xnt = ops.quantize_t(sv.x, global_scale=sv.g_xn, row_scale=sv.inv_rms, gamma=gamma)
     _wgrad(q_dgut, s_dgut, q_xnt, s_xnt, g_dgu, sv.g_xn, grad_gu, accumulate)
     del q_dgut, s_dgut, q_xnt, s_xnt
-    dx = ops.rmsnorm_bwd(sv.x, gamma, sv.inv_rms, dxn, dres=dy, dgamma_acc=grad_gamma)
+    dx = ops.rmsnorm_bwd(sv.x, gamma, sv.inv_rms, dxn, dres=dres, dgamma_acc=grad_gamma)
     return dx
+
+
+class SandwichNormFunction(torch.autograd.Function):
+    """``ops.sandwich_norm`` with gradients in b, x, gamma_post, gate and gamma_pre."""
+
+    @staticmethod
+    def forward(ctx, b, x, gamma_post, gate, gamma_pre, residual_scale, branch_scale, eps, pre):
+        d = b.shape[-1]
+        b2 = b.reshape(-1, d)
+        y, n, inv_b, inv_y = ops.sandwich_norm(b2, x.reshape(-1, d), gamma_post, gate, gamma_pre,
+                                               residual_scale=residual_scale, branch_scale=branch_scale, eps=eps,
+                                               pre=pre)
+        ctx.save_for_backward(b2, y if n is not None else None, inv_b, inv_y, gamma_post, gate, gamma_pre)
+        ctx.scales, ctx.shape = (residual_scale, branch_scale), b.shape
+        ctx.set_materialize_grads(False)
+        if b.dim() != 2:   # not views, so that users may change the results in place
+            y, n = (None if t is None else torch.ops.aten._unsafe_view(t, b.shape) for t in (y, n))
+        return y if n is None else (y, n)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dn=None):
+        if dy is None and dn is None:
+            return (None,) * 9
+        b, y, inv_b, inv_y, gamma_post, gate, gamma_pre = ctx.saved_tensors
+        flat = lambda t: None if t is None else t.reshape(b.shape)
+        more = dict(dn=flat(dn), y=y, inv_y=inv_y, gamma_pre=gamma_pre) if dn is not None else {}
+        g = ops.sandwich_norm_bwd(flat(dy), b, inv_b, gamma_post, gate, residual_scale=ctx.scales[0],
+                                  branch_scale=ctx.scales[1], **more)
+        like = lambda v, p: None if p is None or v is None else v.reshape(p.shape).to(p.dtype)
+        return (g["db"].view(ctx.shape), g["dx"].view(ctx.shape), like(g["dgamma_post"], gamma_post),
+                like(g["dgate"], gate), like(g["dgamma_pre"], gamma_pre), None, None, None, None)
+
+
+def sandwich_norm(b: torch.Tensor, x: torch.Tensor, gamma_post: Optional[torch.Tensor] = None,
+                  gate: Optional[torch.Tensor] = None, gamma_pre: Optional[torch.Tensor] = None, *,
+                  residual_scale: float = 1.0, branch_scale: float = 1.0, eps: float = 1e-6,
+                  pre: Optional[bool] = None):
+    """Differentiable ``ops.sandwich_norm`` on b, x [..., D]: y, or (y, n) when the
+    next block's pre-norm is asked for (``gamma_pre`` given or ``pre=True``).
+    A gate of shape [B, D] (or [B, 1, D]) goes with x of shape [B, S, D]."""
+    return SandwichNormFunction.apply(b, x, gamma_post, gate, gamma_pre, float(residual_scale), float(branch_scale),
+                                      float(eps), pre)
 
 
 # ----------------------------------------------------------------------------
@@ -173,35 +244,52 @@ def block_backward(dy: torch.Tensor, gamma: torch.Tensor, qw: QWeights, sv: Save
 
 class NVFP4SwiGLUFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gamma, w_gu, w_down, eps):
+    def forward(ctx, x, gamma, w_gu, w_down, eps, post_gamma=None, gate=None, scales=None):
         shape = x.shape
         x2 = x.reshape(-1, shape[-1]).contiguous()
         qw = quantize_weights(w_gu, w_down, need_t=True)
-        y, sv = block_forward(x2, gamma, qw, eps)
+        post = None if scales is None else PostNorm(post_gamma, gate, *scales)
+        y, sv = block_forward(x2, gamma, qw, eps, post=post)
         ctx.qw, ctx.sv = qw, sv
-        ctx.save_for_backward(gamma)
-        ctx.shape = shape
+        ctx.save_for_backward(gamma, post_gamma, gate)
+        ctx.shape, ctx.scales = shape, scales
         return y.reshape(shape)
 
     @staticmethod
     def backward(ctx, dy):
-        (gamma,) = ctx.saved_tensors
+        gamma, post_gamma, gate = ctx.saved_tensors
+        post = None if ctx.scales is None else PostNorm(post_gamma, gate, *ctx.scales)
+        grad_post = {}
         dy2 = dy.reshape(-1, ctx.shape[-1]).contiguous().to(torch.bfloat16)
         d = gamma.numel()
         grad_gamma = torch.zeros(d, device=dy.device, dtype=torch.float32)
         grad_gu = torch.empty((ctx.sv.gu.shape[1], d), device=dy.device, dtype=torch.bfloat16)
         grad_down = torch.empty((d, ctx.sv.h.shape[1]), device=dy.device, dtype=torch.bfloat16)
-        dx = block_backward(dy2, gamma, ctx.qw, ctx.sv, grad_gamma, grad_gu, grad_down, accumulate=False)
+        dx = block_backward(dy2, gamma, ctx.qw, ctx.sv, grad_gamma, grad_gu, grad_down, accumulate=False, post=post,
+                            grad_post=grad_post)
         ctx.qw = ctx.sv = None
-        return dx.reshape(ctx.shape), grad_gamma.to(gamma.dtype), grad_gu, grad_down, None
+        like = lambda v, p: None if p is None or v is None else v.reshape(p.shape).to(p.dtype)
+        return (dx.reshape(ctx.shape), grad_gamma.to(gamma.dtype), grad_gu, grad_down, None,
+                like(grad_post.get("gamma"), post_gamma), like(grad_post.get("gate"), gate), None)
 
 
 class NVFP4SwiGLUMLP(nn.Module):
-    """Pre-norm residual SwiGLU MLP block with NVFP4 GEMMs in forward and backward."""
+    """Pre-norm residual SwiGLU MLP block with NVFP4 GEMMs in forward and backward.
+
+    ``post_norm`` adds a norm after the block, to which a learned channel
+    ``gate`` and the two scales belong: the block then ends in
+    y = residual_scale * x + branch_scale * gate * (b * inv_rms(b) * post_gamma)
+    (``sandwich_norm``) instead of y = x + b."""
 
     def __init__(self, d_model: int, d_ff: int, eps: float = 1e-6, device=None, dtype=torch.bfloat16,
-                 init_std: float = 0.02):
+                 init_std: float = 0.02, post_norm: bool = False, gate: bool = False, residual_scale: float = 1.0,
+                 branch_scale: float = 1.0):
         super().__init__()
+        if not post_norm and (gate or residual_scale != 1.0 or branch_scale != 1.0):
+            raise ValueError("gate and scales belong to the post-norm: pass post_norm=True")
+        ones = lambda on: nn.Parameter(torch.ones(d_model, device=device, dtype=dtype)) if on else None
+        self.post_gamma, self.gate = ones(post_norm), ones(gate)
+        self.scales = (float(residual_scale), float(branch_scale)) if post_norm else None
         self.d_model, self.d_ff, self.eps = d_model, d_ff, eps
         self.gamma = nn.Parameter(torch.ones(d_model, device=device, dtype=dtype))
         self.w_gu = nn.Parameter(torch.empty(2 * d_ff, d_model, device=device, dtype=dtype))
@@ -211,7 +299,8 @@ class NVFP4SwiGLUMLP(nn.Module):
             self.w_down.normal_(0.0, init_std)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return NVFP4SwiGLUFunction.apply(x, self.gamma, self.w_gu, self.w_down, self.eps)
+        return NVFP4SwiGLUFunction.apply(x, self.gamma, self.w_gu, self.w_down, self.eps, self.post_gamma, self.gate,
+                                         self.scales)
 
 
 # ----------------------------------------------------------------------------
@@ -225,13 +314,16 @@ class AdamConfig:
     AdamW updates the master and the bf16 parameter is its round-to-nearest
     copy, so steps smaller than half a bf16 ulp of a weight (lr = 1e-4 against
     |w| > ~0.05) still move it over time.  Without it the update is applied
-    to the bf16 parameter directly and such steps are lost."""
+    to the bf16 parameter directly and such steps are lost.  ``max_grad_norm``
+    clips the global norm of all blocks' gradients (the mean over ranks) before
+    the update; the norm found is the trainer's ``grad_norm``."""
     lr: float = 1e-4
     beta1: float = 0.9
     beta2: float = 0.95
     eps: float = 1e-8
     weight_decay: float = 0.0
     master_weights: bool = True
+    max_grad_norm: Optional[float] = None
 
 
 class ShardQuantLayout:
@@ -502,6 +594,8 @@ class NVFP4MLPStackTrainer:
             if world > 1:
                 self.reducer = BucketAllReducer(process_group)
         self.step_count = 0
+        # with max_grad_norm: the last step's gradient norm before clipping (1-element fp32 tensor)
+        self.grad_norm: Optional[torch.Tensor] = None
         # the weights' global scales for the next step, from the amaxes the AdamW
         # update records while writing the weights ([block, (W_gu, W_down)]); None
         # until the first update (then they are computed from the weights)
@@ -600,10 +694,11 @@ class NVFP4MLPStackTrainer:
                         self.reducer.launch(bi, b.grad)
         self.step_count += 1
         a = self.adam
+        clip = None if a.max_grad_norm is None else self._clip_coef(a.max_grad_norm, n_micro)
 
         def adamw(p, g, m, v, w=None, amax=None):
             kw = dict(lr=a.lr, beta1=a.beta1, beta2=a.beta2, eps=a.eps, weight_decay=a.weight_decay,
-                      step=self.step_count, grad_scale=1.0 / self.world)
+                      step=self.step_count, grad_scale=1.0 / self.world, clip=clip)
             if w is not None:
                 ops.adamw_master_step(p, w, g, m, v, amax_bits=amax, **kw)
             else:
@@ -678,6 +773,28 @@ class NVFP4MLPStackTrainer:
                 for bi in reversed(range(self.n_blocks)):
                     self.gathered[bi].gather_transposed(self.opt.rank, self.pg)
         return out_sum
+
+    def _clip_coef(self, max_norm: float, n_micro: int) -> torch.Tensor:
+        """Waits for every block's exchanged gradient and returns the factor that
+        clips their global norm; AdamW multiplies it in, so the gradients are
+        read once more (by the norm) but not written.  Sets ``grad_norm``."""
+        scale = 1.0 / self.world
+        if self.opt is not None:   # each rank holds a shard: sum the ranks' sums of squares
+            import torch.distributed as dist
+            for bi in reversed(range(self.n_blocks)):
+                self.opt.wait_grads(bi)
+            total = ops.grad_norm_total([self.opt.grad_shard[bi] for bi in range(self.n_blocks)])
+            dist.all_reduce(total, op=dist.ReduceOp.SUM, group=self.pg)
+            self.grad_norm, coef = ops.grad_norm_finish(total, max_norm, grad_scale=scale)
+            return coef
+        if self.reducer is not None:
+            self.reducer.wait_all()
+        if self.world == 1 and n_micro > 1:
+            grads = [g for b in self.blocks for g in (b.grad_gamma32, b.acc_gu, b.acc_down)]
+        else:
+            grads = [b.grad for b in self.blocks]
+        self.grad_norm, coef = ops.grad_norm_coef(grads, max_norm, grad_scale=scale)
+        return coef
 
     def _shard_amax(self) -> None:
         """w_amax from this rank's rows of every weight (rank-major buckets)."""

@@ -9,8 +9,9 @@ system).  Packed E2M1 tensors are returned as ``uint8``; the
 """
 from __future__ import annotations
 
+import array
 import math
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -18,6 +19,7 @@ from . import _lib
 
 EPI_NONE, EPI_RELU, EPI_RELU2 = 0, 1, 2
 _DT_BF16, _DT_F32 = 0, 1
+_DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 
 
 def round_up(x: int, m: int) -> int:
@@ -53,6 +55,15 @@ def _scalar_f32(g: Optional[torch.Tensor], device) -> Optional[torch.Tensor]:
              "global scales are 1-element float32 CUDA tensors")
     _require(g.device == device, "global scale on a different device")
     return g
+
+
+def _run(t: torch.Tensor, name: str, *args) -> None:
+    """Call an entry point on the device of ``t`` and that device's current stream."""
+    if t.device.index == torch.cuda.current_device():
+        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(t.device):
+            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
 
 
 _WS = {}
@@ -260,6 +271,369 @@ def gemm(qa: torch.Tensor, sa: torch.Tensor, qb: torch.Tensor, sb: torch.Tensor,
 
 
 # ----------------------------------------------------------------------------
+# MXFP4: quantizers, the way back, products
+# ----------------------------------------------------------------------------
+
+
+def _float_matrix(x: torch.Tensor, what: str) -> torch.Tensor:
+    """x as the MXFP4 quantizers read it: 2-D, unit column stride, 16-byte
+    aligned rows; copied when it is laid out otherwise."""
+    _require(x.is_cuda and x.dtype in _DTYPES, f"{what} expects a CUDA bf16, fp16 or fp32 tensor")
+    _require(x.dim() == 2, f"{what} expects a 2-D tensor")
+    if x.stride(1) == 1 and x.stride(0) >= x.shape[1] and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _mx_factors(x: torch.Tensor, row_scale, gamma):
+    r, c = x.shape
+    if row_scale is not None:
+        _require(row_scale.dtype == torch.float32 and row_scale.numel() == r and row_scale.device == x.device,
+                 "row_scale is float32 [R] on the input's device")
+        row_scale = row_scale.contiguous()
+    if gamma is not None:
+        _check_bf16(gamma, "gamma")
+        _require(gamma.numel() == c and gamma.device == x.device, "gamma is bf16 [K] on the input's device")
+        gamma = gamma.contiguous()
+        if gamma.data_ptr() % 16:
+            gamma = gamma.clone()
+    return row_scale, gamma
+
+
+def _mx_quant(x, row_scale, gamma, rows: bool, cols: bool, out, what: str):
+    x = _float_matrix(x, what)
+    r, c = x.shape
+    _require(not rows or c % 32 == 0, "K must be divisible by 32 for MXFP4 1x32 scaling.")
+    _require(c > 0 and c % 8 == 0, f"{what} needs columns divisible by 8")
+    row_scale, gamma = _mx_factors(x, row_scale, gamma)
+    q = s = qt = st = None
+    if rows:
+        q, s = _outputs(out, (r, c // 2), mx_scale_shape(r, c), x.device)
+    if cols:
+        pr = round_up(r, 32)
+        qt, st = _outputs(None if rows else out, (c, pr // 2), mx_scale_shape(c, pr), x.device)
+    if r:
+        _run(x, "nvfp4b200_mx_quant", x.data_ptr(), _DTYPES[x.dtype], _ptr(row_scale), _ptr(gamma), _ptr(q), _ptr(s),
+             _ptr(qt), _ptr(st), r, c, max(x.stride(0), c))
+    return q, s, qt, st
+
+
+def mx_quantize(x: torch.Tensor, row_scale: Optional[torch.Tensor] = None, gamma: Optional[torch.Tensor] = None,
+                out=None):
+    """MXFP4-quantize x [R, K] (bf16, fp16 or fp32; K % 32 == 0) along K ->
+    (q u8 [R, K/2], s u8 swizzled ``mx_scale_shape(R, K)``).
+
+    Blocks of 32 share the power of two 2^(floor(log2 amax) - 2); elements are
+    rounded to nearest even and saturate at 6 times it.  ``row_scale`` (fp32
+    [R]) and ``gamma`` (bf16 [K]) are multiplied in first; a block with an
+    infinity or a NaN becomes NaN as a whole.  ``out=(q, s)`` writes into given
+    tensors of those shapes."""
+    return _mx_quant(x, row_scale, gamma, True, False, out, "mx_quantize")[:2]
+
+
+def mx_quantize_t(x: torch.Tensor, row_scale: Optional[torch.Tensor] = None, gamma: Optional[torch.Tensor] = None,
+                  out=None):
+    """MXFP4-quantize x^T (x [R, C], C % 8 == 0) along R -> (q u8 [C, P/2], s
+    swizzled for (C, P)), P = R rounded up to 32: the rows past the last count
+    as zeros, so a product over P is the product over R."""
+    return _mx_quant(x, row_scale, gamma, False, True, out, "mx_quantize_t")[2:]
+
+
+def mx_quantize_both(x: torch.Tensor, row_scale: Optional[torch.Tensor] = None, gamma: Optional[torch.Tensor] = None):
+    """Both orientations of x [R, K] from one read: the pairs of ``mx_quantize``
+    and ``mx_quantize_t`` as (q, s, qt, st)."""
+    return _mx_quant(x, row_scale, gamma, True, True, None, "mx_quantize_both")
+
+
+def mx_dequantize(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values [R, K] (bf16 or fp32) that an MXFP4 matrix stands for."""
+    _require(q.is_cuda and q.dtype == torch.uint8 and q.dim() == 2, "mx_dequantize expects packed uint8 [R, K/2]")
+    r, k = q.shape[0], 2 * q.shape[1]
+    _require(k % 32 == 0, "K must be divisible by 32 for MXFP4 1x32 scaling.")
+    _require(dtype in (torch.bfloat16, torch.float32), "output dtype must be bf16 or fp32")
+    _require(s.device == q.device and s.element_size() == 1 and s.numel() == math.prod(mx_scale_shape(r, k)),
+             "MXFP4 scale tensors must be the padded swizzled [round_up(rows,128), round_up(k/32,4)] layout")
+    q, s = q.contiguous(), s.contiguous()
+    y = torch.empty((r, k), device=q.device, dtype=dtype)
+    if r and k:
+        _run(q, "nvfp4b200_mx_dequant", q.data_ptr(), s.data_ptr(), y.data_ptr(), _DTYPES[dtype], r, k)
+    return y
+
+
+def mx_gemm(qa: torch.Tensor, sa: torch.Tensor, qb: torch.Tensor, sb: torch.Tensor, *,
+            bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+            out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16, accumulate: bool = False,
+            epilogue: int = EPI_NONE) -> torch.Tensor:
+    """D[m, n] = epilogue(A.B^T + bias) + residual on packed MXFP4 operands:
+    ``gemm`` for 1x32 blocks with UE8M0 scales.
+
+    qa: [m, k/2], qb: [n, k/2] packed bytes; fp32 outputs can accumulate."""
+    _require(qa.is_cuda and all(t.device == qa.device for t in (sa, qb, sb)), "mx_gemm requires CUDA tensors of one device")
+    m, kh = qa.shape
+    n, kh2 = qb.shape
+    _require(kh == kh2, f"K mismatch: A has {2 * kh}, B has {2 * kh2}")
+    k = 2 * kh
+    _require(k > 0 and k % 32 == 0, "K must be divisible by 32 for MXFP4 1x32 scaling.")
+    _require(qa.is_contiguous() and qb.is_contiguous() and sa.is_contiguous() and sb.is_contiguous(),
+             "gemm operands must be contiguous")
+    _require(sa.numel() == math.prod(mx_scale_shape(m, k)) and sb.numel() == math.prod(mx_scale_shape(n, k)),
+             "MXFP4 scale tensors must be the padded swizzled [round_up(rows,128), round_up(k/32,4)] layout")
+    if out is None:
+        _require(not accumulate, "accumulate needs an existing output")
+        out = torch.empty((m, n), device=qa.device, dtype=out_dtype)
+    _require(out.dtype in (torch.bfloat16, torch.float32) and out.device == qa.device, "output dtype must be bf16 or fp32")
+    _require(out.dim() == 2 and out.shape == (m, n) and out.stride(1) == 1, "output must be [m, n] with unit column stride")
+    _require(not accumulate or out.dtype == torch.float32, "accumulate needs an fp32 output")
+    if bias is not None:
+        _check_bf16(bias, "bias")
+        _require(bias.numel() == n and bias.device == qa.device, "bias is bf16 [n]")
+        bias = bias.contiguous()
+    if residual is not None:
+        _check_bf16(residual, "residual")
+        _require(out.dtype == torch.bfloat16 and residual.shape == (m, n) and residual.stride() == out.stride(),
+                 "residual must match a bf16 output's layout")
+    if m == 0 or n == 0:
+        return out
+    _run(qa, "nvfp4b200_mx_gemm", qa.data_ptr(), qb.data_ptr(), sa.data_ptr(), sb.data_ptr(), _ptr(bias),
+         _ptr(residual), out.data_ptr(), _DTYPES[out.dtype], int(bool(accumulate)), int(epilogue), m, n, k,
+         out.stride(0))
+    return out
+
+
+def mx_linear(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y = x . W^T + bias with W held in MXFP4 (qw [n, k/2], sw; ``mx_quantize``):
+    x bf16 [..., k] is quantized along k, y is bf16 [..., n].  n % 8 == 0."""
+    _check_bf16(x, "mx_linear")
+    n, k = qw.shape[0], 2 * qw.shape[1]
+    _require(x.shape[-1] == k, f"K mismatch: x has {x.shape[-1]}, W has {k}")
+    x2 = x.reshape(-1, k)
+    if x2.shape[0] == 0:
+        return torch.empty((*x.shape[:-1], n), device=x.device, dtype=x.dtype)
+    q, s = mx_quantize(x2)
+    return mx_gemm(q, s, qw, sw, bias=bias).reshape(*x.shape[:-1], n)
+
+
+# ----------------------------------------------------------------------------
+# global gradient norm and clipping
+# ----------------------------------------------------------------------------
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Every element once in one stretch of memory, in whatever order of dimensions."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if st != expect:
+            return False
+        expect *= n
+    return True
+
+
+def _grad_call(grads, outs, norm_type, grad_scale, max_norm, want):
+    """Run nvfp4b200_grad_norm; ``want`` names the outputs: n(orm), c(oef), t(otal)."""
+    if isinstance(grads, torch.Tensor):
+        grads = (grads,)
+    grads = list(grads)
+    _require(norm_type == 2 or norm_type == math.inf, "norm_type must be 2 or inf")
+    max_norm = float(max_norm)
+    _require(max_norm >= 0.0, "max_norm must not be negative")
+    dev = grads[0].device if grads else torch.device("cuda", torch.cuda.current_device())
+    for t in grads:
+        _require(t.is_cuda and t.device == dev and t.dtype in _DTYPES, "gradients are bf16, fp16 or fp32 CUDA tensors of one device")
+        _require(t.is_contiguous() or _dense(t), "gradients must be dense: every element once in one stretch of memory")
+    count = len(grads)
+    ptrs = array.array("Q", [t.data_ptr() for t in grads])
+    dts = array.array("i", [_DTYPES[t.dtype] for t in grads])
+    lens = array.array("q", [t.numel() for t in grads])
+    outp = outd = None
+    if outs is not None:
+        outs = [outs] if isinstance(outs, torch.Tensor) else list(outs)
+        _require(len(outs) == count, "out must hold one tensor per gradient")
+        for t, o in zip(grads, outs):
+            _require(o.device == dev and o.dtype in _DTYPES and o.shape == t.shape
+                     and (o.stride() == t.stride() or (o.is_contiguous() and t.is_contiguous())),
+                     "out tensors match their gradient's shape and layout (bf16, fp16 or fp32)")
+        outp = array.array("Q", [t.data_ptr() for t in outs])
+        outd = array.array("i", [_DTYPES[t.dtype] for t in outs])
+    ws = torch.empty(1024 * (1 + count // 112), device=dev, dtype=torch.float64)
+    # the results in one allocation: fp32 norm, fp32 coefficient, fp64 total
+    res = torch.empty(4, device=dev, dtype=torch.float32)
+    base = res.data_ptr()
+    addr = lambda a: None if a is None else a.buffer_info()[0]
+    _run(res, "nvfp4b200_grad_norm", addr(ptrs), addr(dts), addr(outp), addr(outd), addr(lens), count,
+         2 if norm_type == 2 else 0, float(grad_scale), max_norm, ws.data_ptr(), ws.numel(),
+         base if "n" in want else None, base + 4 if "c" in want else None, base + 8 if "t" in want else None)
+    return res
+
+
+def grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], norm_type: float = 2.0,
+              grad_scale: float = 1.0) -> torch.Tensor:
+    """Norm of all gradients together (2 or inf), of grad * grad_scale, as a
+    1-element fp32 tensor.  The list may mix bf16, fp16 and fp32 and hold empty
+    tensors; the sum is carried in fp64 and does not depend on timing."""
+    return _grad_call(grads, None, norm_type, grad_scale, math.inf, "n")[:1]
+
+
+def grad_norm_coef(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
+                   grad_scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(norm, coef) with coef = min(1, max_norm / (norm + 1e-6)), both 1-element
+    fp32 tensors: hand coef to ``adamw_step`` / ``adamw_master_step`` as
+    ``clip`` and the gradients are clipped without a pass of their own."""
+    res = _grad_call(grads, None, norm_type, grad_scale, max_norm, "nc")
+    return res[:1], res[1:2]
+
+
+def grad_norm_total(grads: Union[torch.Tensor, Sequence[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
+    """The sum of squares (or the largest magnitude) as a 1-element fp64 tensor:
+    what a rank holding a shard of the gradients sends to a sum (maximum) over
+    the ranks before ``grad_norm_finish``."""
+    return _grad_call(grads, None, norm_type, 1.0, math.inf, "t")[2:].view(torch.float64)
+
+
+def grad_norm_finish(totals: torch.Tensor, max_norm: float, norm_type: float = 2.0,
+                     grad_scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(norm, coef) from one or more ``grad_norm_total`` values."""
+    _require(totals.is_cuda and totals.dtype == torch.float64 and totals.is_contiguous(),
+             "totals are a contiguous float64 CUDA tensor")
+    _require(norm_type == 2 or norm_type == math.inf, "norm_type must be 2 or inf")
+    res = torch.empty(2, device=totals.device, dtype=torch.float32)
+    _run(totals, "nvfp4b200_grad_norm_finish", totals.data_ptr(), totals.numel(), 2 if norm_type == 2 else 0,
+         float(grad_scale), float(max_norm), res.data_ptr(), res.data_ptr() + 4)
+    return res[:1], res[1:]
+
+
+def clip_grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
+                   grad_scale: float = 1.0, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
+    """Clip the gradients' global norm to ``max_norm`` and return the norm before
+    clipping (1-element fp32; of grad * grad_scale).
+
+    out_i = grad_i * grad_scale * min(1, max_norm / (norm + 1e-6)), written in
+    place or into ``out`` (same shapes, any of the three types: e.g. fp32
+    accumulators into bf16 communication buckets).  In place and with nothing
+    to scale, nothing is written.  Outputs must not overlap one another or
+    another gradient.  A NaN gradient makes every output NaN, an infinite norm
+    makes them 0 (NaN where the gradient was infinite)."""
+    if isinstance(grads, torch.Tensor):
+        grads = (grads,)
+    grads = list(grads)
+    return _grad_call(grads, grads if out is None else out, norm_type, grad_scale, max_norm, "n")[:1]
+
+
+# ----------------------------------------------------------------------------
+# norms after and before a block, with gate and residual scale
+# ----------------------------------------------------------------------------
+
+
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    """A [T, D] tensor with unit column stride (rows may be strided), copied otherwise."""
+    if (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1):
+        return t
+    return t.contiguous()
+
+
+def _ld(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1])
+
+
+def _norm_params(x: torch.Tensor, gamma_post, gate, gamma_pre):
+    """Checked contiguous parameters and the number of gate groups."""
+    t, d = x.shape
+    for g, name in ((gamma_post, "gamma_post"), (gamma_pre, "gamma_pre")):
+        _require(g is None or (g.numel() == d and g.dtype == x.dtype and g.device == x.device),
+                 f"{name} must be [D] of the activations' dtype and device")
+    groups = 0
+    if gate is not None:
+        _require(gate.dtype == x.dtype and gate.device == x.device and gate.shape[-1] == d,
+                 "gate must be [D] or [G, D] of the activations' dtype and device")
+        gate = gate.reshape(-1, d).contiguous()
+        groups = gate.shape[0]
+        _require(groups > 0 and t % groups == 0, "the rows must split evenly over the gate's groups")
+    return (None if gamma_post is None else gamma_post.contiguous(), gate,
+            None if gamma_pre is None else gamma_pre.contiguous(), groups)
+
+
+def sandwich_norm(b: torch.Tensor, x: torch.Tensor, gamma_post: Optional[torch.Tensor] = None,
+                  gate: Optional[torch.Tensor] = None, gamma_pre: Optional[torch.Tensor] = None, *,
+                  residual_scale: float = 1.0, branch_scale: float = 1.0, eps: float = 1e-6,
+                  pre: Optional[bool] = None):
+    """The norms after one block and before the next, in one pass:
+
+        y = residual_scale * x + branch_scale * gate * (b * inv_rms(b) * gamma_post)
+        n = y * inv_rms(y) * gamma_pre                  (of y as stored)
+
+    b (the block's output) and x (the residual stream): [T, D] of one dtype
+    (bf16, fp16, fp32), rows may be strided.  ``gate`` is [D] or [G, D], group g
+    taking rows [g T/G, (g+1) T/G).  n is computed when ``gamma_pre`` is given
+    or ``pre=True`` (then with weight 1).  Returns (y, n, inv_b, inv_y), the
+    last two fp32 [T]; n and inv_y are None without n.  D <= 16384."""
+    _require(b.is_cuda and b.dtype in _DTYPES and b.dim() == 2, "sandwich_norm expects CUDA bf16, fp16 or fp32 [T, D]")
+    _require(x.dtype == b.dtype and x.device == b.device and x.shape == b.shape, "b and x must match in shape, dtype and device")
+    gamma_post, gate, gamma_pre, groups = _norm_params(b, gamma_post, gate, gamma_pre)
+    t, d = b.shape
+    _require(0 < d <= 16384, "sandwich_norm takes 1 to 16384 columns")
+    b, x = _rows_of(b), _rows_of(x)
+    pre = gamma_pre is not None if pre is None else pre
+    _require(pre or gamma_pre is None, "gamma_pre without the norm it belongs to")
+    y = torch.empty((t, d), device=b.device, dtype=b.dtype)
+    n = torch.empty((t, d), device=b.device, dtype=b.dtype) if pre else None
+    inv = torch.empty((2 if pre else 1, t), device=b.device, dtype=torch.float32)
+    inv_b, inv_y = inv[0], (inv[1] if pre else None)
+    if t:
+        _run(b, "nvfp4b200_sandwich_norm", b.data_ptr(), x.data_ptr(), _ptr(gamma_post), _ptr(gate), _ptr(gamma_pre),
+             y.data_ptr(), _ptr(n), inv_b.data_ptr(), _ptr(inv_y), _DTYPES[b.dtype], t, d, groups, _ld(b), _ld(x),
+             float(residual_scale), float(branch_scale), float(eps))
+    return y, n, inv_b, inv_y
+
+
+def sandwich_norm_bwd(dy: Optional[torch.Tensor], b: torch.Tensor, inv_b: torch.Tensor,
+                      gamma_post: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, *,
+                      dn: Optional[torch.Tensor] = None, y: Optional[torch.Tensor] = None,
+                      inv_y: Optional[torch.Tensor] = None, gamma_pre: Optional[torch.Tensor] = None,
+                      residual_scale: float = 1.0, branch_scale: float = 1.0) -> dict:
+    """Backward of ``sandwich_norm`` given dy and, when n was used, dn (with y
+    and inv_y as the forward returned them); either gradient may be None.
+
+    Returns a dict: dx, db [T, D] in the activations' dtype; dgamma_post [D],
+    dgate [G, D], dgamma_pre [D] in fp32 (None without dn, and dgate without a
+    gate).  Column sums are added up in a fixed order."""
+    _require(dy is not None or dn is not None, "sandwich_norm_bwd needs dy or dn")
+    _require(b.is_cuda and b.dtype in _DTYPES and b.dim() == 2, "sandwich_norm_bwd expects CUDA bf16, fp16 or fp32 [T, D]")
+    _require((dn is None) == (y is None) and (dn is None) == (inv_y is None), "dn comes with y and inv_y")
+    _require(dn is not None or gamma_pre is None, "gamma_pre without the norm it belongs to")
+    for g, name in ((dy, "dy"), (dn, "dn"), (y, "y")):
+        _require(g is None or (g.dtype == b.dtype and g.device == b.device and g.shape == b.shape),
+                 f"{name} must match b in shape, dtype and device")
+    t, d = b.shape
+    for g in (inv_b, inv_y):
+        _require(g is None or (g.dtype == torch.float32 and g.numel() == t and g.device == b.device and g.is_contiguous()),
+                 "inv_b and inv_y are contiguous float32 [T]")
+    gamma_post, gate, gamma_pre, groups = _norm_params(b, gamma_post, gate, gamma_pre)
+    _require(0 < d <= 16384, "sandwich_norm takes 1 to 16384 columns")
+    b = _rows_of(b)
+    dy, dn, y = (None if g is None else _rows_of(g) for g in (dy, dn, y))
+    dev = b.device
+    dx = torch.empty((t, d), device=dev, dtype=b.dtype)
+    db = torch.empty((t, d), device=dev, dtype=b.dtype)
+    par = torch.empty((groups + 1 + (dn is not None), d), device=dev, dtype=torch.float32)
+    dpost, dpre = par[0], (par[1] if dn is not None else None)
+    dgate = par[par.shape[0] - groups:] if groups else None
+    if t == 0:
+        par.zero_()
+    else:
+        floats = _lib.c_i64(0)
+        with torch.cuda.device(dev):
+            _lib.call("nvfp4b200_sandwich_norm_bwd_ws", t, d, groups, _lib.ctypes.byref(floats))
+        ws = torch.empty(floats.value, device=dev, dtype=torch.float32)
+        ld = lambda g: 0 if g is None else _ld(g)
+        _run(b, "nvfp4b200_sandwich_norm_bwd", _ptr(dy), _ptr(dn), b.data_ptr(), _ptr(y), inv_b.data_ptr(),
+             _ptr(inv_y), _ptr(gamma_post), _ptr(gate), _ptr(gamma_pre), dx.data_ptr(), db.data_ptr(),
+             dpost.data_ptr(), _ptr(dgate), _ptr(dpre), ws.data_ptr(), ws.numel(), _DTYPES[b.dtype], t, d, groups,
+             ld(dy), ld(dn), _ld(b), ld(y), float(residual_scale), float(branch_scale))
+    return {"dx": dx, "db": db, "dgamma_post": dpost, "dgate": dgate, "dgamma_pre": dpre}
+
+
+# ----------------------------------------------------------------------------
 # training-step element-wise kernels
 # ----------------------------------------------------------------------------
 
@@ -361,34 +735,40 @@ def add_bf16(a: torch.Tensor, b: torch.Tensor, out: Optional[torch.Tensor] = Non
 
 def adamw_step(param: torch.Tensor, grad: torch.Tensor, m: torch.Tensor, v: torch.Tensor, *, lr: float,
                beta1: float, beta2: float, eps: float, weight_decay: float, step: int,
-               grad_scale: float = 1.0) -> None:
+               grad_scale: float = 1.0, clip: Optional[torch.Tensor] = None) -> None:
+    """AdamW on a bf16 parameter with fp32 moments; ``clip`` (a 1-element fp32
+    CUDA tensor, e.g. from ``grad_norm_coef``) is one more factor on the gradient."""
     _require(param.dtype == torch.bfloat16 and m.dtype == torch.float32 and v.dtype == torch.float32,
              "AdamW: bf16 parameter, fp32 moments")
     _require(grad.dtype in (torch.bfloat16, torch.float32), "AdamW: bf16 or fp32 gradient")
     bc1 = 1.0 - beta1 ** step
     bc2 = 1.0 - beta2 ** step
-    _lib.call("nvfp4b200_adamw_step", param.data_ptr(), grad.data_ptr(),
+    _lib.call("nvfp4b200_adamw_step_clipped", param.data_ptr(), grad.data_ptr(),
               _DT_BF16 if grad.dtype == torch.bfloat16 else _DT_F32, m.data_ptr(), v.data_ptr(), param.numel(),
-              lr, beta1, beta2, eps, weight_decay, bc1, bc2, grad_scale, _stream(param))
+              lr, beta1, beta2, eps, weight_decay, bc1, bc2, grad_scale, _ptr(_scalar_f32(clip, param.device)),
+              _stream(param))
 
 
 def adamw_master_step(param: torch.Tensor, master: torch.Tensor, grad: torch.Tensor, m: torch.Tensor,
                       v: torch.Tensor, *, lr: float, beta1: float, beta2: float, eps: float, weight_decay: float,
-                      step: int, grad_scale: float = 1.0, amax_bits: Optional[torch.Tensor] = None) -> None:
+                      step: int, grad_scale: float = 1.0, amax_bits: Optional[torch.Tensor] = None,
+                      clip: Optional[torch.Tensor] = None) -> None:
     """AdamW on an fp32 master copy (torch.optim.AdamW's operation order);
     the bf16 ``param`` receives bf16(master) after the update.  ``amax_bits``
     (a 1-element int32 CUDA tensor, zeroed by the caller) collects the
-    largest |bf16 parameter| written, as float bits (atomic max)."""
+    largest |bf16 parameter| written, as float bits (atomic max); ``clip`` (a
+    1-element fp32 CUDA tensor, e.g. from ``grad_norm_coef``) is one more
+    factor on the gradient."""
     _require(param.dtype == torch.bfloat16 and master.dtype == torch.float32 and m.dtype == torch.float32
              and v.dtype == torch.float32, "AdamW: bf16 parameter, fp32 master and moments")
     _require(grad.dtype in (torch.bfloat16, torch.float32), "AdamW: bf16 or fp32 gradient")
     n = param.numel()
     _require(master.numel() == n and m.numel() == n and v.numel() == n and grad.numel() == n,
              "AdamW: parameter, master, gradient and moments must have the same length")
-    _lib.call("nvfp4b200_adamw_master_step", param.data_ptr(), master.data_ptr(), grad.data_ptr(),
+    _lib.call("nvfp4b200_adamw_master_step_clipped", param.data_ptr(), master.data_ptr(), grad.data_ptr(),
               _DT_BF16 if grad.dtype == torch.bfloat16 else _DT_F32, m.data_ptr(), v.data_ptr(), n,
-              *adamw_master_scalars(lr, beta1, beta2, eps, weight_decay, step), grad_scale, _ptr(amax_bits),
-              _stream(param))
+              *adamw_master_scalars(lr, beta1, beta2, eps, weight_decay, step), grad_scale,
+              _ptr(_scalar_f32(clip, param.device)), _ptr(amax_bits), _stream(param))
 
 
 def global_scale_from_amax(amax_bits: torch.Tensor) -> torch.Tensor:
