@@ -282,7 +282,7 @@ int nvfp4b200_grad_norm_finish(const double* partials, int64_t n, int norm_type,
 
 /* y = residual_scale * x + branch_scale * gate[g] * (b * inv_b * gamma_post),
  * inv_b = rsqrt(mean(b^2) + eps); and, when n is given, n = y * inv_y *
- * gamma_pre with inv_y = rsqrt(mean(y^2) + eps) of y as stored.  b, x, y, n:
+ * gamma_pre with inv_y = rsqrt(mean(y^2) + eps), y before its rounding.  b, x, y, n:
  * [rows, d] of dtype (bf16, f16 or f32), b and x with row strides ldb, ldx;
  * gamma_post, gamma_pre [d] and gate [groups, d] of the same dtype, each
  * optional (1); row r takes gate row r / (rows / groups); groups = 0 without

@@ -110,8 +110,9 @@ def check(rc: int, what: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    lib = load()
-    check(getattr(lib, name)(*args), name)
+    rc = getattr(_lib or load(), name)(*args)
+    if rc:
+        check(rc, name)
 
 
 def exported_symbols():

@@ -57,13 +57,19 @@ def _scalar_f32(g: Optional[torch.Tensor], device) -> Optional[torch.Tensor]:
     return g
 
 
+# The current device and its current stream's handle, without building the
+# device and stream objects of torch.cuda (0.2 us a call in place of 3.4 us).
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _run(t: torch.Tensor, name: str, *args) -> None:
     """Call an entry point on the device of ``t`` and that device's current stream."""
-    if t.device.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    dev = t.get_device()
+    if dev == _current_device():
+        _lib.call(name, *args, _raw_stream(dev))
     else:
-        with torch.cuda.device(t.device):
-            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, _raw_stream(dev))
 
 
 _WS = {}
@@ -275,13 +281,15 @@ def gemm(qa: torch.Tensor, sa: torch.Tensor, qb: torch.Tensor, sb: torch.Tensor,
 # ----------------------------------------------------------------------------
 
 
-def _float_matrix(x: torch.Tensor, what: str) -> torch.Tensor:
+def _float_matrix(x: torch.Tensor) -> torch.Tensor:
     """x as the MXFP4 quantizers read it: 2-D, unit column stride, 16-byte
     aligned rows; copied when it is laid out otherwise."""
-    _require(x.is_cuda and x.dtype in _DTYPES, f"{what} expects a CUDA bf16, fp16 or fp32 tensor")
-    _require(x.dim() == 2, f"{what} expects a 2-D tensor")
-    if x.stride(1) == 1 and x.stride(0) >= x.shape[1] and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
-        return x
+    if not (x.is_cuda and x.dtype in _DTYPES and x.dim() == 2):
+        raise RuntimeError("MXFP4 quantizers expect a 2-D CUDA bf16, fp16 or fp32 tensor")
+    if x.data_ptr() % 16 == 0:
+        rs, cs = x.stride()
+        if cs == 1 and rs >= x.shape[1] and rs % 8 == 0:
+            return x
     return x.clone(memory_format=torch.contiguous_format)
 
 
@@ -300,18 +308,29 @@ def _mx_factors(x: torch.Tensor, row_scale, gamma):
     return row_scale, gamma
 
 
-def _mx_quant(x, row_scale, gamma, rows: bool, cols: bool, out, what: str):
-    x = _float_matrix(x, what)
+def _mx_pair(rows: int, k: int, device, out):
+    """(q, s) tensors of an MXFP4 operand of ``rows`` rows along k."""
+    if out is not None:
+        return _outputs(out, (rows, k // 2), mx_scale_shape(rows, k), device)
+    return (torch.empty((rows, k // 2), device=device, dtype=torch.uint8),
+            torch.empty(mx_scale_shape(rows, k), device=device, dtype=torch.uint8))
+
+
+def _mx_quant(x, row_scale, gamma, rows: bool, cols: bool, out):
+    x = _float_matrix(x)
     r, c = x.shape
-    _require(not rows or c % 32 == 0, "K must be divisible by 32 for MXFP4 1x32 scaling.")
-    _require(c > 0 and c % 8 == 0, f"{what} needs columns divisible by 8")
-    row_scale, gamma = _mx_factors(x, row_scale, gamma)
+    if rows and c % 32:
+        raise RuntimeError("K must be divisible by 32 for MXFP4 1x32 scaling.")
+    if c == 0 or c % 8:
+        raise RuntimeError("MXFP4 quantizers need columns divisible by 8")
+    if row_scale is not None or gamma is not None:
+        row_scale, gamma = _mx_factors(x, row_scale, gamma)
     q = s = qt = st = None
+    dev = x.device
     if rows:
-        q, s = _outputs(out, (r, c // 2), mx_scale_shape(r, c), x.device)
+        q, s = _mx_pair(r, c, dev, out)
     if cols:
-        pr = round_up(r, 32)
-        qt, st = _outputs(None if rows else out, (c, pr // 2), mx_scale_shape(c, pr), x.device)
+        qt, st = _mx_pair(c, (r + 31) // 32 * 32, dev, None if rows else out)
     if r:
         _run(x, "nvfp4b200_mx_quant", x.data_ptr(), _DTYPES[x.dtype], _ptr(row_scale), _ptr(gamma), _ptr(q), _ptr(s),
              _ptr(qt), _ptr(st), r, c, max(x.stride(0), c))
@@ -328,7 +347,7 @@ def mx_quantize(x: torch.Tensor, row_scale: Optional[torch.Tensor] = None, gamma
     [R]) and ``gamma`` (bf16 [K]) are multiplied in first; a block with an
     infinity or a NaN becomes NaN as a whole.  ``out=(q, s)`` writes into given
     tensors of those shapes."""
-    return _mx_quant(x, row_scale, gamma, True, False, out, "mx_quantize")[:2]
+    return _mx_quant(x, row_scale, gamma, True, False, out)[:2]
 
 
 def mx_quantize_t(x: torch.Tensor, row_scale: Optional[torch.Tensor] = None, gamma: Optional[torch.Tensor] = None,
@@ -336,13 +355,13 @@ def mx_quantize_t(x: torch.Tensor, row_scale: Optional[torch.Tensor] = None, gam
     """MXFP4-quantize x^T (x [R, C], C % 8 == 0) along R -> (q u8 [C, P/2], s
     swizzled for (C, P)), P = R rounded up to 32: the rows past the last count
     as zeros, so a product over P is the product over R."""
-    return _mx_quant(x, row_scale, gamma, False, True, out, "mx_quantize_t")[2:]
+    return _mx_quant(x, row_scale, gamma, False, True, out)[2:]
 
 
 def mx_quantize_both(x: torch.Tensor, row_scale: Optional[torch.Tensor] = None, gamma: Optional[torch.Tensor] = None):
     """Both orientations of x [R, K] from one read: the pairs of ``mx_quantize``
     and ``mx_quantize_t`` as (q, s, qt, st)."""
-    return _mx_quant(x, row_scale, gamma, True, True, None, "mx_quantize_both")
+    return _mx_quant(x, row_scale, gamma, True, True, None)
 
 
 def mx_dequantize(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -368,25 +387,35 @@ def mx_gemm(qa: torch.Tensor, sa: torch.Tensor, qb: torch.Tensor, sb: torch.Tens
     ``gemm`` for 1x32 blocks with UE8M0 scales.
 
     qa: [m, k/2], qb: [n, k/2] packed bytes; fp32 outputs can accumulate."""
-    _require(qa.is_cuda and all(t.device == qa.device for t in (sa, qb, sb)), "mx_gemm requires CUDA tensors of one device")
+    dev = qa.get_device()
+    if not qa.is_cuda or sa.get_device() != dev or qb.get_device() != dev or sb.get_device() != dev:
+        raise RuntimeError("mx_gemm requires CUDA tensors of one device")
     m, kh = qa.shape
     n, kh2 = qb.shape
-    _require(kh == kh2, f"K mismatch: A has {2 * kh}, B has {2 * kh2}")
     k = 2 * kh
-    _require(k > 0 and k % 32 == 0, "K must be divisible by 32 for MXFP4 1x32 scaling.")
-    _require(qa.is_contiguous() and qb.is_contiguous() and sa.is_contiguous() and sb.is_contiguous(),
-             "gemm operands must be contiguous")
-    _require(sa.numel() == math.prod(mx_scale_shape(m, k)) and sb.numel() == math.prod(mx_scale_shape(n, k)),
-             "MXFP4 scale tensors must be the padded swizzled [round_up(rows,128), round_up(k/32,4)] layout")
+    if kh != kh2:
+        raise RuntimeError(f"K mismatch: A has {k}, B has {2 * kh2}")
+    if k == 0 or k % 32:
+        raise RuntimeError("K must be divisible by 32 for MXFP4 1x32 scaling.")
+    if not (qa.is_contiguous() and qb.is_contiguous() and sa.is_contiguous() and sb.is_contiguous()):
+        raise RuntimeError("gemm operands must be contiguous")
+    cols = (k + 127) // 128 * 4
+    if sa.numel() != (m + 127) // 128 * 128 * cols or sb.numel() != (n + 127) // 128 * 128 * cols:
+        raise RuntimeError("MXFP4 scale tensors must be the padded swizzled "
+                           "[round_up(rows,128), round_up(k/32,4)] layout")
     if out is None:
         _require(not accumulate, "accumulate needs an existing output")
+        _require(out_dtype in (torch.bfloat16, torch.float32), "output dtype must be bf16 or fp32")
         out = torch.empty((m, n), device=qa.device, dtype=out_dtype)
-    _require(out.dtype in (torch.bfloat16, torch.float32) and out.device == qa.device, "output dtype must be bf16 or fp32")
-    _require(out.dim() == 2 and out.shape == (m, n) and out.stride(1) == 1, "output must be [m, n] with unit column stride")
-    _require(not accumulate or out.dtype == torch.float32, "accumulate needs an fp32 output")
+    else:
+        _require(out.dtype in (torch.bfloat16, torch.float32) and out.get_device() == dev,
+                 "output must be bf16 or fp32 on the operands' device")
+        _require(out.dim() == 2 and out.shape == (m, n) and out.stride(1) == 1,
+                 "output must be [m, n] with unit column stride")
+        _require(not accumulate or out.dtype == torch.float32, "accumulate needs an fp32 output")
     if bias is not None:
         _check_bf16(bias, "bias")
-        _require(bias.numel() == n and bias.device == qa.device, "bias is bf16 [n]")
+        _require(bias.numel() == n and bias.get_device() == dev, "bias is bf16 [n]")
         bias = bias.contiguous()
     if residual is not None:
         _check_bf16(residual, "residual")
@@ -435,36 +464,46 @@ def _grad_call(grads, outs, norm_type, grad_scale, max_norm, want):
     if isinstance(grads, torch.Tensor):
         grads = (grads,)
     grads = list(grads)
-    _require(norm_type == 2 or norm_type == math.inf, "norm_type must be 2 or inf")
-    max_norm = float(max_norm)
-    _require(max_norm >= 0.0, "max_norm must not be negative")
-    dev = grads[0].device if grads else torch.device("cuda", torch.cuda.current_device())
+    if norm_type != 2 and norm_type != math.inf:
+        raise RuntimeError("norm_type must be 2 or inf")
+    if not max_norm >= 0.0:
+        raise RuntimeError("max_norm must not be negative")
+    dev = grads[0].get_device() if grads else _current_device()
+    ptrs, dts, lens = array.array("Q"), array.array("i"), array.array("q")
     for t in grads:
-        _require(t.is_cuda and t.device == dev and t.dtype in _DTYPES, "gradients are bf16, fp16 or fp32 CUDA tensors of one device")
-        _require(t.is_contiguous() or _dense(t), "gradients must be dense: every element once in one stretch of memory")
+        dt = _DTYPES.get(t.dtype)
+        if dt is None or dev < 0 or t.get_device() != dev:
+            raise RuntimeError("gradients are bf16, fp16 or fp32 CUDA tensors of one device")
+        if not (t.is_contiguous() or _dense(t)):
+            raise RuntimeError("gradients must be dense: every element once in one stretch of memory")
+        ptrs.append(t.data_ptr())
+        dts.append(dt)
+        lens.append(t.numel())
     count = len(grads)
-    ptrs = array.array("Q", [t.data_ptr() for t in grads])
-    dts = array.array("i", [_DTYPES[t.dtype] for t in grads])
-    lens = array.array("q", [t.numel() for t in grads])
     outp = outd = None
-    if outs is not None:
+    if outs is grads:
+        outp, outd = ptrs, dts
+    elif outs is not None:
         outs = [outs] if isinstance(outs, torch.Tensor) else list(outs)
         _require(len(outs) == count, "out must hold one tensor per gradient")
+        outp, outd = array.array("Q"), array.array("i")
         for t, o in zip(grads, outs):
-            _require(o.device == dev and o.dtype in _DTYPES and o.shape == t.shape
-                     and (o.stride() == t.stride() or (o.is_contiguous() and t.is_contiguous())),
-                     "out tensors match their gradient's shape and layout (bf16, fp16 or fp32)")
-        outp = array.array("Q", [t.data_ptr() for t in outs])
-        outd = array.array("i", [_DTYPES[t.dtype] for t in outs])
-    ws = torch.empty(1024 * (1 + count // 112), device=dev, dtype=torch.float64)
-    # the results in one allocation: fp32 norm, fp32 coefficient, fp64 total
-    res = torch.empty(4, device=dev, dtype=torch.float32)
-    base = res.data_ptr()
+            dt = _DTYPES.get(o.dtype)
+            if (dt is None or o.get_device() != dev or o.shape != t.shape
+                    or not ((o.is_contiguous() and t.is_contiguous()) or o.stride() == t.stride())):
+                raise RuntimeError("out tensors match their gradient's shape and layout (bf16, fp16 or fp32)")
+            outp.append(o.data_ptr())
+            outd.append(dt)
+    device = torch.device("cuda", dev)
+    words = 1024 * (1 + count // 112)
+    ws = torch.empty(words, device=device, dtype=torch.float64)
+    norm = torch.empty(1, device=device, dtype=torch.float32) if "n" in want else None
+    coef = torch.empty(1, device=device, dtype=torch.float32) if "c" in want else None
+    total = torch.empty(1, device=device, dtype=torch.float64) if "t" in want else None
     addr = lambda a: None if a is None else a.buffer_info()[0]
-    _run(res, "nvfp4b200_grad_norm", addr(ptrs), addr(dts), addr(outp), addr(outd), addr(lens), count,
-         2 if norm_type == 2 else 0, float(grad_scale), max_norm, ws.data_ptr(), ws.numel(),
-         base if "n" in want else None, base + 4 if "c" in want else None, base + 8 if "t" in want else None)
-    return res
+    _run(ws, "nvfp4b200_grad_norm", addr(ptrs), addr(dts), addr(outp), addr(outd), addr(lens), count,
+         2 if norm_type == 2 else 0, grad_scale, max_norm, ws.data_ptr(), words, _ptr(norm), _ptr(coef), _ptr(total))
+    return norm, coef, total
 
 
 def grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], norm_type: float = 2.0,
@@ -472,7 +511,7 @@ def grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], norm_type: flo
     """Norm of all gradients together (2 or inf), of grad * grad_scale, as a
     1-element fp32 tensor.  The list may mix bf16, fp16 and fp32 and hold empty
     tensors; the sum is carried in fp64 and does not depend on timing."""
-    return _grad_call(grads, None, norm_type, grad_scale, math.inf, "n")[:1]
+    return _grad_call(grads, None, norm_type, grad_scale, math.inf, "n")[0]
 
 
 def grad_norm_coef(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
@@ -480,15 +519,14 @@ def grad_norm_coef(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm:
     """(norm, coef) with coef = min(1, max_norm / (norm + 1e-6)), both 1-element
     fp32 tensors: hand coef to ``adamw_step`` / ``adamw_master_step`` as
     ``clip`` and the gradients are clipped without a pass of their own."""
-    res = _grad_call(grads, None, norm_type, grad_scale, max_norm, "nc")
-    return res[:1], res[1:2]
+    return _grad_call(grads, None, norm_type, grad_scale, max_norm, "nc")[:2]
 
 
 def grad_norm_total(grads: Union[torch.Tensor, Sequence[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
     """The sum of squares (or the largest magnitude) as a 1-element fp64 tensor:
     what a rank holding a shard of the gradients sends to a sum (maximum) over
     the ranks before ``grad_norm_finish``."""
-    return _grad_call(grads, None, norm_type, 1.0, math.inf, "t")[2:].view(torch.float64)
+    return _grad_call(grads, None, norm_type, 1.0, math.inf, "t")[2]
 
 
 def grad_norm_finish(totals: torch.Tensor, max_norm: float, norm_type: float = 2.0,
@@ -517,7 +555,7 @@ def clip_grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm:
     if isinstance(grads, torch.Tensor):
         grads = (grads,)
     grads = list(grads)
-    return _grad_call(grads, grads if out is None else out, norm_type, grad_scale, max_norm, "n")[:1]
+    return _grad_call(grads, grads if out is None else out, norm_type, grad_scale, max_norm, "n")[0]
 
 
 # ----------------------------------------------------------------------------
@@ -527,7 +565,7 @@ def clip_grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm:
 
 def _rows_of(t: torch.Tensor) -> torch.Tensor:
     """A [T, D] tensor with unit column stride (rows may be strided), copied otherwise."""
-    if (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1):
+    if t.is_contiguous() or (t.stride(1) == 1 and t.stride(0) >= t.shape[1]):
         return t
     return t.contiguous()
 
@@ -539,18 +577,27 @@ def _ld(t: torch.Tensor) -> int:
 def _norm_params(x: torch.Tensor, gamma_post, gate, gamma_pre):
     """Checked contiguous parameters and the number of gate groups."""
     t, d = x.shape
-    for g, name in ((gamma_post, "gamma_post"), (gamma_pre, "gamma_pre")):
-        _require(g is None or (g.numel() == d and g.dtype == x.dtype and g.device == x.device),
-                 f"{name} must be [D] of the activations' dtype and device")
+    dev, dt = x.get_device(), x.dtype
+    for g in (gamma_post, gamma_pre):
+        if g is not None and (g.numel() != d or g.dtype != dt or g.get_device() != dev):
+            raise RuntimeError("gamma_post and gamma_pre must be [D] of the activations' dtype and device")
     groups = 0
     if gate is not None:
-        _require(gate.dtype == x.dtype and gate.device == x.device and gate.shape[-1] == d,
-                 "gate must be [D] or [G, D] of the activations' dtype and device")
-        gate = gate.reshape(-1, d).contiguous()
-        groups = gate.shape[0]
-        _require(groups > 0 and t % groups == 0, "the rows must split evenly over the gate's groups")
+        if gate.dtype != dt or gate.get_device() != dev or gate.shape[-1] != d:
+            raise RuntimeError("gate must be [D] or [G, D] of the activations' dtype and device")
+        groups = gate.numel() // d
+        if groups == 0 or t % groups:
+            raise RuntimeError("the rows must split evenly over the gate's groups")
+        gate = gate.contiguous()
     return (None if gamma_post is None else gamma_post.contiguous(), gate,
             None if gamma_pre is None else gamma_pre.contiguous(), groups)
+
+
+def _norm_input(b: torch.Tensor) -> None:
+    if not (b.is_cuda and b.dtype in _DTYPES and b.dim() == 2):
+        raise RuntimeError("the norms expect CUDA bf16, fp16 or fp32 [T, D]")
+    if not 0 < b.shape[1] <= 16384:
+        raise RuntimeError("the norms take 1 to 16384 columns")
 
 
 def sandwich_norm(b: torch.Tensor, x: torch.Tensor, gamma_post: Optional[torch.Tensor] = None,
@@ -560,30 +607,47 @@ def sandwich_norm(b: torch.Tensor, x: torch.Tensor, gamma_post: Optional[torch.T
     """The norms after one block and before the next, in one pass:
 
         y = residual_scale * x + branch_scale * gate * (b * inv_rms(b) * gamma_post)
-        n = y * inv_rms(y) * gamma_pre                  (of y as stored)
+        n = y * inv_rms(y) * gamma_pre            (from y before its rounding)
 
     b (the block's output) and x (the residual stream): [T, D] of one dtype
     (bf16, fp16, fp32), rows may be strided.  ``gate`` is [D] or [G, D], group g
     taking rows [g T/G, (g+1) T/G).  n is computed when ``gamma_pre`` is given
     or ``pre=True`` (then with weight 1).  Returns (y, n, inv_b, inv_y), the
     last two fp32 [T]; n and inv_y are None without n.  D <= 16384."""
-    _require(b.is_cuda and b.dtype in _DTYPES and b.dim() == 2, "sandwich_norm expects CUDA bf16, fp16 or fp32 [T, D]")
-    _require(x.dtype == b.dtype and x.device == b.device and x.shape == b.shape, "b and x must match in shape, dtype and device")
+    _norm_input(b)
+    if x.dtype != b.dtype or x.get_device() != b.get_device() or x.shape != b.shape:
+        raise RuntimeError("b and x must match in shape, dtype and device")
     gamma_post, gate, gamma_pre, groups = _norm_params(b, gamma_post, gate, gamma_pre)
     t, d = b.shape
-    _require(0 < d <= 16384, "sandwich_norm takes 1 to 16384 columns")
     b, x = _rows_of(b), _rows_of(x)
     pre = gamma_pre is not None if pre is None else pre
-    _require(pre or gamma_pre is None, "gamma_pre without the norm it belongs to")
-    y = torch.empty((t, d), device=b.device, dtype=b.dtype)
-    n = torch.empty((t, d), device=b.device, dtype=b.dtype) if pre else None
+    if gamma_pre is not None and not pre:
+        raise RuntimeError("gamma_pre without the norm it belongs to")
+    y = b.new_empty((t, d))
     inv = torch.empty((2 if pre else 1, t), device=b.device, dtype=torch.float32)
-    inv_b, inv_y = inv[0], (inv[1] if pre else None)
+    n = inv_y = None
+    if pre:
+        n = torch.empty_like(y)
+        inv_b, inv_y = inv.unbind()
+    else:
+        inv_b = inv.view(t)
     if t:
         _run(b, "nvfp4b200_sandwich_norm", b.data_ptr(), x.data_ptr(), _ptr(gamma_post), _ptr(gate), _ptr(gamma_pre),
              y.data_ptr(), _ptr(n), inv_b.data_ptr(), _ptr(inv_y), _DTYPES[b.dtype], t, d, groups, _ld(b), _ld(x),
-             float(residual_scale), float(branch_scale), float(eps))
+             residual_scale, branch_scale, eps)
     return y, n, inv_b, inv_y
+
+
+def _bwd_words(dev: int, t: int, d: int, groups: int) -> int:
+    """fp32 words of workspace of the backward on a device."""
+    floats = _lib.c_i64(0)
+    args = ("nvfp4b200_sandwich_norm_bwd_ws", t, d, groups, _lib.ctypes.byref(floats))
+    if dev == _current_device():
+        _lib.call(*args)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(*args)
+    return floats.value
 
 
 def sandwich_norm_bwd(dy: Optional[torch.Tensor], b: torch.Tensor, inv_b: torch.Tensor,
@@ -597,39 +661,40 @@ def sandwich_norm_bwd(dy: Optional[torch.Tensor], b: torch.Tensor, inv_b: torch.
     Returns a dict: dx, db [T, D] in the activations' dtype; dgamma_post [D],
     dgate [G, D], dgamma_pre [D] in fp32 (None without dn, and dgate without a
     gate).  Column sums are added up in a fixed order."""
-    _require(dy is not None or dn is not None, "sandwich_norm_bwd needs dy or dn")
-    _require(b.is_cuda and b.dtype in _DTYPES and b.dim() == 2, "sandwich_norm_bwd expects CUDA bf16, fp16 or fp32 [T, D]")
-    _require((dn is None) == (y is None) and (dn is None) == (inv_y is None), "dn comes with y and inv_y")
-    _require(dn is not None or gamma_pre is None, "gamma_pre without the norm it belongs to")
-    for g, name in ((dy, "dy"), (dn, "dn"), (y, "y")):
-        _require(g is None or (g.dtype == b.dtype and g.device == b.device and g.shape == b.shape),
-                 f"{name} must match b in shape, dtype and device")
-    t, d = b.shape
+    if dy is None and dn is None:
+        raise RuntimeError("sandwich_norm_bwd needs dy or dn")
+    _norm_input(b)
+    if (dn is None) != (y is None) or (dn is None) != (inv_y is None):
+        raise RuntimeError("dn comes with y and inv_y")
+    if dn is None and gamma_pre is not None:
+        raise RuntimeError("gamma_pre without the norm it belongs to")
+    dt, dev, shape = b.dtype, b.get_device(), b.shape
+    for g in (dy, dn, y):
+        if g is not None and (g.dtype != dt or g.get_device() != dev or g.shape != shape):
+            raise RuntimeError("dy, dn and y must match b in shape, dtype and device")
+    t, d = shape
     for g in (inv_b, inv_y):
-        _require(g is None or (g.dtype == torch.float32 and g.numel() == t and g.device == b.device and g.is_contiguous()),
-                 "inv_b and inv_y are contiguous float32 [T]")
+        if g is not None and (g.dtype != torch.float32 or g.numel() != t or g.get_device() != dev
+                              or not g.is_contiguous()):
+            raise RuntimeError("inv_b and inv_y are contiguous float32 [T]")
     gamma_post, gate, gamma_pre, groups = _norm_params(b, gamma_post, gate, gamma_pre)
-    _require(0 < d <= 16384, "sandwich_norm takes 1 to 16384 columns")
     b = _rows_of(b)
     dy, dn, y = (None if g is None else _rows_of(g) for g in (dy, dn, y))
-    dev = b.device
-    dx = torch.empty((t, d), device=dev, dtype=b.dtype)
-    db = torch.empty((t, d), device=dev, dtype=b.dtype)
-    par = torch.empty((groups + 1 + (dn is not None), d), device=dev, dtype=torch.float32)
+    dx, db = b.new_empty((t, d)), b.new_empty((t, d))
+    # the parameters' gradients: dgamma_post, dgamma_pre (with dn), dgate
+    par = torch.empty((groups + 1 + (dn is not None), d), device=b.device, dtype=torch.float32)
     dpost, dpre = par[0], (par[1] if dn is not None else None)
     dgate = par[par.shape[0] - groups:] if groups else None
     if t == 0:
         par.zero_()
     else:
-        floats = _lib.c_i64(0)
-        with torch.cuda.device(dev):
-            _lib.call("nvfp4b200_sandwich_norm_bwd_ws", t, d, groups, _lib.ctypes.byref(floats))
-        ws = torch.empty(floats.value, device=dev, dtype=torch.float32)
+        floats = _bwd_words(dev, t, d, groups)
+        ws = torch.empty(floats, device=b.device, dtype=torch.float32)
         ld = lambda g: 0 if g is None else _ld(g)
         _run(b, "nvfp4b200_sandwich_norm_bwd", _ptr(dy), _ptr(dn), b.data_ptr(), _ptr(y), inv_b.data_ptr(),
              _ptr(inv_y), _ptr(gamma_post), _ptr(gate), _ptr(gamma_pre), dx.data_ptr(), db.data_ptr(),
-             dpost.data_ptr(), _ptr(dgate), _ptr(dpre), ws.data_ptr(), ws.numel(), _DTYPES[b.dtype], t, d, groups,
-             ld(dy), ld(dn), _ld(b), ld(y), float(residual_scale), float(branch_scale))
+             dpost.data_ptr(), _ptr(dgate), _ptr(dpre), ws.data_ptr(), floats, _DTYPES[dt], t, d, groups, ld(dy),
+             ld(dn), _ld(b), ld(y), residual_scale, branch_scale)
     return {"dx": dx, "db": db, "dgamma_post": dpost, "dgate": dgate, "dgamma_pre": dpre}
 
 

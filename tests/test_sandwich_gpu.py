@@ -95,11 +95,11 @@ def test_forward_backward(pkg, t, d, g, post, pre, dtype):
     close(ib, rib, rib)
     close(y, ry, mag, dtype)
     if pre:
-        yd = y.double()
-        riy = (yd.square().mean(1) + eps).rsqrt()
-        close(iy, riy, riy)
-        rn = yd * riy[:, None] * gn.double()
-        close(n, rn, rn.abs(), dtype)
+        # y is off by at most F32 * mag before its rounding; its root mean square by that of the same
+        riy = (ry.square().mean(1) + eps).rsqrt()
+        off = riy * (mag.square().mean(1) + eps).sqrt()
+        close(iy, riy, riy * (1 + off))
+        close(n, ry * riy[:, None] * gn.double(), (mag * (1 + off[:, None])) * riy[:, None] * gn.double().abs(), dtype)
     else:
         assert n is None and iy is None
     dy, dn = rnd((t, d), 6, dtype, 0.1), (rnd((t, d), 7, dtype, 0.1) if pre else None)
