@@ -123,6 +123,45 @@ __device__ __forceinline__ float row_sum(float s, float* red, int group) {
   return s;
 }
 
+template <int DT>
+struct Pairs;   // 8 stored elements -> 4 packed pairs
+template <>
+struct Pairs<NVFP4B200_BF16> {
+  static __device__ __forceinline__ void get(const uint4* p, int stride, uint64_t (&o)[4]) {
+    const uint4 v = *p;
+    o[0] = bf16x2_to_f2(v.x); o[1] = bf16x2_to_f2(v.y); o[2] = bf16x2_to_f2(v.z); o[3] = bf16x2_to_f2(v.w);
+  }
+};
+template <>
+struct Pairs<NVFP4B200_F16> {
+  static __device__ __forceinline__ void get(const uint4* p, int stride, uint64_t (&o)[4]) {
+    const uint4 v = *p;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      o[i] = f2pack(f.x, f.y);
+    }
+  }
+};
+template <>
+struct Pairs<NVFP4B200_F32> {
+  static __device__ __forceinline__ void get(const uint4* p, int stride, uint64_t (&o)[4]) {
+    const uint4 a = p[0], b = p[stride];
+    o[0] = ((uint64_t)a.y << 32) | a.x; o[1] = ((uint64_t)a.w << 32) | a.z;
+    o[2] = ((uint64_t)b.y << 32) | b.x; o[3] = ((uint64_t)b.w << 32) | b.z;
+  }
+};
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ uint64_t f2two(float v) { return f2pack(v, v); }
+__device__ __forceinline__ float f2sum(uint64_t v) { return f2lo(v) + f2hi(v); }
+
+constexpr int STAGES = 3;
+
 struct FwdArgs {
   const void *b, *x, *gamma_post, *gate, *gamma_pre;
   void *y, *n;
@@ -189,6 +228,137 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) sandwich_fwd_kernel(con
     }
     buf ^= 2;   // a row's two sums use two slots; a slot is written again two rows later, past two barriers
   }
+}
+
+// The same forward with the rows staged ahead in shared memory: every thread
+// copies its own columns of b and x (cp.async, 16 bytes each) into a ring of
+// STAGES rows and reads back only what it copied, so the ring needs no
+// barrier and the loads of the next rows run while a row waits for its two
+// reductions.  (The second sum is not folded into the first exchange: y's
+// square sum from those of its parts cancels where y is small.)
+template <int DT, int TPR>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, DT == NVFP4B200_F32 ? (TPR < 512 ? 2 : 1) : TPR < 512 ? 4 : 1024 / TPR)
+    sandwich_fwd_staged_kernel(const FwdArgs a) {
+  using E = Elem<DT>;
+  using Raw = typename E::Raw;
+  constexpr int Q = (int)sizeof(Raw) * 8 / 16;
+  constexpr int NP = CPT / 2;
+  constexpr int THREADS = TPR < 256 ? 256 : TPR, GROUPS = THREADS / TPR;
+  extern __shared__ __align__(16) uint4 ring[];   // [STAGES][2][VPT * Q][THREADS]
+  __shared__ float red[4][GROUPS * (TPR / 32)];
+  const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  const float inv_d = 1.0f / (float)a.d;
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  auto slot = [&](int stage, int tensor, int piece) {
+    return ring + ((stage * 2 + tensor) * (VPT * Q) + piece) * THREADS + threadIdx.x;
+  };
+  auto fetch = [&](int64_t r, int stage) {
+    if (r < a.rows) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const Raw* row = k ? static_cast<const Raw*>(a.x) + r * a.ldx : static_cast<const Raw*>(a.b) + r * a.ldb;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          const int c = column<true, TPR>(t, 8 * i);
+          if (c < a.d) {
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+              cp_async16(slot(stage, k, i * Q + q), reinterpret_cast<const uint4*>(row + c) + q);
+          }
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)   // columns past the end stay zero in every stage
+    if (column<true, TPR>(t, 8 * i) >= a.d)
+      for (int k = 0; k < STAGES * 2; ++k)
+        for (int q = 0; q < Q; ++q) *slot(k >> 1, k & 1, i * Q + q) = make_uint4(0, 0, 0, 0);
+  int64_t r = (int64_t)blockIdx.x * GROUPS + group;
+#pragma unroll
+  for (int st = 0; st < STAGES - 1; ++st) fetch(r + st * step, st);
+
+  // a weight vector's pairs times v, or v where there is none
+  auto weigh = [&](const typename E::Vec8 (&w)[VPT], uint64_t (&v)[NP]) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float f[8];
+      E::unpack(w[i], f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[4 * i + j] = f2mul(v[4 * i + j], f2pack(f[2 * j], f[2 * j + 1]));
+    }
+  };
+  auto load_w = [&](const void* p, int64_t off, typename E::Vec8 (&w)[VPT]) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = column<true, TPR>(t, 8 * i);
+      w[i] = c < a.d ? E::load(static_cast<const Raw*>(p) + off + c) : E::zero();
+    }
+  };
+  auto put = [&](void* base, int64_t r, const uint64_t (&v)[NP]) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = column<true, TPR>(t, 8 * i);
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[2 * j] = f2lo(v[4 * i + j]);
+        f[2 * j + 1] = f2hi(v[4 * i + j]);
+      }
+      if (c < a.d) E::store(static_cast<Raw*>(base) + r * a.d + c, E::pack(f));
+    }
+  };
+  int stage = 0, buf = 0;
+  for (; r < a.rows; r += step) {
+    typename E::Vec8 wp[VPT], wg[VPT], wn[VPT];   // read (from L1 after the first row) ahead of the reductions
+    if (a.gamma_post) load_w(a.gamma_post, 0, wp);
+    if (a.gate) load_w(a.gate, (r / a.rows_per_gate) * a.d, wg);
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    uint64_t v[NP], ss = 0ull;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      uint64_t p[4];
+      Pairs<DT>::get(slot(stage, 0, i * Q), THREADS, p);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[4 * i + j] = p[j];
+        ss = f2fma(p[j], p[j], ss);
+      }
+    }
+    fetch(r + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
+    const float inv_b = rsqrtf(row_sum<TPR>(f2sum(ss), red[buf], group) * inv_d + a.eps);
+#pragma unroll
+    for (int j = 0; j < NP; ++j) v[j] = f2mul(v[j], f2two(inv_b));
+    if (a.gamma_post) weigh(wp, v);
+    if (a.gate) weigh(wg, v);
+    if (a.gamma_pre) load_w(a.gamma_pre, 0, wn);
+    ss = 0ull;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      uint64_t x[4];
+      Pairs<DT>::get(slot(stage, 1, i * Q), THREADS, x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint64_t& y = v[4 * i + j];
+        y = f2fma(f2two(a.s), y, f2mul(f2two(a.alpha), x[j]));
+        ss = f2fma(y, y, ss);
+      }
+    }
+    put(a.y, r, v);
+    if (t == 0) a.inv_b[r] = inv_b;
+    if (a.pre) {
+      const float inv_y = rsqrtf(row_sum<TPR>(f2sum(ss), red[buf + 1], group) * inv_d + a.eps);
+#pragma unroll
+      for (int j = 0; j < NP; ++j) v[j] = f2mul(v[j], f2two(inv_y));
+      if (a.gamma_pre) weigh(wn, v);
+      put(a.n, r, v);
+      if (t == 0) a.inv_y[r] = inv_y;
+    }
+    buf ^= 2;
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 struct BwdArgs {
@@ -337,45 +507,6 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
 // Arithmetic is on packed pairs of floats.  A CTA's rows lie in one group (W
 // stays in registers), so dgamma_post's part is gate * S at the end.
 // The column sums S leave out s; it is multiplied in at the end.
-template <int DT>
-struct Pairs;   // 8 stored elements -> 4 packed pairs
-template <>
-struct Pairs<NVFP4B200_BF16> {
-  static __device__ __forceinline__ void get(const uint4* p, int stride, uint64_t (&o)[4]) {
-    const uint4 v = *p;
-    o[0] = bf16x2_to_f2(v.x); o[1] = bf16x2_to_f2(v.y); o[2] = bf16x2_to_f2(v.z); o[3] = bf16x2_to_f2(v.w);
-  }
-};
-template <>
-struct Pairs<NVFP4B200_F16> {
-  static __device__ __forceinline__ void get(const uint4* p, int stride, uint64_t (&o)[4]) {
-    const uint4 v = *p;
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      o[i] = f2pack(f.x, f.y);
-    }
-  }
-};
-template <>
-struct Pairs<NVFP4B200_F32> {
-  static __device__ __forceinline__ void get(const uint4* p, int stride, uint64_t (&o)[4]) {
-    const uint4 a = p[0], b = p[stride];
-    o[0] = ((uint64_t)a.y << 32) | a.x; o[1] = ((uint64_t)a.w << 32) | a.z;
-    o[2] = ((uint64_t)b.y << 32) | b.x; o[3] = ((uint64_t)b.w << 32) | b.z;
-  }
-};
-
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
-               : "memory");
-}
-__device__ __forceinline__ uint64_t f2two(float v) { return f2pack(v, v); }
-__device__ __forceinline__ float f2sum(uint64_t v) { return f2lo(v) + f2hi(v); }
-
-constexpr int STAGES = 3;
-
 template <int DT, int TPR, bool PRE>
 __global__ void __launch_bounds__(TPR, 512 / TPR) sandwich_bwd_staged_kernel(const BwdArgs a, int64_t parts_per_group) {
   using E = Elem<DT>;
@@ -457,8 +588,13 @@ __global__ void __launch_bounds__(TPR, 512 / TPR) sandwich_bwd_staged_kernel(con
   }
 
   int stage = 0, buf = 0;
+  float next_b = r0 < end ? __ldg(a.inv_b + r0) : 0.0f, next_y = PRE && r0 < end ? __ldg(a.inv_y + r0) : 0.0f;
   for (int64_t r = r0; r < end; ++r) {
-    const float inv_b = __ldg(a.inv_b + r), inv_y = PRE ? __ldg(a.inv_y + r) : 0.0f;
+    const float inv_b = next_b, inv_y = next_y;
+    if (r + 1 < end) {   // a row ahead, so that its latency is not exposed once per row
+      next_b = __ldg(a.inv_b + r + 1);
+      if (PRE) next_y = __ldg(a.inv_y + r + 1);
+    }
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     uint64_t t0[NP], yh[PRE ? NP : 1], bh[NP];
     uint64_t A = 0ull, B = 0ull, C = 0ull;
@@ -561,9 +697,10 @@ __global__ void __launch_bounds__(TPR, 512 / TPR) sandwich_bwd_staged_kernel(con
 }
 
 // Column sums of the partials, in CTA order.  Job 0 is dgamma_post, 1
-// dgamma_pre, 2 + g dgate of group g, each over blocks of 32 columns.  32
-// warps share a column's partials, each a contiguous run of them; the runs'
-// sums are added in order.
+// dgamma_pre, 2 + g dgate of group g.  A CTA takes 32 * V columns of a job;
+// its 16 warps share the partials, each a contiguous run of them, and the
+// runs' sums are added in order.  V = 4 where rows of partials are 16-byte
+// aligned: wide loads and a quarter of the CTAs.
 struct FinishArgs {
   const float *part, *part_gate;
   const void* gamma_post;
@@ -571,13 +708,14 @@ struct FinishArgs {
   int64_t ctas, parts_per_group;
   int d;
 };
+constexpr int FINISH_WARPS = 16;
 
-template <int DT>
-__global__ void __launch_bounds__(1024) sandwich_bwd_finish_kernel(const FinishArgs a) {
-  __shared__ float red[32][33];
-  const int col = threadIdx.x & 31, seg = threadIdx.x >> 5;
-  const int blocks = (a.d + 31) / 32;
-  const int c = (int)(blockIdx.x % blocks) * 32 + col;
+template <int DT, int V>
+__global__ void __launch_bounds__(32 * FINISH_WARPS) sandwich_bwd_finish_kernel(const FinishArgs a) {
+  __shared__ float red[FINISH_WARPS][32 * V];
+  const int lane = threadIdx.x & 31, seg = threadIdx.x >> 5;
+  const int blocks = (a.d + 32 * V - 1) / (32 * V);
+  const int c0 = (int)(blockIdx.x % blocks) * 32 * V, c = c0 + lane * V;
   const int64_t job = blockIdx.x / blocks;
   const float* p;
   float* out;
@@ -586,19 +724,30 @@ __global__ void __launch_bounds__(1024) sandwich_bwd_finish_kernel(const FinishA
   else if (job == 1) { p = a.part + a.ctas * a.d; out = a.dgamma_pre; n = a.ctas; }
   else { p = a.part_gate + (job - 2) * a.parts_per_group * a.d; out = a.dgate + (job - 2) * a.d; n = a.parts_per_group; }
   if ((job == 0 && !a.dgamma_post) || (job == 1 && !a.dgamma_pre)) return;
-  const int64_t per = (n + 31) / 32, lo = per * seg, hi = imin64(n, lo + per);
-  float s = 0.0f;
-  if (c < a.d) {
-#pragma unroll 4
-    for (int64_t i = lo; i < hi; ++i) s += __ldg(p + i * a.d + c);
-  }
-  red[seg][col] = s;
-  __syncthreads();
-  if (seg == 0 && c < a.d) {
+  const int64_t per = (n + FINISH_WARPS - 1) / FINISH_WARPS, lo = per * seg, hi = imin64(n, lo + per);
+  float s[V];
 #pragma unroll
-    for (int i = 1; i < 32; ++i) s += red[i][col];
-    if (job >= 2 && a.gamma_post) s *= Elem<DT>::get(static_cast<const typename Elem<DT>::Raw*>(a.gamma_post) + c);
-    out[c] = s;
+  for (int j = 0; j < V; ++j) s[j] = 0.0f;
+  if (c < a.d) {   // V = 4: d % 4 == 0
+#pragma unroll 8
+    for (int64_t i = lo; i < hi; ++i) {
+      if (V == 4) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(p + i * a.d + c));
+        s[0] += v.x; s[V > 1 ? 1 : 0] += v.y; s[V > 2 ? 2 : 0] += v.z; s[V > 3 ? 3 : 0] += v.w;
+      } else {
+        s[0] += __ldg(p + i * a.d + c);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) red[seg][lane * V + j] = s[j];
+  __syncthreads();
+  for (int k = threadIdx.x; k < 32 * V && c0 + k < a.d; k += 32 * FINISH_WARPS) {
+    float u = red[0][k];
+#pragma unroll
+    for (int i = 1; i < FINISH_WARPS; ++i) u += red[i][k];
+    if (job >= 2 && a.gamma_post) u *= Elem<DT>::get(static_cast<const typename Elem<DT>::Raw*>(a.gamma_post) + c0 + k);
+    out[c0 + k] = u;
   }
 }
 
@@ -683,7 +832,19 @@ int nvfp4b200_sandwich_norm(const void* b, const void* x, const void* gamma_post
   return norm::by_type(dtype, vec, [&](auto dt, auto v) {
     return norm::by_width((int)d, [&](auto tpr) {
       constexpr int T = decltype(tpr)::value, THREADS = T < 256 ? 256 : T, GROUPS = THREADS / T;
+      constexpr int DT = decltype(dt)::value;
       const int64_t want = ceil_div(rows, GROUPS);
+      // the staged kernel where its ring fits: 195 -> NNN us at 16384 x 8192 bf16 with the next norm
+      constexpr int smem = norm::STAGES * 2 * THREADS * norm::CPT * norm::dtype_size<DT>();
+      if constexpr (decltype(v)::value && smem <= norm::MAX_SMEM) {
+        auto* fn = norm::sandwich_fwd_staged_kernel<DT, T>;
+        if (smem > 32 * 1024 &&   // with the static arrays, past the default limit
+            cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+          return (int)NVFP4B200_ERR_CUDA;
+        const int per_sm = std::max(1, std::min(norm::MAX_SMEM / smem, T < 512 ? 4 : 1024 / T));
+        fn<<<(unsigned)std::min<int64_t>(want, (int64_t)sm_count_current() * per_sm), THREADS, smem, st>>>(a);
+        return launch_status();
+      }
       const unsigned grid = (unsigned)std::min<int64_t>(want, (int64_t)sm_count_current() * (2048 / THREADS));
       norm::sandwich_fwd_kernel<decltype(dt)::value, decltype(v)::value, T><<<grid, THREADS, 0, st>>>(a);
       return launch_status();
@@ -764,7 +925,12 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
     if (r) return r;
     if (!dgamma_post && !dgamma_pre && !dgate) return (int)NVFP4B200_OK;
     const int64_t jobs = dgate && sp.parts_per_group > 1 ? groups + 2 : 2;
-    norm::sandwich_bwd_finish_kernel<decltype(dt)::value><<<(unsigned)(jobs * ceil_div(d, 32)), 1024, 0, st>>>(f);
+    if (d % 4 == 0 && aligned(ws, 16))
+      norm::sandwich_bwd_finish_kernel<decltype(dt)::value, 4>
+          <<<(unsigned)(jobs * ceil_div(d, 128)), 32 * norm::FINISH_WARPS, 0, st>>>(f);
+    else
+      norm::sandwich_bwd_finish_kernel<decltype(dt)::value, 1>
+          <<<(unsigned)(jobs * ceil_div(d, 32)), 32 * norm::FINISH_WARPS, 0, st>>>(f);
     return launch_status();
   });
 }
