@@ -23,6 +23,8 @@ int check_device();
 
 // Returns and clears the quantizer kernels' device error word (0 if none).
 int take_quant_device_error();
+// The same for the norm kernels.
+int take_norm_device_error();
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 

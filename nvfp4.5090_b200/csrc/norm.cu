@@ -24,6 +24,7 @@
 // fixed order (rows in a CTA, CTAs in a second kernel), never by atomics.
 //
 // Bound: HBM, one read of each input and one write of each output.
+#include "bulk.cuh"
 #include "vec.cuh"
 
 #include <algorithm>
@@ -496,63 +497,59 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
   }
 }
 
-// The same backward with the rows staged ahead in shared memory: every thread
-// copies its own columns of dy, dn, b and y (cp.async, 16 bytes each) into a
-// ring of STAGES rows and reads back only what it copied, so the ring needs
-// no barrier.  The row's two means come from one exchange of three sums:
-// with W = s * gate * gamma_post and t0 = dy + inv_y * v,
+// The same backward with the rows staged ahead in shared memory: one thread
+// copies whole rows of dy, dn, b and y into a ring of STAGES rows (bulk
+// copies on one barrier per row) and refills a row's place right after the
+// barrier of the row's reduction, by when every thread has read it.  The
+// row's two means come from that one exchange of three sums: with
+// W = s * gate * gamma_post and t0 = dy + inv_y * v,
 //     A = sum v yh,  B = sum W bh t0,  C = sum W bh yh
 //     m1 = A / d,    m2 = (B - inv_y * m1 * C) / d
 //     t = t0 - inv_y * m1 * yh,    db = inv_b * (W t - m2 bh).
 // Arithmetic is on packed pairs of floats.  A CTA's rows lie in one group (W
-// stays in registers), so dgamma_post's part is gate * S at the end.
-// The column sums S leave out s; it is multiplied in at the end.
+// stays in registers), so dgamma_post's part is gate * S at the end.  The
+// column sums S leave out s; it is multiplied in at the end.
+// What bounds it is the instruction stream of 16 warps per SM at 128 registers.
+__device__ int g_norm_error = 0;
+
 template <int DT, int TPR, bool PRE>
 __global__ void __launch_bounds__(TPR, 512 / TPR) sandwich_bwd_staged_kernel(const BwdArgs a, int64_t parts_per_group) {
   using E = Elem<DT>;
   using Raw = typename E::Raw;
-  constexpr int Q = (int)sizeof(Raw) * 8 / 16;    // 16-byte pieces per 8 elements
   constexpr int NT = PRE ? 4 : 2;                 // tensors: dy, b [, dn, y]
   constexpr int NP = CPT / 2;                     // packed pairs per thread
-  extern __shared__ __align__(16) uint4 ring[];   // [STAGES][NT][VPT * Q][TPR]
-  __shared__ float red[2][3][TPR / 32];
+  constexpr int W4 = (TPR / 32 + 3) / 4;          // 16-byte words of one sum's warp parts
+  extern __shared__ __align__(16) uint8_t row_ring[];   // [STAGES][NT][d]
+  __shared__ __align__(16) float red[2][3][4 * W4];
+  __shared__ __align__(8) uint64_t full[STAGES];
+  __shared__ int gave_up;
   const int t = threadIdx.x;
   const float inv_d = 1.0f / (float)a.d;
+  const int row_bytes = a.d * (int)sizeof(Raw);
   const int64_t g = blockIdx.x / parts_per_group, p = blockIdx.x % parts_per_group;
   const int64_t r0 = g * a.rows_per_gate + p * a.rows_per_cta;
-  const int64_t end = imin64(r0 + a.rows_per_cta, (g + 1) * a.rows_per_gate);
+  const int rows = (int)(imin64(r0 + a.rows_per_cta, (g + 1) * a.rows_per_gate) - r0);
 
-  auto slot = [&](int stage, int tensor, int piece) { return ring + ((stage * NT + tensor) * (VPT * Q) + piece) * TPR + t; };
-  auto fetch = [&](int64_t r, int stage) {
-    if (r < end) {
-      const void* base[4] = {a.dy, a.b, a.dn, a.y};
-      const int64_t ld[4] = {a.ld_dy, a.ldb, a.ld_dn, a.ldy};
-#pragma unroll
-      for (int k = 0; k < NT; ++k) {
-        if (k == 0 && !a.dy) continue;
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-          const int c = column<true, TPR>(t, 8 * i);
-          if (c < a.d) {
-            const Raw* src = static_cast<const Raw*>(base[k]) + r * ld[k] + c;
-#pragma unroll
-            for (int q = 0; q < Q; ++q) cp_async16(slot(stage, k, i * Q + q), reinterpret_cast<const uint4*>(src) + q);
-          }
-        }
-      }
+  auto fetch = [&](int i, int stage) {   // one thread: row r0 + i into a stage
+    if (i >= rows) return;
+    uint8_t* dst = row_ring + (size_t)stage * NT * row_bytes;
+    bulk::expect(&full[stage], (uint32_t)((NT - (a.dy ? 0 : 1)) * row_bytes));
+    const int64_t r = r0 + i;
+    if (a.dy) bulk::copy(dst, static_cast<const Raw*>(a.dy) + r * a.ld_dy, row_bytes, &full[stage]);
+    bulk::copy(dst + row_bytes, static_cast<const Raw*>(a.b) + r * a.ldb, row_bytes, &full[stage]);
+    if (PRE) {
+      bulk::copy(dst + 2 * row_bytes, static_cast<const Raw*>(a.dn) + r * a.ld_dn, row_bytes, &full[stage]);
+      bulk::copy(dst + 3 * row_bytes, static_cast<const Raw*>(a.y) + r * a.ldy, row_bytes, &full[stage]);
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // columns past the end stay zero in every stage
-#pragma unroll
-  for (int i = 0; i < VPT; ++i)
-    if (column<true, TPR>(t, 8 * i) >= a.d || !a.dy)
-      for (int st = 0; st < STAGES; ++st)
-        for (int k = 0; k < NT; ++k)
-          if (column<true, TPR>(t, 8 * i) >= a.d || k == 0)
-            for (int q = 0; q < Q; ++q) *slot(st, k, i * Q + q) = make_uint4(0, 0, 0, 0);
-#pragma unroll
-  for (int st = 0; st < STAGES - 1; ++st) fetch(r0 + st, st);
+  if (t < 3 * 4 * W4 * 2) (&red[0][0][0])[t] = 0.0f;   // warp parts past the last stay zero
+  if (t == 0) {
+    gave_up = 0;
+    bulk::init(full, STAGES);
+  }
+  __syncthreads();
+  if (t == 0)
+    for (int st = 0; st < STAGES; ++st) fetch(st, st);
 
   uint64_t W[NP], gpre[PRE ? NP : 1], S[NP], pre[PRE ? NP : 1];
   {
@@ -587,33 +584,48 @@ __global__ void __launch_bounds__(TPR, 512 / TPR) sandwich_bwd_staged_kernel(con
     }
   }
 
+  Raw *dx = static_cast<Raw*>(a.dx) + r0 * a.d, *db = static_cast<Raw*>(a.db) + r0 * a.d;
+  const float *ib = a.inv_b + r0, *iy = PRE ? a.inv_y + r0 : nullptr;
+  float next_b = __ldg(ib), next_y = PRE ? __ldg(iy) : 0.0f;
   int stage = 0, buf = 0;
-  float next_b = r0 < end ? __ldg(a.inv_b + r0) : 0.0f, next_y = PRE && r0 < end ? __ldg(a.inv_y + r0) : 0.0f;
-  for (int64_t r = r0; r < end; ++r) {
+  uint32_t parity = 0;
+  for (int i = 0; i < rows; ++i) {
     const float inv_b = next_b, inv_y = next_y;
-    if (r + 1 < end) {   // a row ahead, so that its latency is not exposed once per row
-      next_b = __ldg(a.inv_b + r + 1);
-      if (PRE) next_y = __ldg(a.inv_y + r + 1);
+    if (i + 1 < rows) {   // a row ahead, so that its latency is not exposed once per row
+      next_b = __ldg(ib + i + 1);
+      if (PRE) next_y = __ldg(iy + i + 1);
     }
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    if (!bulk::wait(&full[stage], parity)) gave_up = 1;
+    const uint8_t* src = row_ring + (size_t)stage * NT * row_bytes;
+    auto get = [&](int tensor, int c, uint64_t (&o)[4]) {
+      Pairs<DT>::get(reinterpret_cast<const uint4*>(src + tensor * row_bytes + c * (int)sizeof(Raw)), 1, o);
+    };
     uint64_t t0[NP], yh[PRE ? NP : 1], bh[NP];
     uint64_t A = 0ull, B = 0ull, C = 0ull;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      uint64_t x[4], z[4];
-      Pairs<DT>::get(slot(stage, 0, i * Q), TPR, x);
-      Pairs<DT>::get(slot(stage, 1, i * Q), TPR, z);
+    for (int h = 0; h < VPT; ++h) {
+      const int c = column<true, TPR>(t, 8 * h);
+      uint64_t x[4] = {0ull, 0ull, 0ull, 0ull}, z[4] = {0ull, 0ull, 0ull, 0ull};
+      if (c < a.d) {
+        if (a.dy) get(0, c, x);
+        get(1, c, z);
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        t0[4 * i + j] = x[j];
-        bh[4 * i + j] = f2mul(z[j], f2two(inv_b));
+        t0[4 * h + j] = x[j];
+        bh[4 * h + j] = f2mul(z[j], f2two(inv_b));
       }
       if (PRE) {
-        Pairs<DT>::get(slot(stage, 2, i * Q), TPR, x);
-        Pairs<DT>::get(slot(stage, 3, i * Q), TPR, z);
+        if (c < a.d) {
+          get(2, c, x);
+          get(3, c, z);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = z[j] = 0ull;
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int k = 4 * i + j;
+          const int k = 4 * h + j;
           yh[k] = f2mul(z[j], f2two(inv_y));
           pre[k] = f2fma(x[j], yh[k], pre[k]);
           const uint64_t v = f2mul(x[j], gpre[k]);
@@ -623,42 +635,45 @@ __global__ void __launch_bounds__(TPR, 512 / TPR) sandwich_bwd_staged_kernel(con
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int k = 4 * i + j;
+        const int k = 4 * h + j;
         const uint64_t wb = f2mul(W[k], bh[k]);
         B = f2fma(wb, t0[k], B);
         if (PRE) C = f2fma(wb, yh[k], C);
       }
     }
-    // this stage's slots are read: fetch the row STAGES - 1 ahead into the one read before it
-    fetch(r + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
     float sums[3] = {f2sum(B), PRE ? f2sum(A) : 0.0f, PRE ? f2sum(C) : 0.0f};
 #pragma unroll
-    for (int k = 0; k < (PRE ? 3 : 1); ++k) {
+    for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sums[k] += __shfl_xor_sync(0xffffffffu, sums[k], o);
-      if (TPR > 32) {
-        if ((t & 31) == 0) red[buf][k][t >> 5] = sums[k];
-      }
+      for (int k = 0; k < (PRE ? 3 : 1); ++k) sums[k] += __shfl_xor_sync(0xffffffffu, sums[k], o);
+    if ((t & 31) == 0) {
+#pragma unroll
+      for (int k = 0; k < (PRE ? 3 : 1); ++k) red[buf][k][t >> 5] = sums[k];
     }
+    __syncthreads();
+    if (t == 0) fetch(i + STAGES, stage);
     if (TPR > 32) {
-      __syncthreads();
 #pragma unroll
       for (int k = 0; k < (PRE ? 3 : 1); ++k) {
         float u = 0.0f;
 #pragma unroll
-        for (int w = 0; w < TPR / 32; ++w) u += red[buf][k][w];
+        for (int w = 0; w < W4; ++w) {
+          const float4 q = reinterpret_cast<const float4*>(red[buf][k])[w];
+          u += (q.x + q.y) + (q.z + q.w);
+        }
         sums[k] = u;
       }
-      buf ^= 1;
     }
+    buf ^= 1;
+    if (gave_up) break;   // set before the barrier: every thread sees it
     const float m1 = PRE ? sums[1] * inv_d : 0.0f;
     const float m2 = (PRE ? fmaf(-inv_y * m1, sums[2], sums[0]) : sums[0]) * inv_d;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
+    for (int h = 0; h < VPT; ++h) {
       float dxv[8], dbv[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int k = 4 * i + j;
+        const int k = 4 * h + j;
         const uint64_t tt = PRE ? f2fma(yh[k], f2two(-inv_y * m1), t0[k]) : t0[k];
         S[k] = f2fma(tt, bh[k], S[k]);
         const uint64_t d = f2mul(f2fma(bh[k], f2two(-m2), f2mul(W[k], tt)), f2two(inv_b));
@@ -666,15 +681,24 @@ __global__ void __launch_bounds__(TPR, 512 / TPR) sandwich_bwd_staged_kernel(con
         dxv[2 * j] = f2lo(e); dxv[2 * j + 1] = f2hi(e);
         dbv[2 * j] = f2lo(d); dbv[2 * j + 1] = f2hi(d);
       }
-      const int c = column<true, TPR>(t, 8 * i);
+      const int c = column<true, TPR>(t, 8 * h);
       if (c < a.d) {
-        E::store(static_cast<Raw*>(a.dx) + r * a.d + c, E::pack(dxv));
-        E::store(static_cast<Raw*>(a.db) + r * a.d + c, E::pack(dbv));
+        E::store(dx + c, E::pack(dxv));
+        E::store(db + c, E::pack(dbv));
       }
     }
-    stage = stage == STAGES - 1 ? 0 : stage + 1;
+    dx += a.d;
+    db += a.d;
+    if (++stage == STAGES) {
+      stage = 0;
+      parity ^= 1u;
+    }
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (gave_up && t == 0) {
+    // a copy did not arrive in time: report it, and leave no copy in flight behind
+    atomicExch(&g_norm_error, NVFP4B200_ERR_TIMEOUT);
+    for (int st = 0; st < STAGES; ++st) bulk::wait(&full[st], parity ^ (st < stage ? 1u : 0u));
+  }
 
   // partial column sums: s * S, gate * s * S and dgamma_pre
   float w[CPT];
@@ -799,6 +823,14 @@ static Split split_rows(int64_t rows, int64_t groups, int64_t d, int sms) {
 }
 
 }  // namespace norm
+
+int take_norm_device_error() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, norm::g_norm_error, sizeof(int)) != cudaSuccess) return NVFP4B200_ERR_CUDA;
+  if (v && cudaMemcpyToSymbol(norm::g_norm_error, &zero, sizeof(int)) != cudaSuccess) return NVFP4B200_ERR_CUDA;
+  return v;
+}
+
 }  // namespace nvfp4b200
 
 using namespace nvfp4b200;
@@ -834,7 +866,7 @@ int nvfp4b200_sandwich_norm(const void* b, const void* x, const void* gamma_post
       constexpr int T = decltype(tpr)::value, THREADS = T < 256 ? 256 : T, GROUPS = THREADS / T;
       constexpr int DT = decltype(dt)::value;
       const int64_t want = ceil_div(rows, GROUPS);
-      // the staged kernel where its ring fits: 195 -> NNN us at 16384 x 8192 bf16 with the next norm
+      // the staged kernel where its ring fits: 195 -> 176 us at 16384 x 8192 bf16 with the next norm
       constexpr int smem = norm::STAGES * 2 * THREADS * norm::CPT * norm::dtype_size<DT>();
       if constexpr (decltype(v)::value && smem <= norm::MAX_SMEM) {
         auto* fn = norm::sandwich_fwd_staged_kernel<DT, T>;
@@ -906,9 +938,9 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
     const int r = norm::by_width((int)d, [&](auto tpr) {
       constexpr int T = decltype(tpr)::value, DT = decltype(dt)::value;
       // the staged kernel where its ring fits and a CTA's rows have one gate:
-      // 346 -> 185 us at 16000 x 4096 bf16 with 8 gates and the next norm
+      // 346 -> 162 us at 16000 x 4096 bf16 with 8 gates and the next norm
       if constexpr (decltype(v)::value && T <= 512) {
-        const int smem = norm::STAGES * (dn ? 4 : 2) * T * norm::CPT * norm::dtype_size<DT>();
+        const int smem = norm::STAGES * (dn ? 4 : 2) * (int)d * norm::dtype_size<DT>();
         if (smem <= norm::MAX_SMEM && (!gate || sp.parts_per_group > 1)) {
           auto* fn = dn ? norm::sandwich_bwd_staged_kernel<DT, T, true> : norm::sandwich_bwd_staged_kernel<DT, T, false>;
           if (smem > 32 * 1024 &&   // with the static arrays, past the default limit
