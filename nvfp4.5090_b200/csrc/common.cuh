@@ -23,8 +23,12 @@ int check_device();
 
 // Returns and clears the quantizer kernels' device error word (0 if none).
 int take_quant_device_error();
-// The same for the norm kernels.
+// The same for the norm kernels and the few-token MXFP4 product.
 int take_norm_device_error();
+int take_mxlin_device_error();
+
+// SM count of the current device, looked up once per device.
+int sm_count_current();
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 

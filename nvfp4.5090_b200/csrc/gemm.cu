@@ -1398,9 +1398,11 @@ int nvfp4b200_get_device_error(int* out) {
   const int qe = take_quant_device_error();
   if (qe == NVFP4B200_ERR_CUDA) return qe;
   if (*out == 0) *out = qe;
-  const int ne = take_norm_device_error();
-  if (ne == NVFP4B200_ERR_CUDA) return ne;
-  if (*out == 0) *out = ne;
+  for (int (*take)() : {take_norm_device_error, take_mxlin_device_error}) {
+    const int e = take();
+    if (e == NVFP4B200_ERR_CUDA) return e;
+    if (*out == 0) *out = e;
+  }
   if (*out != 0) {   // a launch gave up: make sure no tile counter is left dirty (the device is idle here)
     static const uint32_t zeros[gemm::SCHED_SLOTS][2] = {};
     if (cudaMemcpyToSymbol(gemm::g_tile_sched, zeros, sizeof(zeros)) != cudaSuccess) return NVFP4B200_ERR_CUDA;

@@ -95,6 +95,8 @@ template <int DT, bool ROWS, bool COLS, bool SCALED>
 __global__ void __launch_bounds__(QTHREADS) mx_quant_kernel(const QuantArgs a) {
   using E = Elem<DT>;
   using Raw = typename E::Raw;
+  // a few-token product may follow as this kernel's programmatic dependent
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(16) uint8_t smem[];
   Raw* tile = reinterpret_cast<Raw*>(smem);                                      // COLS: [128][128]
   uint8_t* stage = smem + (COLS ? TILE * TILE * sizeof(Raw) : 0);                // COLS: [128][64]
@@ -212,7 +214,7 @@ template <int DT, bool ROWS, bool COLS, bool SCALED>
 static int launch_quant(const QuantArgs& a, cudaStream_t st) {
   const int smem = COLS ? TILE * TILE * (int)sizeof(typename Elem<DT>::Raw) + TILE * 64 : 0;
   auto* fn = mx_quant_kernel<DT, ROWS, COLS, SCALED>;
-  if (smem > 48 * 1024 &&
+  if (smem > 32 * 1024 &&   // with the static arrays, past the default limit
       cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return NVFP4B200_ERR_CUDA;
   fn<<<(unsigned)(a.row_tiles * a.col_tiles), QTHREADS, smem, st>>>(a);
@@ -266,6 +268,12 @@ __global__ void __launch_bounds__(256) mx_dequant_kernel(const uint8_t* __restri
 }
 
 }  // namespace mx
+
+// Checked rows quantizer of bf16 x for the few-token product.
+int mx_quant_rows_async(const void* x, void* q, void* s, int64_t rows, int64_t cols, int64_t ldx, cudaStream_t st) {
+  return nvfp4b200_mx_quant(x, NVFP4B200_BF16, nullptr, nullptr, q, s, nullptr, nullptr, rows, cols, ldx, (void*)st);
+}
+
 }  // namespace nvfp4b200
 
 using namespace nvfp4b200;

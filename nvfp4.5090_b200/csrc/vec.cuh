@@ -99,7 +99,4 @@ struct Elem<NVFP4B200_F32> {
 inline bool valid_dtype(int dt) { return dt == NVFP4B200_BF16 || dt == NVFP4B200_F32 || dt == NVFP4B200_F16; }
 inline int dtype_bytes(int dt) { return dt == NVFP4B200_F32 ? 4 : 2; }
 
-// SM count of the current device, looked up once per device.
-int sm_count_current();
-
 }  // namespace nvfp4b200

@@ -435,11 +435,24 @@ def mx_linear(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, bias: Optiona
     _check_bf16(x, "mx_linear")
     n, k = qw.shape[0], 2 * qw.shape[1]
     _require(x.shape[-1] == k, f"K mismatch: x has {x.shape[-1]}, W has {k}")
-    x2 = x.reshape(-1, k)
-    if x2.shape[0] == 0:
-        return torch.empty((*x.shape[:-1], n), device=x.device, dtype=x.dtype)
-    q, s = mx_quantize(x2)
-    return mx_gemm(q, s, qw, sw, bias=bias).reshape(*x.shape[:-1], n)
+    if k == 0 or k % 32 or n % 8:
+        raise RuntimeError("mx_linear needs K divisible by 32 and N by 8")
+    dev = x.get_device()
+    if (qw.get_device() != dev or sw.get_device() != dev or not qw.is_contiguous() or not sw.is_contiguous()
+            or sw.numel() != (n + 127) // 128 * 128 * ((k + 127) // 128 * 4)):
+        raise RuntimeError("the weight is contiguous q [n, k/2] and its padded swizzled scales on x's device")
+    if bias is not None:
+        _check_bf16(bias, "bias")
+        _require(bias.numel() == n and bias.get_device() == dev, "bias is bf16 [n]")
+        bias = bias.contiguous()
+    x2 = _float_matrix(x if x.dim() == 2 else x.reshape(-1, k))
+    m = x2.shape[0]
+    y = torch.empty((*x.shape[:-1], n), device=x.device, dtype=torch.bfloat16)
+    if m and n:
+        qx, sx = _mx_pair(m, k, x.device, None)
+        _run(x2, "nvfp4b200_mx_linear", x2.data_ptr(), qw.data_ptr(), sw.data_ptr(), _ptr(bias), qx.data_ptr(),
+             sx.data_ptr(), y.data_ptr(), m, n, k, max(x2.stride(0), k))
+    return y
 
 
 # ----------------------------------------------------------------------------
