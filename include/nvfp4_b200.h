@@ -248,10 +248,15 @@ int nvfp4b200_mx_gemm(const void* a, const void* b, const void* sfa, const void*
                       const void* residual, void* d, int d_dtype, int accumulate, int epilogue, int64_t m, int64_t n,
                       int64_t k, int64_t ldd, void* stream);
 
+/* 1 where nvfp4b200_mx_linear quantizes the tokens inside its product and so
+ * takes no workspace (up to 16 tokens, k <= 32768), else 0. */
+int nvfp4b200_mx_linear_fused(int64_t m, int64_t n, int64_t k);
+
 /* y = Q(x) . W^T + bias for W held in MXFP4: x bf16 [m, k] (row stride ldx) is
- * quantized along k into qx [m, k/2] and sfx (as nvfp4b200_mx_quant's q and s),
- * then multiplied: up to 128 tokens by a kernel that streams the weights over
- * all SMs, more by nvfp4b200_mx_gemm.  qw [n, k/2], sfw: the weight; bias bf16
+ * quantized along k, into qx [m, k/2] and sfx (as nvfp4b200_mx_quant's q and s;
+ * may be NULL where nvfp4b200_mx_linear_fused says so), and multiplied: up to
+ * 128 tokens by a kernel that streams the weights over all SMs, more by
+ * nvfp4b200_mx_gemm.  qw [n, k/2], sfw: the weight; bias bf16
  * [n] or NULL; y bf16 [m, n].  k % 32 == 0, n % 8 == 0. */
 int nvfp4b200_mx_linear(const void* x, const void* qw, const void* sfw, const void* bias, void* qx, void* sfx,
                         void* y, int64_t m, int64_t n, int64_t k, int64_t ldx, void* stream);

@@ -51,6 +51,7 @@ SIGNATURES = {
     "nvfp4b200_mx_quant": [c_void_p, c_int] + [c_void_p] * 6 + [c_i64] * 3 + [c_void_p],
     "nvfp4b200_mx_dequant": [c_void_p] * 3 + [c_int, c_i64, c_i64, c_void_p],
     "nvfp4b200_mx_gemm": [c_void_p] * 7 + [c_int] * 3 + [c_i64] * 4 + [c_void_p],
+    "nvfp4b200_mx_linear_fused": [c_i64] * 3,
     "nvfp4b200_mx_linear": [c_void_p] * 7 + [c_i64] * 4 + [c_void_p],
     "nvfp4b200_grad_norm": [c_void_p] * 5 + [c_int, c_int, c_float, c_float, c_void_p, c_i64] + [c_void_p] * 4,
     "nvfp4b200_grad_norm_finish": [c_void_p, c_i64, c_int, c_float, c_float, c_void_p, c_void_p, c_void_p],

@@ -11,10 +11,10 @@ constexpr long long WAIT_CYCLES = 4000000000ll;   // about 2 s
 
 __device__ __forceinline__ uint32_t addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-// One thread, before a __syncthreads(): `n` barriers that one arrival completes.
-__device__ __forceinline__ void init(uint64_t* bars, int n) {
+// One thread, before a __syncthreads(): `n` barriers that `count` arrivals complete.
+__device__ __forceinline__ void init(uint64_t* bars, int n, uint32_t count = 1) {
   for (int i = 0; i < n; ++i)
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(addr(bars + i)) : "memory");
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(addr(bars + i)), "r"(count) : "memory");
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
 

@@ -9,22 +9,27 @@
 // cluster, so that 128-row tiles x K parts fill the SMs.  The parts' fp32 sums
 // meet through distributed shared memory in one fixed order.
 //
-//   grid (tiles * parts, token blocks), cluster (parts, 1): CTA rank r of a
-//     cluster takes every stage (256 k) of its share of K for 128 weight rows;
+//   grid (tiles * parts), cluster (parts): CTA rank r of a cluster takes every
+//     stage (256 k) of its share of K for 128 weight rows;
 //   warp 0      producer: weights (one 128-byte-swizzled TMA box of 128 rows x
-//               128 bytes, and their 2 scale atoms) and tokens (N x 128 bytes,
-//               2 atoms) per stage, into a ring of up to 8 stages;
+//               128 bytes, and their 2 scale atoms) per stage into a ring of up
+//               to 8 stages, and the quantized tokens (N x 128 bytes, 2 atoms);
 //   warp 1      MMA issuer: 4 tcgen05.mma.cta_group::1 kind::mxf4 128 x N x 64
 //               per stage and the copies of the scale atoms to TMEM;
-//   all 4 warps epilogue: TMEM -> shared memory as [token][row]; after a
+//   all 8 warps epilogue: TMEM -> shared memory as [token][row]; after a
 //               cluster barrier the CTA of rank r adds up the parts of tokens
 //               r, r + parts, .. and writes them with the bias.
-// The tokens are quantized by the row quantizer just before; this kernel is
-// its programmatic dependent, so the weights' first stages are under way (they
-// need nothing of it) while the tokens are being quantized.
+// Up to 16 tokens are quantized here (FUSED): warps 2-7 read a token's 256 k
+// of a stage, a warp each, and write nibbles and scale codes where the MMA
+// reads them, while the weights are still under way; one launch, no
+// workspace.  More tokens would make every 128-row tile's CTA spend longer on
+// them than on its weights: they are quantized once by the row quantizer just
+// before, and this kernel is its programmatic dependent, so its first weights
+// load meanwhile.
 //
 // Every wait is bounded; a timeout sets the library's device error word.
 #include "bulk.cuh"
+#include "mx.cuh"
 
 #include <cuda.h>
 
@@ -43,13 +48,17 @@ constexpr int TILE_ROWS = 128;
 constexpr int BK = 256, BK_BYTES = BK / 2;
 constexpr int A_BYTES = TILE_ROWS * BK_BYTES;     // 16 KB
 constexpr int SF_BYTES = 1024;                    // two atoms: 128 rows x 8 scales
-constexpr int THREADS = 128;
+constexpr int THREADS = 256;
+constexpr int FUSED_TOKENS = 16;
+constexpr int FUSED_STEPS = 16;                   // stages of tokens that stay in shared memory (48 KB)
 constexpr int MAX_STAGES = 8;
 constexpr int MAX_PARTS = 8;
 constexpr int SMEM_SM = 227 * 1024;
 
 struct Args {
-  const uint8_t *sfw, *sfx;     // scale atoms of the weights and of the tokens
+  const uint8_t *sfw, *sfx;     // scale atoms of the weights and (not FUSED) of the tokens
+  const uint16_t* x;            // FUSED: bf16 [m, k], row stride ldx
+  int64_t ldx;
   const uint16_t* bias;         // bf16 [n] or null
   uint16_t* y;                  // bf16 [m, n]
   int64_t m, n, k;
@@ -71,11 +80,11 @@ __device__ __forceinline__ uint32_t cluster_size() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t local_addr, uint32_t rank) {
-  float v;
+__device__ __forceinline__ float4 ld_cluster(uint32_t local_addr, uint32_t rank) {
+  float4 v;
   asm volatile(
-      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
-      : "=f"(v)
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
       : "r"(local_addr), "r"(rank)
       : "memory");
   return v;
@@ -126,38 +135,42 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "memory");
 }
 
-template <int N>
-constexpr int stage_bytes() { return A_BYTES + N * BK_BYTES + 2 * SF_BYTES; }
+// Ring stage: weights, and unless they are quantized here the tokens, each with scale atoms.
+template <int N, bool FUSED>
+constexpr int stage_bytes() { return A_BYTES + SF_BYTES + (FUSED ? 0 : N * BK_BYTES + SF_BYTES); }
 template <int N>
 constexpr int tmem_cols() { return 2 * N; }   // N accumulator columns, 8 + 8 of scales; a power of two, at least 32
 
-template <int N>
+template <int N, bool FUSED>
 __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constant__ CUtensorMap wmap,
                                                             const __grid_constant__ CUtensorMap xmap, const Args a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  // ring: operands of every stage (1024-byte aligned), then the scales
-  uint8_t* s_a = smem;
-  uint8_t* s_b = s_a + a.stages * A_BYTES;
-  uint8_t* s_sfa = s_b + a.stages * N * BK_BYTES;
-  uint8_t* s_sfb = s_sfa + a.stages * SF_BYTES;
-  __shared__ __align__(8) uint64_t full[MAX_STAGES], empty[MAX_STAGES], done;
+  __shared__ __align__(8) uint64_t full[MAX_STAGES], empty[MAX_STAGES], tok[FUSED_STEPS], done;
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank(), parts = (int)cluster_size();
   const int tile = blockIdx.x / parts;
-  const int tok0 = blockIdx.y * N;
   const int k_lo = (int)((int64_t)a.k_stages * rank / parts), k_hi = (int)((int64_t)a.k_stages * (rank + 1) / parts);
   const int steps = k_hi - k_lo;
+  // weights of every stage and tokens (1024-byte aligned), then the scales; the
+  // tokens sit in the ring, or (FUSED) all steps of them stay
+  const int tok_slots = FUSED ? steps : a.stages;
+  uint8_t* s_a = smem;
+  uint8_t* s_b = s_a + a.stages * A_BYTES;
+  uint8_t* s_sfa = s_b + tok_slots * N * BK_BYTES;
+  uint8_t* s_sfb = s_sfa + a.stages * SF_BYTES;
 
   if (threadIdx.x == 0) {
     gave_up = 0;
     bulk::init(full, MAX_STAGES);
     bulk::init(empty, MAX_STAGES);
     bulk::init(&done, 1);
+    if (FUSED)
+      for (int i = 0; i < FUSED_STEPS; ++i) bulk::init(tok + i, 1, (uint32_t)a.m);
     asm volatile("prefetch.tensormap [%0];" ::"l"(&wmap) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&xmap) : "memory");
+    if (!FUSED) asm volatile("prefetch.tensormap [%0];" ::"l"(&xmap) : "memory");
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bulk::addr(&tmem_slot)),
@@ -176,19 +189,21 @@ __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constan
     auto sf_bytes = [&](int i) { return (uint32_t)min(2, a.atoms - 2 * (k_lo + i)) * 512u; };
     auto weights = [&](int i, int st) {
       const uint32_t sf = sf_bytes(i);
-      bulk::expect(&full[st], (uint32_t)(A_BYTES + N * BK_BYTES) + 2 * sf);
+      bulk::expect(&full[st], (uint32_t)A_BYTES + sf + (FUSED ? 0u : N * BK_BYTES + sf));
       tma_2d(s_a + st * A_BYTES, &wmap, &full[st], (k_lo + i) * BK_BYTES, tile * TILE_ROWS);
       bulk::copy(s_sfa + st * SF_BYTES, a.sfw + ((int64_t)tile * a.atoms + 2 * (k_lo + i)) * 512, sf, &full[st]);
     };
     auto tokens = [&](int i, int st) {
-      tma_2d(s_b + st * N * BK_BYTES, &xmap, &full[st], (k_lo + i) * BK_BYTES, tok0);
-      bulk::copy(s_sfb + st * SF_BYTES, a.sfx + ((int64_t)(tok0 / 128) * a.atoms + 2 * (k_lo + i)) * 512, sf_bytes(i),
-                 &full[st]);
+      if (FUSED) return;
+      tma_2d(s_b + st * N * BK_BYTES, &xmap, &full[st], (k_lo + i) * BK_BYTES, 0);
+      bulk::copy(s_sfb + st * SF_BYTES, a.sfx + (int64_t)2 * (k_lo + i) * 512, sf_bytes(i), &full[st]);
     };
     const int first = min(steps, a.stages);
     for (int i = 0; i < first; ++i) weights(i, i);
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // the tokens are quantized from here on
-    for (int i = 0; i < first; ++i) tokens(i, i);
+    if (!FUSED) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");   // the tokens are quantized from here on
+      for (int i = 0; i < first; ++i) tokens(i, i);
+    }
     issued = first;
     int st = 0;
     uint32_t phase = 0;
@@ -212,15 +227,16 @@ __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constan
     bool ok = true;
     const uint32_t sfa = tmem + N, sfb = sfa + 8;
     for (int i = 0; i < steps; ++i) {
-      if (!bulk::wait(&full[st], phase)) {
+      if ((FUSED && !bulk::wait(&tok[i], 0)) || !bulk::wait(&full[st], phase)) {
         ok = false;
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int64_t rem = a.k - (int64_t)(k_lo + i) * BK;
       const int kb = (int)imin64(4, (rem + 63) / 64);
-      const uint64_t ad = operand_desc(bulk::addr(s_a + st * A_BYTES)), bd = operand_desc(bulk::addr(s_b + st * N * BK_BYTES));
-      const uint64_t sad = atom_desc(bulk::addr(s_sfa + st * SF_BYTES)), sbd = atom_desc(bulk::addr(s_sfb + st * SF_BYTES));
+      const int bs = FUSED ? i : st;
+      const uint64_t ad = operand_desc(bulk::addr(s_a + st * A_BYTES)), bd = operand_desc(bulk::addr(s_b + bs * N * BK_BYTES));
+      const uint64_t sad = atom_desc(bulk::addr(s_sfa + st * SF_BYTES)), sbd = atom_desc(bulk::addr(s_sfb + bs * SF_BYTES));
       // the scale cells are reused by every stage: one thread's tcgen05
       // operations execute in the order it issues them
       for (int j = 0; j < kb; ++j) {
@@ -240,6 +256,35 @@ __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constan
     commit(&done);
     if (!bulk::wait(&done, 0)) ok = false;
     if (!ok) gave_up = 1;
+  } else if (FUSED && warp >= 2) {
+    // ---- tokens: a warp quantizes 256 k of one token, 8 values a lane, 4 lanes a block ----
+    // Rows past m are left as they are: they are columns of the product that nobody reads.
+    for (int task = warp - 2; task < steps * (int)a.m; task += THREADS / 32 - 2) {
+      const int i = task / (int)a.m, t = task - i * (int)a.m;
+      const int64_t c = (int64_t)(k_lo + i) * BK + 8 * lane;
+      uint4 raw = make_uint4(0, 0, 0, 0);
+      if (c < a.k) raw = __ldg(reinterpret_cast<const uint4*>(a.x + t * a.ldx + c));
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+      uint32_t top = 0;
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        top = __vmaxu2(top, w[j] & 0x7FFF7FFFu);
+        f[2 * j] = bf16lo(w[j]);
+        f[2 * j + 1] = bf16hi(w[j]);
+      }
+      top = max(top & 0xFFFFu, top >> 16);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t code = mx::block_code(top << 16);
+      const uint32_t nib = mx::encode8(f, mx::code_inverse(code));
+      const int j = lane >> 2;   // the stage's block, a 16-byte piece of the swizzled row
+      *reinterpret_cast<uint32_t*>(s_b + i * N * BK_BYTES + t * BK_BYTES + ((j ^ (t & 7)) << 4) + 4 * (lane & 3)) = nib;
+      if ((lane & 3) == 0) s_sfb[i * SF_BYTES + (j >> 2) * 512 + atom_offset(t, j & 3)] = (uint8_t)code;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMA reads through the async proxy
+      __syncwarp();
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bulk::addr(&tok[i])) : "memory");
+    }
   }
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -252,13 +297,17 @@ __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constan
     }
   }
   // ---- epilogue: this part's sums as [token][row], over the ring (every MMA has read it) ----
+  __syncthreads();
   float* part = reinterpret_cast<float*>(smem);
-  const int tokens_here = (int)imin64(N, a.m - tok0);
-  for (int t = 0; t < tokens_here; t += 16) {
-    uint32_t v[16];
-    tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + t, v);
+  const int m = (int)a.m;
+  {
+    const int row = 32 * (warp & 3) + lane;   // a warp reads the TMEM lanes of its quarter
+    for (int t = 16 * (warp >> 2); t < m; t += 32) {
+      uint32_t v[16];
+      tmem_ld16(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + t, v);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) part[(t + j) * TILE_ROWS + threadIdx.x] = __uint_as_float(v[j]);
+      for (int j = 0; j < 16; ++j) part[(t + j) * TILE_ROWS + row] = __uint_as_float(v[j]);
+    }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -266,14 +315,37 @@ __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constan
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols<N>()) : "memory");
   __syncwarp();
   if (parts > 1) cluster_sync();
-  const int64_t row = (int64_t)tile * TILE_ROWS + threadIdx.x;
+  const int64_t row = (int64_t)tile * TILE_ROWS + 4 * lane;   // n % 8 == 0: all four rows or none
   if (row < a.n && !gave_up) {
-    const float bias = a.bias ? __uint_as_float((uint32_t)__ldg(a.bias + row) << 16) : 0.0f;
-    for (int t = rank; t < tokens_here; t += parts) {
-      const uint32_t at = bulk::addr(part + t * TILE_ROWS + threadIdx.x);
-      float s = 0.0f;
-      for (int r = 0; r < parts; ++r) s += parts > 1 ? ld_cluster(at, (uint32_t)r) : part[t * TILE_ROWS + threadIdx.x];
-      a.y[(int64_t)(tok0 + t) * a.n + row] = __bfloat16_as_ushort(__float2bfloat16_rn(s + bias));
+    float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (a.bias) {
+      const uint2 w = __ldg(reinterpret_cast<const uint2*>(a.bias + row));
+      bias[0] = bf16lo(w.x); bias[1] = bf16hi(w.x); bias[2] = bf16lo(w.y); bias[3] = bf16hi(w.y);
+    }
+#pragma unroll 2
+    for (int t = rank + parts * warp; t < m; t += parts * (THREADS / 32)) {
+      const float* at = part + t * TILE_ROWS + 4 * lane;
+      float4 v[MAX_PARTS];
+      if (parts == 1) {
+        v[0] = *reinterpret_cast<const float4*>(at);
+      } else {
+#pragma unroll
+        for (int r = 0; r < MAX_PARTS; ++r)
+          if (r < parts) v[r] = ld_cluster(bulk::addr(at), (uint32_t)r);
+      }
+      float4 s = v[0];   // the parts in order
+#pragma unroll
+      for (int r = 1; r < MAX_PARTS; ++r)
+        if (r < parts) {
+          s.x += v[r].x;
+          s.y += v[r].y;
+          s.z += v[r].z;
+          s.w += v[r].w;
+        }
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(s.x + bias[0], s.y + bias[1]);
+      const __nv_bfloat162 hi = __floats2bfloat162_rn(s.z + bias[2], s.w + bias[3]);
+      *reinterpret_cast<uint2*>(a.y + (int64_t)t * a.n + row) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
     }
   }
   if (parts > 1) cluster_sync();   // no CTA leaves while another reads its sums
@@ -305,25 +377,32 @@ static bool operand_map(CUtensorMap* map, const void* base, int64_t rows, int64_
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int N>
-static int launch(const void* qw, const void* qx, Args a, int sms, cudaStream_t st) {
-  CUtensorMap wm, xm;
-  if (!operand_map(&wm, qw, a.n, a.k / 2, TILE_ROWS) || !operand_map(&xm, qx, a.m, a.k / 2, N)) return NVFP4B200_ERR_CUDA;
-  const int64_t tiles = ceil_div(a.n, TILE_ROWS), blocks = ceil_div(a.m, N);
-  // K parts: double them while that leaves every CTA at least 2 stages and
-  // the grid under two CTAs per SM
+// K parts: doubled while that leaves every CTA at least 2 stages and the grid
+// at most two CTAs per SM.
+static int parts_for(int64_t tiles, int k_stages, int sms) {
   int parts = 1;
-  while (parts < MAX_PARTS && a.k_stages >= 4 * parts && tiles * blocks * parts * 2 <= 2 * sms) parts *= 2;
+  while (parts < MAX_PARTS && k_stages >= 4 * parts && tiles * parts * 2 <= 2 * sms) parts *= 2;
+  return parts;
+}
+
+template <int N, bool FUSED>
+static int launch(const void* qw, const void* qx, Args a, int parts, cudaStream_t st) {
+  CUtensorMap wm, xm;
+  if (!operand_map(&wm, qw, a.n, a.k / 2, TILE_ROWS)) return NVFP4B200_ERR_CUDA;
+  if (FUSED) xm = wm;   // not used
+  else if (!operand_map(&xm, qx, a.m, a.k / 2, N)) return NVFP4B200_ERR_CUDA;
+  const int64_t tiles = ceil_div(a.n, TILE_ROWS);
   const int most = (int)ceil_div(a.k_stages, parts);
+  const int held = FUSED ? most * (N * BK_BYTES + SF_BYTES) : 0;
   // two CTAs per SM share its memory; the [N][128] sums reuse the ring
-  const int fit = (SMEM_SM / 2 - 2048) / stage_bytes<N>();
+  const int fit = (SMEM_SM / 2 - 2048 - held) / stage_bytes<N, FUSED>();
   a.stages = std::max(1, std::min({most, fit, MAX_STAGES}));
-  const int smem = std::max(a.stages * stage_bytes<N>(), N * TILE_ROWS * 4) + 1024;
-  auto* fn = mx_linear_kernel<N>;
+  const int smem = std::max(a.stages * stage_bytes<N, FUSED>() + held, N * TILE_ROWS * 4) + 1024;
+  auto* fn = mx_linear_kernel<N, FUSED>;
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return NVFP4B200_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * parts), (unsigned)blocks, 1);
+  cfg.gridDim = dim3((unsigned)(tiles * parts), 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -335,7 +414,7 @@ static int launch(const void* qw, const void* qx, Args a, int sms, cudaStream_t 
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = FUSED ? 1 : 2;   // FUSED follows kernels that know nothing of it
   if (cudaLaunchKernelEx(&cfg, fn, wm, xm, a) != cudaSuccess) {
     cudaGetLastError();
     return NVFP4B200_ERR_LAUNCH;
@@ -356,9 +435,18 @@ int take_mxlin_device_error() {
 
 using namespace nvfp4b200;
 
-extern "C" int nvfp4b200_mx_linear(const void* x, const void* qw, const void* sfw, const void* bias, void* qx, void* sfx,
-                                   void* y, int64_t m, int64_t n, int64_t k, int64_t ldx, void* stream) {
-  if (!x || !qw || !sfw || !qx || !sfx || !y) return NVFP4B200_ERR_INVALID_ARG;
+extern "C" {
+
+int nvfp4b200_mx_linear_fused(int64_t m, int64_t n, int64_t k) {
+  if (m < 1 || m > mxlin::FUSED_TOKENS || n < 1 || k < 1) return 0;
+  // K parts that hold their tokens in shared memory: 8 parts of 16 stages at most
+  return ceil_div(k, mxlin::BK) <= mxlin::MAX_PARTS * mxlin::FUSED_STEPS;
+}
+
+int nvfp4b200_mx_linear(const void* x, const void* qw, const void* sfw, const void* bias, void* qx, void* sfx, void* y,
+                        int64_t m, int64_t n, int64_t k, int64_t ldx, void* stream) {
+  const bool fused = nvfp4b200_mx_linear_fused(m, n, k);
+  if (!x || !qw || !sfw || (!fused && (!qx || !sfx)) || !y) return NVFP4B200_ERR_INVALID_ARG;
   if (m < 0 || n < 0 || n % 8 || k <= 0 || k % 32 || ldx < k || ldx % 8 || m > (1ll << 30) || n > (1ll << 30) ||
       k > (1ll << 30))
     return NVFP4B200_ERR_BAD_SHAPE;
@@ -368,12 +456,13 @@ extern "C" int nvfp4b200_mx_linear(const void* x, const void* qw, const void* sf
   if (rc) return rc;
   if (m == 0 || n == 0) return NVFP4B200_OK;
   cudaStream_t st = (cudaStream_t)stream;
-  rc = mx_quant_rows_async(x, qx, sfx, m, k, ldx, st);
-  if (rc) return rc;
-  if (m > 128) return nvfp4b200_mx_gemm(qx, qw, sfx, sfw, bias, nullptr, y, NVFP4B200_BF16, 0, NVFP4B200_EPI_NONE, m, n, k, n, stream);
+  const int sms = sm_count_current();
+  const int64_t tiles = ceil_div(n, mxlin::TILE_ROWS);
   mxlin::Args a;
   a.sfw = static_cast<const uint8_t*>(sfw);
   a.sfx = static_cast<const uint8_t*>(sfx);
+  a.x = static_cast<const uint16_t*>(x);
+  a.ldx = ldx;
   a.bias = static_cast<const uint16_t*>(bias);
   a.y = static_cast<uint16_t*>(y);
   a.m = m;
@@ -382,9 +471,20 @@ extern "C" int nvfp4b200_mx_linear(const void* x, const void* qw, const void* sf
   a.atoms = (int)ceil_div(k, 128);
   a.k_stages = (int)ceil_div(k, mxlin::BK);
   a.stages = 0;
-  const int sms = sm_count_current();
-  if (m <= 16) return mxlin::launch<16>(qw, qx, a, sms, st);
-  if (m <= 32) return mxlin::launch<32>(qw, qx, a, sms, st);
-  if (m <= 64) return mxlin::launch<64>(qw, qx, a, sms, st);
-  return mxlin::launch<128>(qw, qx, a, sms, st);
+  int parts = mxlin::parts_for(tiles, a.k_stages, sms);
+  if (fused) {
+    while (ceil_div(a.k_stages, parts) > mxlin::FUSED_STEPS) parts *= 2;
+    return mxlin::launch<16, true>(qw, nullptr, a, parts, st);
+  }
+  rc = mx_quant_rows_async(x, qx, sfx, m, k, ldx, st);
+  if (rc) return rc;
+  if (m > 128)
+    return nvfp4b200_mx_gemm(qx, qw, sfx, sfw, bias, nullptr, y, NVFP4B200_BF16, 0, NVFP4B200_EPI_NONE, m, n, k, n,
+                             stream);
+  if (m <= 16) return mxlin::launch<16, false>(qw, qx, a, parts, st);
+  if (m <= 32) return mxlin::launch<32, false>(qw, qx, a, parts, st);
+  if (m <= 64) return mxlin::launch<64, false>(qw, qx, a, parts, st);
+  return mxlin::launch<128, false>(qw, qx, a, parts, st);
 }
+
+}  // extern "C"
