@@ -249,7 +249,7 @@ int nvfp4b200_mx_gemm(const void* a, const void* b, const void* sfa, const void*
                       int64_t k, int64_t ldd, void* stream);
 
 /* 1 where nvfp4b200_mx_linear quantizes the tokens inside its product and so
- * takes no workspace (up to 16 tokens, k <= 32768), else 0. */
+ * takes no workspace (up to 12 tokens, k <= 32768), else 0. */
 int nvfp4b200_mx_linear_fused(int64_t m, int64_t n, int64_t k);
 
 /* y = Q(x) . W^T + bias for W held in MXFP4: x bf16 [m, k] (row stride ldx) is

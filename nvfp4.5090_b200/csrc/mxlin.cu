@@ -19,13 +19,17 @@
 //   all 8 warps epilogue: TMEM -> shared memory as [token][row]; after a
 //               cluster barrier the CTA of rank r adds up the parts of tokens
 //               r, r + parts, .. and writes them with the bias.
-// Up to 16 tokens are quantized here (FUSED): warps 2-7 read a token's 256 k
+// Up to 12 tokens are quantized here (FUSED): warps 2-7 read a token's 256 k
 // of a stage, a warp each, and write nibbles and scale codes where the MMA
 // reads them, while the weights are still under way; one launch, no
 // workspace.  More tokens would make every 128-row tile's CTA spend longer on
 // them than on its weights: they are quantized once by the row quantizer just
 // before, and this kernel is its programmatic dependent, so its first weights
-// load meanwhile.
+// load meanwhile (they were complete before the quantizer, an ordinary launch,
+// began).  At 12 tokens the two forms are level: 17.5 against 17.7 us through
+// 28672 x 4096; at 16 it is 21.5 against 17.7, at 1 it is 14.7 against 16.5.
+// FUSED is launched as a dependent too, of whatever comes before it:
+// only its set-up runs early, it reads nothing before that is complete.
 //
 // Every wait is bounded; a timeout sets the library's device error word.
 #include "bulk.cuh"
@@ -49,7 +53,7 @@ constexpr int BK = 256, BK_BYTES = BK / 2;
 constexpr int A_BYTES = TILE_ROWS * BK_BYTES;     // 16 KB
 constexpr int SF_BYTES = 1024;                    // two atoms: 128 rows x 8 scales
 constexpr int THREADS = 256;
-constexpr int FUSED_TOKENS = 16;
+constexpr int FUSED_TOKENS = 12;
 constexpr int FUSED_STEPS = 16;                   // stages of tokens that stay in shared memory (48 KB)
 constexpr int MAX_STAGES = 8;
 constexpr int MAX_PARTS = 8;
@@ -199,6 +203,8 @@ __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constan
       bulk::copy(s_sfb + st * SF_BYTES, a.sfx + (int64_t)2 * (k_lo + i) * 512, sf_bytes(i), &full[st]);
     };
     const int first = min(steps, a.stages);
+    // FUSED: whatever ran before may have written the weights themselves
+    if (FUSED) asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int i = 0; i < first; ++i) weights(i, i);
     if (!FUSED) {
       asm volatile("griddepcontrol.wait;" ::: "memory");   // the tokens are quantized from here on
@@ -220,6 +226,8 @@ __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constan
         phase ^= 1u;
       }
     }
+    // every load is under way: a next call's CTAs may set themselves up
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   } else if (warp == 1 && lane == 0) {
     // ---- MMA issuer ----
     int st = 0;
@@ -259,31 +267,43 @@ __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constan
   } else if (FUSED && warp >= 2) {
     // ---- tokens: a warp quantizes 256 k of one token, 8 values a lane, 4 lanes a block ----
     // Rows past m are left as they are: they are columns of the product that nobody reads.
-    for (int task = warp - 2; task < steps * (int)a.m; task += THREADS / 32 - 2) {
-      const int i = task / (int)a.m, t = task - i * (int)a.m;
-      const int64_t c = (int64_t)(k_lo + i) * BK + 8 * lane;
-      uint4 raw = make_uint4(0, 0, 0, 0);
-      if (c < a.k) raw = __ldg(reinterpret_cast<const uint4*>(a.x + t * a.ldx + c));
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-      uint32_t top = 0;
-      float f[8];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr int WARPS = THREADS / 32 - 2, AHEAD = 4;   // reads in flight per warp
+    const int m = (int)a.m, tasks = steps * m;
+    for (int t0 = warp - 2; t0 < tasks; t0 += WARPS * AHEAD) {
+      uint4 raw[AHEAD];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        top = __vmaxu2(top, w[j] & 0x7FFF7FFFu);
-        f[2 * j] = bf16lo(w[j]);
-        f[2 * j + 1] = bf16hi(w[j]);
+      for (int u = 0; u < AHEAD; ++u) {
+        const int task = t0 + u * WARPS, i = task / m, t = task - i * m;
+        const int64_t c = (int64_t)(k_lo + i) * BK + 8 * lane;
+        raw[u] = make_uint4(0, 0, 0, 0);
+        if (task < tasks && c < a.k) raw[u] = __ldg(reinterpret_cast<const uint4*>(a.x + t * a.ldx + c));
       }
-      top = max(top & 0xFFFFu, top >> 16);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const uint32_t code = mx::block_code(top << 16);
-      const uint32_t nib = mx::encode8(f, mx::code_inverse(code));
-      const int j = lane >> 2;   // the stage's block, a 16-byte piece of the swizzled row
-      *reinterpret_cast<uint32_t*>(s_b + i * N * BK_BYTES + t * BK_BYTES + ((j ^ (t & 7)) << 4) + 4 * (lane & 3)) = nib;
-      if ((lane & 3) == 0) s_sfb[i * SF_BYTES + (j >> 2) * 512 + atom_offset(t, j & 3)] = (uint8_t)code;
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMA reads through the async proxy
-      __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bulk::addr(&tok[i])) : "memory");
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int task = t0 + u * WARPS, i = task / m, t = task - i * m;
+        if (task >= tasks) break;
+        const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+        uint32_t top = 0;
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          top = __vmaxu2(top, w[j] & 0x7FFF7FFFu);
+          f[2 * j] = bf16lo(w[j]);
+          f[2 * j + 1] = bf16hi(w[j]);
+        }
+        top = max(top & 0xFFFFu, top >> 16);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t code = mx::block_code(top << 16);
+        const uint32_t nib = mx::encode8(f, mx::code_inverse(code));
+        const int j = lane >> 2;   // the stage's block, a 16-byte piece of the swizzled row
+        *reinterpret_cast<uint32_t*>(s_b + i * N * BK_BYTES + t * BK_BYTES + ((j ^ (t & 7)) << 4) + 4 * (lane & 3)) = nib;
+        if ((lane & 3) == 0) s_sfb[i * SF_BYTES + (j >> 2) * 512 + atom_offset(t, j & 3)] = (uint8_t)code;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMA reads through the async proxy
+        __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bulk::addr(&tok[i])) : "memory");
+      }
     }
   }
   __syncthreads();
@@ -414,7 +434,7 @@ static int launch(const void* qw, const void* qx, Args a, int parts, cudaStream_
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = FUSED ? 1 : 2;   // FUSED follows kernels that know nothing of it
+  cfg.numAttrs = 2;
   if (cudaLaunchKernelEx(&cfg, fn, wm, xm, a) != cudaSuccess) {
     cudaGetLastError();
     return NVFP4B200_ERR_LAUNCH;

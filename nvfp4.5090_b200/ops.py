@@ -449,8 +449,8 @@ def mx_linear(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, bias: Optiona
     m = x2.shape[0]
     y = torch.empty((*x.shape[:-1], n), device=x.device, dtype=torch.bfloat16)
     if m and n:
-        # up to 16 tokens are quantized inside the product: no workspace
-        fused = m <= 16 and _lib.load().nvfp4b200_mx_linear_fused(m, n, k)
+        # few tokens are quantized inside the product: no workspace
+        fused = m <= 12 and _lib.load().nvfp4b200_mx_linear_fused(m, n, k)
         qx, sx = (None, None) if fused else _mx_pair(m, k, x.device, None)
         _run(x2, "nvfp4b200_mx_linear", x2.data_ptr(), qw.data_ptr(), sw.data_ptr(), _ptr(bias), _ptr(qx), _ptr(sx),
              y.data_ptr(), m, n, k, max(x2.stride(0), k))
