@@ -295,8 +295,12 @@ __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constan
         top = max(top & 0xFFFFu, top >> 16);
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const uint32_t code = mx::block_code(top << 16);
-        const uint32_t nib = mx::encode8(f, mx::code_inverse(code));
+        uint32_t code;
+        float inv;
+        mx::block_scale(__uint_as_float(top << 16), code, inv);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] *= inv;
+        const uint32_t nib = mx::encode8(f);
         const int j = lane >> 2;   // the stage's block, a 16-byte piece of the swizzled row
         *reinterpret_cast<uint32_t*>(s_b + i * N * BK_BYTES + t * BK_BYTES + ((j ^ (t & 7)) << 4) + 4 * (lane & 3)) = nib;
         if ((lane & 3) == 0) s_sfb[i * SF_BYTES + (j >> 2) * 512 + atom_offset(t, j & 3)] = (uint8_t)code;
