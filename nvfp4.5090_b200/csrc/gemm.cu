@@ -702,7 +702,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
             } else if (!p.mx) {
               for (int j = 0; j < nkb; ++j) kblock(j);
             } else {
-              for (int j = 0; j < nkb; ++j) {
+              auto kblock_mx = [&](int j) {
                 const int a = j >> 1;   // an atom's 4 scales per row cover the 128 k of MMAs 2a, 2a + 1
                 if ((j & 1) == 0) {
                   tc_cp_scales_pair(sfa_t + 4 * a, sfa_d + 32 * a);
@@ -711,6 +711,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
                 }
                 tc_mma_pair_mx(acc, adesc + 2 * j, bdesc + 2 * j, sfa_t + 4 * a, sfb_t + 8 * a, 2u * (j & 1),
                                (kt | j) != 0);
+              };
+              if (nkb == KBLOCKS) {
+#pragma unroll
+                for (int j = 0; j < KBLOCKS; ++j) kblock_mx(j);
+              } else {
+                for (int j = 0; j < nkb; ++j) kblock_mx(j);
               }
             }
             tc_commit_pair(empty_bar(stage));
