@@ -415,42 +415,42 @@ class MXFP4LinearFunction(torch.autograd.Function):
         t = x.shape[0]
         need_x, need_w = ctx.needs_input_grad[:2]
         require(not (need_x or need_w) or n % 32 == 0, "training needs out_features divisible by 32")
-        qxt = sxt = qwt = swt = None
-        if need_w:
-            qx, sx, qxt, sxt = ops.mx_quantize_both(x)
+        qx, qxt = ops.mx_operands(x, True, need_w)
+        qw, qwt = ops.mx_operands(weight, True, need_x)
+        if bias is not None:
+            require(bias.numel() == n and bias.is_cuda, "bias is a CUDA tensor [N]")
+            ctx.bdtype, bias = bias.dtype, bias.to(torch.bfloat16).contiguous()
         else:
-            qx, sx = ops.mx_quantize(x)
-        if need_x:
-            qw, sw, qwt, swt = ops.mx_quantize_both(weight)
-        else:
-            qw, sw = ops.mx_quantize(weight)
-        y = ops.mx_gemm(qx, sx, qw, sw, bias=None if bias is None else bias.to(torch.bfloat16), out_dtype=input.dtype)
-        ctx.save_for_backward(qxt, sxt, qwt, swt)
-        ctx.shape, ctx.tokens, ctx.wdtype = input.shape, t, weight.dtype
-        ctx.bdtype = None if bias is None else bias.dtype
+            ctx.bdtype = None
+        require(n % 8 == 0, "out_features must be divisible by 8")
+        y = ops.mx_product(qx, qw, input.dtype, bias)
+        ctx.save_for_backward(qxt.buf if need_w else None, qwt.buf if need_x else None)
+        ctx.shape, ctx.tokens, ctx.n, ctx.wdtype = input.shape, t, n, weight.dtype
+        if input.dim() == 2:
+            return y
         # not a view, so that users may change the result in place
         return torch.ops.aten._unsafe_view(y, [*input.shape[:-1], n])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output: torch.Tensor):
-        qxt, sxt, qwt, swt = ctx.saved_tensors
+        xt, wt = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
-        dy = grad_output.reshape(-1, grad_output.shape[-1])
-        n, k = dy.shape[1], ctx.shape[-1]
-        dx = dw = db = qd = qdt = None
-        if need_x and need_w:
-            qd, sd, qdt, sdt = ops.mx_quantize_both(dy)
-        elif need_x:
-            qd, sd = ops.mx_quantize(dy)
-        elif need_w:
-            qdt, sdt = ops.mx_quantize_t(dy)
+        n, k, t = ctx.n, ctx.shape[-1], ctx.tokens
+        dy = grad_output if grad_output.dim() == 2 else grad_output.reshape(-1, n)
+        dx = dw = db = None
+        if need_x or need_w:
+            qd, qdt = ops.mx_operands(dy, need_x, need_w)
         if need_x:
-            dx = ops.mx_gemm(qd, sd, qwt, swt, out_dtype=grad_output.dtype).reshape(ctx.shape)
+            dx = ops.mx_product(qd, ops.MXOperand(k, n, dy, wt), grad_output.dtype)
+            if len(ctx.shape) != 2:
+                dx = dx.view(ctx.shape)
         if need_w:
-            out_dtype = torch.float32 if ctx.wdtype == torch.float32 else torch.bfloat16
-            if ctx.tokens:
-                dw = ops.mx_gemm(qdt, sdt, qxt, sxt, out_dtype=out_dtype).to(ctx.wdtype)
+            if t:
+                out_dtype = torch.float32 if ctx.wdtype == torch.float32 else torch.bfloat16
+                dw = ops.mx_product(qdt, ops.MXOperand(k, (t + 31) // 32 * 32, dy, xt), out_dtype)
+                if dw.dtype != ctx.wdtype:
+                    dw = dw.to(ctx.wdtype)
             else:
                 dw = torch.zeros((n, k), device=dy.device, dtype=ctx.wdtype)
         if ctx.bdtype is not None and ctx.needs_input_grad[2]:

@@ -429,6 +429,52 @@ def mx_gemm(qa: torch.Tensor, sa: torch.Tensor, qb: torch.Tensor, sb: torch.Tens
     return out
 
 
+class MXOperand:
+    """One orientation of an MXFP4 matrix in one allocation: nibbles [rows, k/2],
+    then swizzled scales.  For callers that hold operands between a forward and
+    a backward; the fewer allocations halve the wrappers' host time there."""
+    __slots__ = ("buf", "rows", "k")
+
+    def __init__(self, rows: int, k: int, like: torch.Tensor, buf: Optional[torch.Tensor] = None):
+        self.rows, self.k = rows, k
+        # k % 32 == 0: the nibbles end on a 16-byte boundary
+        self.buf = like.new_empty(rows * k // 2 + math.prod(mx_scale_shape(rows, k)),
+                                  dtype=torch.uint8) if buf is None else buf
+
+    def pointers(self) -> Tuple[int, int]:
+        p = self.buf.data_ptr()
+        return p, p + self.rows * self.k // 2
+
+
+def mx_operands(x: torch.Tensor, rows: bool, cols: bool) -> Tuple[Optional[MXOperand], Optional[MXOperand]]:
+    """x [R, K] quantized along K (``rows``) and / or, transposed, along R
+    (``cols``), from one read, as ``MXOperand``s."""
+    x = _float_matrix(x)
+    r, c = x.shape
+    if c == 0 or c % 32:
+        raise RuntimeError("K must be divisible by 32 for MXFP4 1x32 scaling.")
+    a = MXOperand(r, c, x) if rows else None
+    b = MXOperand(c, (r + 31) // 32 * 32, x) if cols else None
+    if r:
+        q, s = a.pointers() if rows else (None, None)
+        qt, st = b.pointers() if cols else (None, None)
+        _run(x, "nvfp4b200_mx_quant", x.data_ptr(), _DTYPES[x.dtype], None, None, q, s, qt, st, r, c,
+             max(x.stride(0), c))
+    return a, b
+
+
+def mx_product(a: MXOperand, b: MXOperand, out_dtype: torch.dtype, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """a . b^T + bias of two operands along the same k (bias bf16 [b.rows], checked by the caller)."""
+    if a.k != b.k or a.k == 0 or a.buf.get_device() != b.buf.get_device():
+        raise RuntimeError("the operands must share their contraction length and device")
+    out = a.buf.new_empty((a.rows, b.rows), dtype=out_dtype)
+    if a.rows and b.rows:
+        (qa, sa), (qb, sb) = a.pointers(), b.pointers()
+        _run(out, "nvfp4b200_mx_gemm", qa, qb, sa, sb, _ptr(bias), None, out.data_ptr(), _DTYPES[out_dtype], 0,
+             EPI_NONE, a.rows, b.rows, a.k, b.rows)
+    return out
+
+
 def mx_linear(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = x . W^T + bias with W held in MXFP4 (qw [n, k/2], sw; ``mx_quantize``):
     x bf16 [..., k] is quantized along k, y is bf16 [..., n].  n % 8 == 0."""
@@ -484,31 +530,33 @@ def _grad_call(grads, outs, norm_type, grad_scale, max_norm, want):
     if not max_norm >= 0.0:
         raise RuntimeError("max_norm must not be negative")
     dev = grads[0].get_device() if grads else _current_device()
-    ptrs, dts, lens = array.array("Q"), array.array("i"), array.array("q")
-    for t in grads:
-        dt = _DTYPES.get(t.dtype)
-        if dt is None or dev < 0 or t.get_device() != dev:
-            raise RuntimeError("gradients are bf16, fp16 or fp32 CUDA tensors of one device")
-        if not (t.is_contiguous() or _dense(t)):
-            raise RuntimeError("gradients must be dense: every element once in one stretch of memory")
-        ptrs.append(t.data_ptr())
-        dts.append(dt)
-        lens.append(t.numel())
     count = len(grads)
+    try:   # whole-list passes: a third of the host time of one loop over the tensors
+        dts = array.array("i", [_DTYPES[t.dtype] for t in grads])
+    except KeyError:
+        dts = None
+    if dts is None or dev < 0 or any([t.get_device() != dev for t in grads]):
+        raise RuntimeError("gradients are bf16, fp16 or fp32 CUDA tensors of one device")
+    if not all([t.is_contiguous() for t in grads]) and not all([_dense(t) for t in grads]):
+        raise RuntimeError("gradients must be dense: every element once in one stretch of memory")
+    ptrs = array.array("Q", [t.data_ptr() for t in grads])
+    lens = array.array("q", [t.numel() for t in grads])
     outp = outd = None
     if outs is grads:
         outp, outd = ptrs, dts
     elif outs is not None:
         outs = [outs] if isinstance(outs, torch.Tensor) else list(outs)
-        _require(len(outs) == count, "out must hold one tensor per gradient")
-        outp, outd = array.array("Q"), array.array("i")
-        for t, o in zip(grads, outs):
-            dt = _DTYPES.get(o.dtype)
-            if (dt is None or o.get_device() != dev or o.shape != t.shape
-                    or not ((o.is_contiguous() and t.is_contiguous()) or o.stride() == t.stride())):
-                raise RuntimeError("out tensors match their gradient's shape and layout (bf16, fp16 or fp32)")
-            outp.append(o.data_ptr())
-            outd.append(dt)
+        try:
+            outd = array.array("i", [_DTYPES[t.dtype] for t in outs])
+        except KeyError:
+            outd = None
+        if (outd is None or len(outs) != count or any([o.get_device() != dev for o in outs])
+                or [o.shape for o in outs] != [t.shape for t in grads]
+                or [o.stride() for o in outs] != [t.stride() for t in grads]
+                and not all([o.is_contiguous() and t.is_contiguous() or o.stride() == t.stride()
+                             for o, t in zip(outs, grads)])):
+            raise RuntimeError("out holds one bf16, fp16 or fp32 tensor of its shape and layout per gradient")
+        outp = array.array("Q", [o.data_ptr() for o in outs])
     device = torch.device("cuda", dev)
     words = 1024 * (1 + count // 112)
     ws = torch.empty(words, device=device, dtype=torch.float64)
