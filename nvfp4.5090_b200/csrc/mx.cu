@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(QTHREADS, DT == NVFP4B200_F32 && (COLS || SCAL
   Raw* tile = reinterpret_cast<Raw*>(smem);                 // COLS: the tile, then the staged columns
   uint8_t* stage = smem + (COLS ? tile_bytes<DT>() : 0);
   __shared__ __align__(16) uint8_t s_row[512], s_col[512];
-  __shared__ float s_scale[TILE];
+  __shared__ __align__(16) float2 s_scale[TILE];   // each row's scale twice, as a packed pair
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int tr = (int)(blockIdx.x / (unsigned)a.col_tiles), tc = (int)(blockIdx.x - tr * (unsigned)a.col_tiles);
   const int64_t r0 = (int64_t)tr * TILE, c0 = (int64_t)tc * TILE;
@@ -164,7 +164,10 @@ __global__ void __launch_bounds__(QTHREADS, DT == NVFP4B200_F32 && (COLS || SCAL
         gam[4 * h + 2] = bf16x2_to_f2(g.z); gam[4 * h + 3] = bf16x2_to_f2(g.w);
       }
     }
-    if (tid < TILE) s_scale[tid] = tid < rows_here && a.row_scale ? __ldg(a.row_scale + r0 + tid) : 1.0f;
+    if (tid < TILE) {
+      const float v = tid < rows_here && a.row_scale ? __ldg(a.row_scale + r0 + tid) : 1.0f;
+      s_scale[tid] = make_float2(v, v);
+    }
     __syncthreads();
   }
   uint8_t* q = ROWS ? a.q + (r0 + row0) * (a.cols >> 1) + ((c0 + lc) >> 1) : nullptr;
@@ -191,7 +194,7 @@ __global__ void __launch_bounds__(QTHREADS, DT == NVFP4B200_F32 && (COLS || SCAL
         }
       }
       if (SCALED) {
-        const uint64_t rs = f2pack(s_scale[rl], s_scale[rl]);
+        const uint64_t rs = *reinterpret_cast<const uint64_t*>(s_scale + rl);
 #pragma unroll
         for (int j = 0; j < 4 * VL; ++j) f[j] = f2mul(f2mul(f[j], rs), gam[j]);
       }
@@ -231,9 +234,9 @@ __global__ void __launch_bounds__(QTHREADS, DT == NVFP4B200_F32 && (COLS || SCAL
       for (int r = 0; r < 16; r += 2) {
         uint64_t p = P::f2(w[r]), n = P::f2(w[r + 1]);
         if (SCALED) {
-          const float sa = s_scale[32 * rb + 16 * half + r], sb = s_scale[32 * rb + 16 * half + r + 1];
-          f[SCALED ? r : 0] = p = f2mul(f2mul(p, f2pack(sa, sa)), g2);
-          f[SCALED ? r + 1 : 0] = n = f2mul(f2mul(n, f2pack(sb, sb)), g2);
+          const ulonglong2 rs = *reinterpret_cast<const ulonglong2*>(s_scale + 32 * rb + 16 * half + r);
+          f[SCALED ? r : 0] = p = f2mul(f2mul(p, rs.x), g2);
+          f[SCALED ? r + 1 : 0] = n = f2mul(f2mul(n, rs.y), g2);
         }
         m0 = absmax3(m0, f2lo(p), f2lo(n));
         m1 = absmax3(m1, f2hi(p), f2hi(n));

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import array
 import math
+import operator
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -520,6 +521,9 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+_dtype_of = operator.attrgetter("dtype")
+
+
 def _grad_call(grads, outs, norm_type, grad_scale, max_norm, want):
     """Run nvfp4b200_grad_norm; ``want`` names the outputs: n(orm), c(oef), t(otal)."""
     if isinstance(grads, torch.Tensor):
@@ -531,32 +535,35 @@ def _grad_call(grads, outs, norm_type, grad_scale, max_norm, want):
         raise RuntimeError("max_norm must not be negative")
     dev = grads[0].get_device() if grads else _current_device()
     count = len(grads)
-    try:   # whole-list passes: a third of the host time of one loop over the tensors
-        dts = array.array("i", [_DTYPES[t.dtype] for t in grads])
+    # whole-list passes through map: about a third of the host time of a loop
+    T = torch.Tensor
+    try:
+        dts = array.array("i", map(_DTYPES.__getitem__, map(_dtype_of, grads)))
     except KeyError:
         dts = None
-    if dts is None or dev < 0 or any([t.get_device() != dev for t in grads]):
+    if dts is None or dev < 0 or set(map(T.get_device, grads)) - {dev}:
         raise RuntimeError("gradients are bf16, fp16 or fp32 CUDA tensors of one device")
-    if not all([t.is_contiguous() for t in grads]) and not all([_dense(t) for t in grads]):
+    contiguous = all(map(T.is_contiguous, grads))
+    if not contiguous and not all(map(_dense, grads)):
         raise RuntimeError("gradients must be dense: every element once in one stretch of memory")
-    ptrs = array.array("Q", [t.data_ptr() for t in grads])
-    lens = array.array("q", [t.numel() for t in grads])
+    ptrs, lens = array.array("Q", map(T.data_ptr, grads)), array.array("q", map(T.numel, grads))
     outp = outd = None
     if outs is grads:
         outp, outd = ptrs, dts
     elif outs is not None:
         outs = [outs] if isinstance(outs, torch.Tensor) else list(outs)
         try:
-            outd = array.array("i", [_DTYPES[t.dtype] for t in outs])
+            outd = array.array("i", map(_DTYPES.__getitem__, map(_dtype_of, outs)))
         except KeyError:
             outd = None
-        if (outd is None or len(outs) != count or any([o.get_device() != dev for o in outs])
-                or [o.shape for o in outs] != [t.shape for t in grads]
-                or [o.stride() for o in outs] != [t.stride() for t in grads]
-                and not all([o.is_contiguous() and t.is_contiguous() or o.stride() == t.stride()
-                             for o, t in zip(outs, grads)])):
-            raise RuntimeError("out holds one bf16, fp16 or fp32 tensor of its shape and layout per gradient")
-        outp = array.array("Q", [o.data_ptr() for o in outs])
+        if (outd is None or len(outs) != count or set(map(T.get_device, outs)) - {dev}
+                or array.array("q", map(T.numel, outs)) != lens
+                or not (contiguous and all(map(T.is_contiguous, outs)))
+                and any(o.shape != t.shape or o.stride() != t.stride() for o, t in zip(outs, grads)
+                        if not (o.is_contiguous() and t.is_contiguous()))):
+            raise RuntimeError("out holds one bf16, fp16 or fp32 tensor per gradient, contiguous and of its number "
+                               "of elements, or of its shape and strides")
+        outp = array.array("Q", map(T.data_ptr, outs))
     device = torch.device("cuda", dev)
     words = 1024 * (1 + count // 112)
     ws = torch.empty(words, device=device, dtype=torch.float64)
@@ -610,7 +617,8 @@ def clip_grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm:
     clipping (1-element fp32; of grad * grad_scale).
 
     out_i = grad_i * grad_scale * min(1, max_norm / (norm + 1e-6)), written in
-    place or into ``out`` (same shapes, any of the three types: e.g. fp32
+    place or into ``out`` (contiguous tensors of as many elements, or of the
+    gradient's shape and strides, in any of the three types: e.g. fp32
     accumulators into bf16 communication buckets).  In place and with nothing
     to scale, nothing is written.  Outputs must not overlap one another or
     another gradient.  A NaN gradient makes every output NaN, an infinite norm
