@@ -372,6 +372,7 @@ struct BwdArgs {
   int64_t rows, ldb, ld_dy, ld_dn, ldy, rows_per_gate, rows_per_cta;
   int d;
   float alpha, s;
+  int ws16;                 // part and part_gate are 16-byte aligned
 };
 
 // A CTA walks rows_per_cta consecutive rows, one at a time.  rows_per_cta
@@ -509,19 +510,28 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
 // Arithmetic is on packed pairs of floats.  A CTA's rows lie in one group (W
 // stays in registers), so dgamma_post's part is gate * S at the end.  The
 // column sums S leave out s; it is multiplied in at the end.
-// What bounds it is the instruction stream of 16 warps per SM at 128 registers.
+// The column sums live in shared memory, each thread's own words, so that a
+// thread fits 64 registers and 32 warps share an SM: with the sums in registers
+// 16 warps did, and waited for one another's barriers (147 us against NNN).
 __device__ int g_norm_error = 0;
 
+// Rows of the ring: two with the next norm's tensors, three without.
+template <bool PRE>
+constexpr int bwd_stages() { return PRE ? 2 : 3; }
+
+// One 8-element vector per thread: TPR threads cover d <= 8 * TPR columns.
 template <int DT, int TPR, bool PRE>
-__global__ void __launch_bounds__(TPR, 512 / TPR) sandwich_bwd_staged_kernel(const BwdArgs a, int64_t parts_per_group) {
+__global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1024 / TPR)
+    sandwich_bwd_staged_kernel(const BwdArgs a, int64_t parts_per_group) {
   using E = Elem<DT>;
   using Raw = typename E::Raw;
   constexpr int NT = PRE ? 4 : 2;                 // tensors: dy, b [, dn, y]
-  constexpr int NP = CPT / 2;                     // packed pairs per thread
+  constexpr int NP = 4;                           // packed pairs per thread
+  constexpr int ST = bwd_stages<PRE>();
   constexpr int W4 = (TPR / 32 + 3) / 4;          // 16-byte words of one sum's warp parts
-  extern __shared__ __align__(16) uint8_t row_ring[];   // [STAGES][NT][d]
+  extern __shared__ __align__(16) uint8_t row_ring[];   // [ST][NT][d], then the column sums
   __shared__ __align__(16) float red[2][3][4 * W4];
-  __shared__ __align__(8) uint64_t full[STAGES];
+  __shared__ __align__(8) uint64_t full[ST];
   __shared__ int gave_up;
   const int t = threadIdx.x;
   const float inv_d = 1.0f / (float)a.d;
@@ -545,43 +555,33 @@ __global__ void __launch_bounds__(TPR, 512 / TPR) sandwich_bwd_staged_kernel(con
   if (t < 3 * 4 * W4 * 2) (&red[0][0][0])[t] = 0.0f;   // warp parts past the last stay zero
   if (t == 0) {
     gave_up = 0;
-    bulk::init(full, STAGES);
+    bulk::init(full, ST);
   }
   __syncthreads();
   if (t == 0)
-    for (int st = 0; st < STAGES; ++st) fetch(st, st);
+    for (int st = 0; st < ST; ++st) fetch(st, st);
 
-  uint64_t W[NP], gpre[PRE ? NP : 1], S[NP], pre[PRE ? NP : 1];
-  {
-    float w[CPT], v[CPT];
-    Row<DT, true, TPR> row;
+  // column sums, each thread's own: S (2 float4) and dgamma_pre's (2 more)
+  ulonglong2* sums_at = reinterpret_cast<ulonglong2*>(row_ring + (size_t)ST * NT * row_bytes) + t;
 #pragma unroll
-    for (int j = 0; j < CPT; ++j) w[j] = a.s;
-    for (const void* q : {a.gamma_post, a.gate ? (const void*)(static_cast<const Raw*>(a.gate) + g * a.d) : nullptr})
-      if (q) {
-        row.load(static_cast<const Raw*>(q), t, a.d);
-        row.values(v);
+  for (int j = 0; j < (PRE ? 4 : 2); ++j) sums_at[j * TPR] = make_ulonglong2(0ull, 0ull);
+  const int c = 8 * t;
+  const bool in = c < a.d;
+  auto weights = [&](const void* p, int64_t off, uint64_t (&w)[NP]) {
+    float f[8];
+    E::unpack(in ? E::load(static_cast<const Raw*>(p) + off + c) : E::zero(), f);
 #pragma unroll
-        for (int j = 0; j < CPT; ++j) w[j] *= v[j];
-      }
+    for (int j = 0; j < NP; ++j) w[j] = f2mul(w[j], f2pack(f[2 * j], f[2 * j + 1]));
+  };
+  uint64_t W[NP], gpre[PRE ? NP : 1];
 #pragma unroll
-    for (int j = 0; j < NP; ++j) {
-      W[j] = f2pack(w[2 * j], w[2 * j + 1]);
-      S[j] = 0ull;
-    }
-    if (PRE) {
+  for (int j = 0; j < NP; ++j) W[j] = f2two(a.s);
+  if (a.gamma_post) weights(a.gamma_post, 0, W);
+  if (a.gate) weights(a.gate, g * a.d, W);
+  if constexpr (PRE) {
 #pragma unroll
-      for (int j = 0; j < CPT; ++j) v[j] = 1.0f;
-      if (a.gamma_pre) {
-        row.load(static_cast<const Raw*>(a.gamma_pre), t, a.d);
-        row.values(v);
-      }
-#pragma unroll
-      for (int j = 0; j < NP; ++j) {
-        gpre[j] = f2pack(v[2 * j], v[2 * j + 1]);
-        pre[j] = 0ull;
-      }
-    }
+    for (int j = 0; j < NP; ++j) gpre[j] = f2two(1.0f);
+    if (a.gamma_pre) weights(a.gamma_pre, 0, gpre);
   }
 
   Raw *dx = static_cast<Raw*>(a.dx) + r0 * a.d, *db = static_cast<Raw*>(a.db) + r0 * a.d;
@@ -602,43 +602,40 @@ __global__ void __launch_bounds__(TPR, 512 / TPR) sandwich_bwd_staged_kernel(con
     };
     uint64_t t0[NP], yh[PRE ? NP : 1], bh[NP];
     uint64_t A = 0ull, B = 0ull, C = 0ull;
+    {
+      uint64_t z[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-    for (int h = 0; h < VPT; ++h) {
-      const int c = column<true, TPR>(t, 8 * h);
-      uint64_t x[4] = {0ull, 0ull, 0ull, 0ull}, z[4] = {0ull, 0ull, 0ull, 0ull};
-      if (c < a.d) {
-        if (a.dy) get(0, c, x);
+      for (int j = 0; j < NP; ++j) t0[j] = 0ull;
+      if (in) {
+        if (a.dy) get(0, c, t0);
         get(1, c, z);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        t0[4 * h + j] = x[j];
-        bh[4 * h + j] = f2mul(z[j], f2two(inv_b));
-      }
-      if (PRE) {
-        if (c < a.d) {
+      for (int j = 0; j < NP; ++j) bh[j] = f2mul(z[j], f2two(inv_b));
+      if constexpr (PRE) {
+        uint64_t x[4] = {0ull, 0ull, 0ull, 0ull};
+        if (in) {
           get(2, c, x);
           get(3, c, z);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = z[j] = 0ull;
         }
+        const ulonglong2 p0 = sums_at[2 * TPR], p1 = sums_at[3 * TPR];
+        uint64_t pre[NP] = {p0.x, p0.y, p1.x, p1.y};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int k = 4 * h + j;
-          yh[k] = f2mul(z[j], f2two(inv_y));
-          pre[k] = f2fma(x[j], yh[k], pre[k]);
-          const uint64_t v = f2mul(x[j], gpre[k]);
-          A = f2fma(v, yh[k], A);
-          t0[k] = f2fma(v, f2two(inv_y), t0[k]);
+        for (int j = 0; j < NP; ++j) {
+          yh[j] = f2mul(z[j], f2two(inv_y));
+          pre[j] = f2fma(x[j], yh[j], pre[j]);
+          const uint64_t v = f2mul(x[j], gpre[j]);
+          A = f2fma(v, yh[j], A);
+          t0[j] = f2fma(v, f2two(inv_y), t0[j]);
         }
+        sums_at[2 * TPR] = make_ulonglong2(pre[0], pre[1]);
+        sums_at[3 * TPR] = make_ulonglong2(pre[2], pre[3]);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = 4 * h + j;
-        const uint64_t wb = f2mul(W[k], bh[k]);
-        B = f2fma(wb, t0[k], B);
-        if (PRE) C = f2fma(wb, yh[k], C);
+      for (int j = 0; j < NP; ++j) {
+        const uint64_t wb = f2mul(W[j], bh[j]);
+        B = f2fma(wb, t0[j], B);
+        if (PRE) C = f2fma(wb, yh[j], C);
       }
     }
     float sums[3] = {f2sum(B), PRE ? f2sum(A) : 0.0f, PRE ? f2sum(C) : 0.0f};
@@ -651,7 +648,7 @@ __global__ void __launch_bounds__(TPR, 512 / TPR) sandwich_bwd_staged_kernel(con
       for (int k = 0; k < (PRE ? 3 : 1); ++k) red[buf][k][t >> 5] = sums[k];
     }
     __syncthreads();
-    if (t == 0) fetch(i + STAGES, stage);
+    if (t == 0) fetch(i + ST, stage);
     if (TPR > 32) {
 #pragma unroll
       for (int k = 0; k < (PRE ? 3 : 1); ++k) {
@@ -668,28 +665,27 @@ __global__ void __launch_bounds__(TPR, 512 / TPR) sandwich_bwd_staged_kernel(con
     if (gave_up) break;   // set before the barrier: every thread sees it
     const float m1 = PRE ? sums[1] * inv_d : 0.0f;
     const float m2 = (PRE ? fmaf(-inv_y * m1, sums[2], sums[0]) : sums[0]) * inv_d;
+    const ulonglong2 s0 = sums_at[0], s1 = sums_at[TPR];
+    uint64_t S[NP] = {s0.x, s0.y, s1.x, s1.y};
+    float dxv[8], dbv[8];
 #pragma unroll
-    for (int h = 0; h < VPT; ++h) {
-      float dxv[8], dbv[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = 4 * h + j;
-        const uint64_t tt = PRE ? f2fma(yh[k], f2two(-inv_y * m1), t0[k]) : t0[k];
-        S[k] = f2fma(tt, bh[k], S[k]);
-        const uint64_t d = f2mul(f2fma(bh[k], f2two(-m2), f2mul(W[k], tt)), f2two(inv_b));
-        const uint64_t e = f2mul(tt, f2two(a.alpha));
-        dxv[2 * j] = f2lo(e); dxv[2 * j + 1] = f2hi(e);
-        dbv[2 * j] = f2lo(d); dbv[2 * j + 1] = f2hi(d);
-      }
-      const int c = column<true, TPR>(t, 8 * h);
-      if (c < a.d) {
-        E::store(dx + c, E::pack(dxv));
-        E::store(db + c, E::pack(dbv));
-      }
+    for (int j = 0; j < NP; ++j) {
+      const uint64_t tt = PRE ? f2fma(yh[j], f2two(-inv_y * m1), t0[j]) : t0[j];
+      S[j] = f2fma(tt, bh[j], S[j]);
+      const uint64_t d = f2mul(f2fma(bh[j], f2two(-m2), f2mul(W[j], tt)), f2two(inv_b));
+      const uint64_t e = f2mul(tt, f2two(a.alpha));
+      dxv[2 * j] = f2lo(e); dxv[2 * j + 1] = f2hi(e);
+      dbv[2 * j] = f2lo(d); dbv[2 * j + 1] = f2hi(d);
+    }
+    sums_at[0] = make_ulonglong2(S[0], S[1]);
+    sums_at[TPR] = make_ulonglong2(S[2], S[3]);
+    if (in) {
+      E::store(dx + c, E::pack(dxv));
+      E::store(db + c, E::pack(dbv));
     }
     dx += a.d;
     db += a.d;
-    if (++stage == STAGES) {
+    if (++stage == ST) {
       stage = 0;
       parity ^= 1u;
     }
@@ -697,26 +693,32 @@ __global__ void __launch_bounds__(TPR, 512 / TPR) sandwich_bwd_staged_kernel(con
   if (gave_up && t == 0) {
     // a copy did not arrive in time: report it, and leave no copy in flight behind
     atomicExch(&g_norm_error, NVFP4B200_ERR_TIMEOUT);
-    for (int st = 0; st < STAGES; ++st) bulk::wait(&full[st], parity ^ (st < stage ? 1u : 0u));
+    for (int st = 0; st < ST; ++st) bulk::wait(&full[st], parity ^ (st < stage ? 1u : 0u));
   }
 
   // partial column sums: s * S, gate * s * S and dgamma_pre
-  float w[CPT];
+  if (!in) return;
+  uint64_t gate[NP];
 #pragma unroll
-  for (int j = 0; j < CPT; ++j) w[j] = 1.0f;
-  if (a.gate) {
-    Row<DT, true, TPR> row;
-    row.load(static_cast<const Raw*>(a.gate) + g * a.d, t, a.d);
-    row.values(w);
-  }
+  for (int j = 0; j < NP; ++j) gate[j] = f2two(1.0f);
+  if (a.gate) weights(a.gate, g * a.d, gate);
+  auto put = [&](float* out, uint64_t lo, uint64_t hi) {   // d % 8 == 0: 16-byte aligned where the workspace is
+    if (a.ws16) {
+      *reinterpret_cast<ulonglong2*>(out) = make_ulonglong2(lo, hi);
+    } else {
+      out[0] = f2lo(lo); out[1] = f2hi(lo); out[2] = f2lo(hi); out[3] = f2hi(hi);
+    }
+  };
 #pragma unroll
-  for (int j = 0; j < CPT; ++j) {
-    const int c = column<true, TPR>(t, j);
-    if (c >= a.d) continue;
-    const float sv = a.s * ((j & 1) ? f2hi(S[j >> 1]) : f2lo(S[j >> 1]));
-    if (a.gate) a.part_gate[(int64_t)blockIdx.x * a.d + c] = sv;
-    a.part[(int64_t)blockIdx.x * a.d + c] = sv * w[j];
-    if (PRE) a.part[((int64_t)gridDim.x + blockIdx.x) * a.d + c] = (j & 1) ? f2hi(pre[j >> 1]) : f2lo(pre[j >> 1]);
+  for (int h = 0; h < 2; ++h) {
+    const ulonglong2 sv = sums_at[h * TPR];
+    const uint64_t lo = f2mul(sv.x, f2two(a.s)), hi = f2mul(sv.y, f2two(a.s));
+    if (a.gate) put(a.part_gate + (int64_t)blockIdx.x * a.d + c + 4 * h, lo, hi);
+    put(a.part + (int64_t)blockIdx.x * a.d + c + 4 * h, f2mul(lo, gate[2 * h]), f2mul(hi, gate[2 * h + 1]));
+    if (PRE) {
+      const ulonglong2 pv = sums_at[(2 + h) * TPR];
+      put(a.part + ((int64_t)gridDim.x + blockIdx.x) * a.d + c + 4 * h, pv.x, pv.y);
+    }
   }
 }
 
@@ -928,7 +930,8 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
   nvfp4b200_sandwich_norm_bwd_ws(rows, d, groups, &need);
   if (ws_floats < need) return NVFP4B200_ERR_BAD_SHAPE;
   norm::BwdArgs a{dy, dn, b, y, gamma_post, gate, gamma_pre, inv_b, inv_y, dx, db, ws, ws + 2 * sp.ctas * d, dgate, rows, ldb,
-                  ld_dy, ld_dn, ldy, rows / g, sp.rows_per_cta, (int)d, residual_scale, branch_scale};
+                  ld_dy, ld_dn, ldy, rows / g, sp.rows_per_cta, (int)d, residual_scale, branch_scale,
+                  aligned(ws, 16)};
   const bool vec = (d * bytes) % 16 == 0 && d % 8 == 0 && vec_ok(dy, ld_dy, bytes) && vec_ok(dn, ld_dn, bytes) &&
                    vec_ok(b, ldb, bytes) && vec_ok(y, ldy, bytes) && vec_ok(gamma_post, d, bytes) &&
                    vec_ok(gate, d, bytes) && vec_ok(gamma_pre, d, bytes) && vec_ok(dx, d, bytes) && vec_ok(db, d, bytes);
@@ -940,13 +943,15 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
       // the staged kernel where its ring fits and a CTA's rows have one gate:
       // 346 -> 162 us at 16000 x 4096 bf16 with 8 gates and the next norm
       if constexpr (decltype(v)::value && T <= 512) {
-        const int smem = norm::STAGES * (dn ? 4 : 2) * (int)d * norm::dtype_size<DT>();
+        constexpr int T2 = 2 * T;
+        const int stages = dn ? norm::bwd_stages<true>() : norm::bwd_stages<false>();
+        const int smem = stages * (dn ? 4 : 2) * (int)d * norm::dtype_size<DT>() + (dn ? 4 : 2) * 16 * T2;
         if (smem <= norm::MAX_SMEM && (!gate || sp.parts_per_group > 1)) {
-          auto* fn = dn ? norm::sandwich_bwd_staged_kernel<DT, T, true> : norm::sandwich_bwd_staged_kernel<DT, T, false>;
+          auto* fn = dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true> : norm::sandwich_bwd_staged_kernel<DT, T2, false>;
           if (smem > 32 * 1024 &&   // with the static arrays, past the default limit
               cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
             return (int)NVFP4B200_ERR_CUDA;
-          fn<<<(unsigned)sp.ctas, T, smem, st>>>(a, sp.parts_per_group);
+          fn<<<(unsigned)sp.ctas, T2, smem, st>>>(a, sp.parts_per_group);
           return launch_status();
         }
       }
