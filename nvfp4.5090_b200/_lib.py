@@ -18,7 +18,7 @@ c_int = ctypes.c_int
 c_i64 = ctypes.c_int64
 c_float = ctypes.c_float
 
-# name -> argument types (all return int status)
+# name -> argument types (all return int: a status, but for nvfp4b200_api_version and nvfp4b200_mx_linear_fused)
 SIGNATURES = {
     "nvfp4b200_api_version": [],
     "nvfp4b200_device_check": [],

@@ -60,7 +60,8 @@ def _scalar_f32(g: Optional[torch.Tensor], device) -> Optional[torch.Tensor]:
 
 # The current device and its current stream's handle, without building the
 # device and stream objects of torch.cuda (0.2 us a call in place of 3.4 us).
-_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
 def _run(t: torch.Tensor, name: str, *args) -> None:
@@ -367,7 +368,7 @@ def mx_quantize_both(x: torch.Tensor, row_scale: Optional[torch.Tensor] = None, 
 
 def mx_dequantize(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values [R, K] (bf16 or fp32) that an MXFP4 matrix stands for."""
-    _require(q.is_cuda and q.dtype == torch.uint8 and q.dim() == 2, "mx_dequantize expects packed uint8 [R, K/2]")
+    _require(q.is_cuda and q.element_size() == 1 and q.dim() == 2, "mx_dequantize expects packed bytes [R, K/2]")
     r, k = q.shape[0], 2 * q.shape[1]
     _require(k % 32 == 0, "K must be divisible by 32 for MXFP4 1x32 scaling.")
     _require(dtype in (torch.bfloat16, torch.float32), "output dtype must be bf16 or fp32")
@@ -391,6 +392,8 @@ def mx_gemm(qa: torch.Tensor, sa: torch.Tensor, qb: torch.Tensor, sb: torch.Tens
     dev = qa.get_device()
     if not qa.is_cuda or sa.get_device() != dev or qb.get_device() != dev or sb.get_device() != dev:
         raise RuntimeError("mx_gemm requires CUDA tensors of one device")
+    if qa.element_size() != 1 or qb.element_size() != 1 or sa.element_size() != 1 or sb.element_size() != 1:
+        raise RuntimeError("mx_gemm expects packed bytes and one-byte scales")
     m, kh = qa.shape
     n, kh2 = qb.shape
     k = 2 * kh
@@ -485,7 +488,7 @@ def mx_linear(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, bias: Optiona
     if k == 0 or k % 32 or n % 8:
         raise RuntimeError("mx_linear needs K divisible by 32 and N by 8")
     dev = x.get_device()
-    if (qw.get_device() != dev or sw.get_device() != dev or not qw.is_contiguous() or not sw.is_contiguous()
+    if (qw.get_device() != dev or sw.get_device() != dev or qw.element_size() != 1 or sw.element_size() != 1 or not qw.is_contiguous() or not sw.is_contiguous()
             or sw.numel() != (n + 127) // 128 * 128 * ((k + 127) // 128 * 4)):
         raise RuntimeError("the weight is contiguous q [n, k/2] and its padded swizzled scales on x's device")
     if bias is not None:

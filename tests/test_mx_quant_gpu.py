@@ -316,3 +316,61 @@ def test_other_stream_and_graph(pkg, f4):
         assert torch.equal(out, ops.mx_linear(new, qw, sw))
         for a, b in zip(both, ops.mx_quantize_both(new)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("m", [1, 5, 12, 13, 40])
+def test_linear_right_after_its_operands(pkg, m):
+    """The product is launched while the kernel before it may still run: weights
+    and tokens written just before must be the ones it reads, call after call,
+    eagerly and replayed."""
+    ops = pkg.ops
+    n, k = 1024, 2048
+    ws = [make(n, k, torch.bfloat16, s) for s in (1, 2, 3)]
+    xs = [make(m, k, torch.bfloat16, s) for s in (4, 5, 6)]
+    held = [ops.mx_quantize(w) for w in ws]
+    torch.cuda.synchronize()
+    ref = []
+    for x, h in zip(xs, held):
+        ref.append(ops.mx_linear(x, *h))
+        torch.cuda.synchronize()
+    buf_w, buf_x = ws[0].clone(), xs[0].clone()
+    out = (torch.empty_like(held[0][0]), torch.empty_like(held[0][1]))
+
+    def step(i):
+        buf_w.copy_(ws[i])
+        ops.mx_quantize(buf_w, out=out)          # the weights, just before
+        y = ops.mx_linear(xs[i], *out)
+        buf_x.copy_(xs[i])                       # the tokens, just before
+        return y, ops.mx_linear(buf_x, *out)
+
+    for rep in range(20):
+        i = rep % 3
+        for y in step(i):
+            assert torch.equal(y, ref[i]), rep
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ys = [y for i in range(3) for y in step(i)]
+    for _ in range(5):
+        for y in ys:
+            y.zero_()
+        graph.replay()
+        assert all(torch.equal(y, ref[j // 2]) for j, y in enumerate(ys))
+    assert ops.device_error() == 0
+
+
+def test_linear_on_two_streams_at_once(pkg):
+    """Few-token products of both forms and a large one side by side."""
+    ops = pkg.ops
+    w = ops.mx_quantize(make(4096, 4096, torch.bfloat16, 1))
+    xs = [make(m, 4096, torch.bfloat16, m) for m in (1, 30, 100, 300)]
+    ref = [ops.mx_linear(x, *w) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(10):
+        got = []
+        for x, st in zip(xs, streams):
+            with torch.cuda.stream(st):
+                got.append(ops.mx_linear(x, *w))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    assert ops.device_error() == 0
