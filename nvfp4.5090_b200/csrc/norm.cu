@@ -49,31 +49,31 @@ __device__ __forceinline__ int column(int t, int j) {
 }
 
 // One row's elements of a tensor as raw vectors (VEC) or floats.
-template <int DT, bool VEC, int TPR>
+template <int DT, bool VEC, int TPR, int V = VPT>
 struct Row {
-  typename Elem<DT>::Vec8 v[VEC ? VPT : 1];
-  float f[VEC ? 1 : CPT];
+  typename Elem<DT>::Vec8 v[VEC ? V : 1];
+  float f[VEC ? 1 : 8 * V];
 
   __device__ __forceinline__ void load(const typename Elem<DT>::Raw* p, int t, int d) {
     if (VEC) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
+      for (int i = 0; i < V; ++i) {
         const int c = column<true, TPR>(t, 8 * i);
         v[i] = Elem<DT>::zero();
         if (c < d) v[i] = Elem<DT>::load(p + c);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < CPT; ++j) {
+      for (int j = 0; j < 8 * V; ++j) {
         const int c = column<false, TPR>(t, j);
         f[j] = c < d ? Elem<DT>::get(p + c) : 0.0f;
       }
     }
   }
-  __device__ __forceinline__ void values(float (&o)[CPT]) const {
+  __device__ __forceinline__ void values(float (&o)[8 * V]) const {
     if (VEC) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
+      for (int i = 0; i < V; ++i) {
         float t[8];
         Elem<DT>::unpack(v[i], t);
 #pragma unroll
@@ -81,17 +81,17 @@ struct Row {
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < CPT; ++j) o[j] = f[j];
+      for (int j = 0; j < 8 * V; ++j) o[j] = f[j];
     }
   }
 };
 
 // Rounds the values to the stored type and writes them.
-template <int DT, bool VEC, int TPR>
-__device__ __forceinline__ void store_row(typename Elem<DT>::Raw* p, int t, int d, const float (&o)[CPT]) {
+template <int DT, bool VEC, int TPR, int V = VPT>
+__device__ __forceinline__ void store_row(typename Elem<DT>::Raw* p, int t, int d, const float (&o)[8 * V]) {
   if (VEC) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
+    for (int i = 0; i < V; ++i) {
       const int c = column<true, TPR>(t, 8 * i);
       float f[8];
 #pragma unroll
@@ -100,7 +100,7 @@ __device__ __forceinline__ void store_row(typename Elem<DT>::Raw* p, int t, int 
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < CPT; ++j) {
+    for (int j = 0; j < 8 * V; ++j) {
       const int c = column<false, TPR>(t, j);
       if (c < d) p[c] = Elem<DT>::bits(o[j]);
     }
@@ -372,6 +372,7 @@ struct BwdArgs {
   int64_t rows, ldb, ld_dy, ld_dn, ldy, rows_per_gate, rows_per_cta;
   int d;
   float alpha, s;
+  int stages;               // staged kernel: rows of the ring
   int ws16;                 // part and part_gate are 16-byte aligned
 };
 
@@ -379,9 +380,10 @@ struct BwdArgs {
 // divides rows_per_gate or is a multiple of it, so a CTA's rows lie in one
 // group or are whole groups.  (Groups of rows that end early are handled by
 // the host: parts of a group are cut at its end.)
-template <int DT, bool VEC, int TPR>
+template <int DT, bool VEC, int TPR, int V>
 __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int64_t parts_per_group) {
   using Raw = typename Elem<DT>::Raw;
+  constexpr int C = 8 * V;   // columns per thread
   __shared__ float red[4][TPR / 32];
   const int t = threadIdx.x;
   const float inv_d = 1.0f / (float)a.d;
@@ -395,30 +397,30 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
     r = (int64_t)blockIdx.x * a.rows_per_cta;
     end = imin64(r + a.rows_per_cta, a.rows);
   }
-  float S[CPT], post[CPT], pre[CPT];
+  float S[C], post[C], pre[C];
 #pragma unroll
-  for (int j = 0; j < CPT; ++j) S[j] = post[j] = pre[j] = 0.0f;
+  for (int j = 0; j < C; ++j) S[j] = post[j] = pre[j] = 0.0f;
   int buf = 0;
   for (; r < end; ++r) {
-    Row<DT, VEC, TPR> row, rb, rw;
-    float tt[CPT], z[CPT], w[CPT], v[CPT];
+    Row<DT, VEC, TPR, V> row, rb, rw;
+    float tt[C], z[C], w[C], v[C];
     if (a.dy) row.load(static_cast<const Raw*>(a.dy) + r * a.ld_dy, t, a.d);
     rb.load(static_cast<const Raw*>(a.b) + r * a.ldb, t, a.d);
     if (a.dy) {
       row.values(tt);
     } else {
 #pragma unroll
-      for (int j = 0; j < CPT; ++j) tt[j] = 0.0f;
+      for (int j = 0; j < C; ++j) tt[j] = 0.0f;
     }
     if (a.dn) {
-      Row<DT, VEC, TPR> rn, ry;
+      Row<DT, VEC, TPR, V> rn, ry;
       rn.load(static_cast<const Raw*>(a.dn) + r * a.ld_dn, t, a.d);
       ry.load(static_cast<const Raw*>(a.y) + r * a.ldy, t, a.d);
       rn.values(v);
       ry.values(z);
       const float inv = __ldg(a.inv_y + r);
 #pragma unroll
-      for (int j = 0; j < CPT; ++j) {
+      for (int j = 0; j < C; ++j) {
         z[j] *= inv;
         pre[j] = fmaf(v[j], z[j], pre[j]);
       }
@@ -426,19 +428,19 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
         rw.load(static_cast<const Raw*>(a.gamma_pre), t, a.d);
         rw.values(w);
 #pragma unroll
-        for (int j = 0; j < CPT; ++j) v[j] *= w[j];
+        for (int j = 0; j < C; ++j) v[j] *= w[j];
       }
       float dot = 0.0f;
 #pragma unroll
-      for (int j = 0; j < CPT; ++j) dot = fmaf(v[j], z[j], dot);
+      for (int j = 0; j < C; ++j) dot = fmaf(v[j], z[j], dot);
       const float mean = row_sum<TPR>(dot, red[buf], 0) * inv_d;
 #pragma unroll
-      for (int j = 0; j < CPT; ++j) tt[j] = fmaf(inv, fmaf(-mean, z[j], v[j]), tt[j]);
+      for (int j = 0; j < C; ++j) tt[j] = fmaf(inv, fmaf(-mean, z[j], v[j]), tt[j]);
     }
     const float inv = __ldg(a.inv_b + r);
     rb.values(z);
 #pragma unroll
-    for (int j = 0; j < CPT; ++j) {
+    for (int j = 0; j < C; ++j) {
       z[j] *= inv;
       v[j] = a.s * tt[j];
       S[j] = fmaf(v[j], z[j], S[j]);
@@ -447,24 +449,24 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
       rw.load(static_cast<const Raw*>(a.gamma_post), t, a.d);
       rw.values(w);
 #pragma unroll
-      for (int j = 0; j < CPT; ++j) v[j] *= w[j];
+      for (int j = 0; j < C; ++j) v[j] *= w[j];
     }
     if (a.gate) {
       rw.load(static_cast<const Raw*>(a.gate) + (r / a.rows_per_gate) * a.d, t, a.d);
       rw.values(w);
 #pragma unroll
-      for (int j = 0; j < CPT; ++j) v[j] *= w[j];
+      for (int j = 0; j < C; ++j) v[j] *= w[j];
     }
     float dot = 0.0f;
 #pragma unroll
-    for (int j = 0; j < CPT; ++j) dot = fmaf(v[j], z[j], dot);
+    for (int j = 0; j < C; ++j) dot = fmaf(v[j], z[j], dot);
     const float mean = row_sum<TPR>(dot, red[buf + 1], 0) * inv_d;
 #pragma unroll
-    for (int j = 0; j < CPT; ++j) z[j] = inv * fmaf(-mean, z[j], v[j]);
-    store_row<DT, VEC, TPR>(static_cast<Raw*>(a.db) + r * a.d, t, a.d, z);
+    for (int j = 0; j < C; ++j) z[j] = inv * fmaf(-mean, z[j], v[j]);
+    store_row<DT, VEC, TPR, V>(static_cast<Raw*>(a.db) + r * a.d, t, a.d, z);
 #pragma unroll
-    for (int j = 0; j < CPT; ++j) tt[j] *= a.alpha;
-    store_row<DT, VEC, TPR>(static_cast<Raw*>(a.dx) + r * a.d, t, a.d, tt);
+    for (int j = 0; j < C; ++j) tt[j] *= a.alpha;
+    store_row<DT, VEC, TPR, V>(static_cast<Raw*>(a.dx) + r * a.d, t, a.d, tt);
     buf ^= 2;
     // the last row of a group (or of this CTA's part of it): hand S over
     if (a.gate && (r + 1 == end || (r + 1) % a.rows_per_gate == 0)) {
@@ -472,16 +474,16 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
       rw.load(static_cast<const Raw*>(a.gate) + g * a.d, t, a.d);
       rw.values(w);
 #pragma unroll
-      for (int j = 0; j < CPT; ++j) post[j] = fmaf(w[j], S[j], post[j]);
+      for (int j = 0; j < C; ++j) post[j] = fmaf(w[j], S[j], post[j]);
       float* out = parts_per_group > 1 ? a.part_gate + (int64_t)blockIdx.x * a.d : a.dgate ? a.dgate + g * a.d : nullptr;
       if (parts_per_group == 1 && a.gamma_post) {
         rw.load(static_cast<const Raw*>(a.gamma_post), t, a.d);
         rw.values(w);
 #pragma unroll
-        for (int j = 0; j < CPT; ++j) S[j] *= w[j];
+        for (int j = 0; j < C; ++j) S[j] *= w[j];
       }
 #pragma unroll
-      for (int j = 0; j < CPT; ++j) {
+      for (int j = 0; j < C; ++j) {
         const int c = column<VEC, TPR>(t, j);
         if (out && c < a.d) out[c] = S[j];
         S[j] = 0.0f;
@@ -489,7 +491,7 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
     }
   }
 #pragma unroll
-  for (int j = 0; j < CPT; ++j) {
+  for (int j = 0; j < C; ++j) {
     const int c = column<VEC, TPR>(t, j);
     if (c < a.d) {
       a.part[(int64_t)blockIdx.x * a.d + c] = a.gate ? post[j] : S[j];
@@ -515,9 +517,7 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
 // 16 warps did, and waited for one another's barriers (147 us against 134 at 16000 x 4096).
 __device__ int g_norm_error = 0;
 
-// Rows of the ring: two with the next norm's tensors, three without.
-template <bool PRE>
-constexpr int bwd_stages() { return PRE ? 2 : 3; }
+constexpr int BWD_STAGES = 3;   // rows of the ring, at most
 
 // One 8-element vector per thread: TPR threads cover d <= 8 * TPR columns.
 template <int DT, int TPR, bool PRE>
@@ -527,11 +527,11 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
   using Raw = typename E::Raw;
   constexpr int NT = PRE ? 4 : 2;                 // tensors: dy, b [, dn, y]
   constexpr int NP = 4;                           // packed pairs per thread
-  constexpr int ST = bwd_stages<PRE>();
+  const int ST = a.stages;
   constexpr int W4 = (TPR / 32 + 3) / 4;          // 16-byte words of one sum's warp parts
   extern __shared__ __align__(16) uint8_t row_ring[];   // [ST][NT][d], then the column sums
   __shared__ __align__(16) float red[2][3][4 * W4];
-  __shared__ __align__(8) uint64_t full[ST];
+  __shared__ __align__(8) uint64_t full[BWD_STAGES];
   __shared__ int gave_up;
   const int t = threadIdx.x;
   const float inv_d = 1.0f / (float)a.d;
@@ -930,7 +930,7 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
   nvfp4b200_sandwich_norm_bwd_ws(rows, d, groups, &need);
   if (ws_floats < need) return NVFP4B200_ERR_BAD_SHAPE;
   norm::BwdArgs a{dy, dn, b, y, gamma_post, gate, gamma_pre, inv_b, inv_y, dx, db, ws, ws + 2 * sp.ctas * d, dgate, rows, ldb,
-                  ld_dy, ld_dn, ldy, rows / g, sp.rows_per_cta, (int)d, residual_scale, branch_scale,
+                  ld_dy, ld_dn, ldy, rows / g, sp.rows_per_cta, (int)d, residual_scale, branch_scale, 0,
                   aligned(ws, 16)};
   const bool vec = (d * bytes) % 16 == 0 && d % 8 == 0 && vec_ok(dy, ld_dy, bytes) && vec_ok(dn, ld_dn, bytes) &&
                    vec_ok(b, ldb, bytes) && vec_ok(y, ldy, bytes) && vec_ok(gamma_post, d, bytes) &&
@@ -940,12 +940,17 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
   return norm::by_type(dtype, vec, [&](auto dt, auto v) {
     const int r = norm::by_width((int)d, [&](auto tpr) {
       constexpr int T = decltype(tpr)::value, DT = decltype(dt)::value;
-      // the staged kernel where its ring fits and a CTA's rows have one gate:
+      // the staged kernel where a row fits and a CTA's rows have one gate:
       // 346 -> 152 us at 16000 x 4096 bf16 with 8 gates and the next norm
       if constexpr (decltype(v)::value && T <= 512) {
         constexpr int T2 = 2 * T;
-        const int stages = dn ? norm::bwd_stages<true>() : norm::bwd_stages<false>();
-        const int smem = stages * (dn ? 4 : 2) * (int)d * norm::dtype_size<DT>() + (dn ? 4 : 2) * 16 * T2;
+        // two CTAs' worth of threads share an SM (fewer where one is that large), and
+        // so its memory: as many ring rows as fit, up to 3 (2 with the next norm's
+        // tensors); one row at least, alone on the SM if need be
+        const int row = (dn ? 4 : 2) * (int)d * norm::dtype_size<DT>(), sums = (dn ? 4 : 2) * 16 * T2;
+        const int share = norm::MAX_SMEM / std::max(1, 1024 / T2);
+        a.stages = std::max(std::min(dn ? 2 : norm::BWD_STAGES, (share - sums) / row), 1);
+        const int smem = a.stages * row + sums;
         if (smem <= norm::MAX_SMEM && (!gate || sp.parts_per_group > 1)) {
           auto* fn = dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true> : norm::sandwich_bwd_staged_kernel<DT, T2, false>;
           if (smem > 32 * 1024 &&   // with the static arrays, past the default limit
@@ -955,8 +960,10 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
           return launch_status();
         }
       }
-      norm::sandwich_bwd_kernel<decltype(dt)::value, decltype(v)::value, T>
-          <<<(unsigned)sp.ctas, T, 0, st>>>(a, sp.parts_per_group);
+      // 8 columns a thread while 1024 threads cover the row: twice the warps of 16
+      // columns (166 -> 123 us at 2013 x 4971 fp16)
+      constexpr int T2 = T <= 512 ? 2 * T : T, V = T <= 512 ? 1 : norm::VPT;
+      norm::sandwich_bwd_kernel<DT, decltype(v)::value, T2, V><<<(unsigned)sp.ctas, T2, 0, st>>>(a, sp.parts_per_group);
       return launch_status();
     });
     if (r) return r;

@@ -10,6 +10,7 @@ system).  Packed E2M1 tensors are returned as ``uint8``; the
 from __future__ import annotations
 
 import array
+import functools
 import math
 import operator
 from typing import Optional, Sequence, Tuple, Union
@@ -712,8 +713,9 @@ def sandwich_norm(b: torch.Tensor, x: torch.Tensor, gamma_post: Optional[torch.T
     return y, n, inv_b, inv_y
 
 
+@functools.lru_cache(maxsize=1024)
 def _bwd_words(dev: int, t: int, d: int, groups: int) -> int:
-    """fp32 words of workspace of the backward on a device."""
+    """fp32 words of workspace of the backward on a device: a function of the sizes alone."""
     floats = _lib.c_i64(0)
     args = ("nvfp4b200_sandwich_norm_bwd_ws", t, d, groups, _lib.ctypes.byref(floats))
     if dev == _current_device():
@@ -753,12 +755,12 @@ def sandwich_norm_bwd(dy: Optional[torch.Tensor], b: torch.Tensor, inv_b: torch.
             raise RuntimeError("inv_b and inv_y are contiguous float32 [T]")
     gamma_post, gate, gamma_pre, groups = _norm_params(b, gamma_post, gate, gamma_pre)
     b = _rows_of(b)
-    dy, dn, y = (None if g is None else _rows_of(g) for g in (dy, dn, y))
+    dy, dn, y = [None if g is None else _rows_of(g) for g in (dy, dn, y)]
     dx, db = b.new_empty((t, d)), b.new_empty((t, d))
     # the parameters' gradients: dgamma_post, dgamma_pre (with dn), dgate
     par = torch.empty((groups + 1 + (dn is not None), d), device=b.device, dtype=torch.float32)
     dpost, dpre = par[0], (par[1] if dn is not None else None)
-    dgate = par[par.shape[0] - groups:] if groups else None
+    dgate = par[-groups:] if groups else None
     if t == 0:
         par.zero_()
     else:
