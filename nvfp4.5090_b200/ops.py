@@ -502,8 +502,9 @@ def mx_linear(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, bias: Optiona
     if m and n:
         # few tokens are quantized inside the product: no workspace
         fused = m <= 12 and _lib.load().nvfp4b200_mx_linear_fused(m, n, k)
-        qx, sx = (None, None) if fused else _mx_pair(m, k, x.device, None)
-        _run(x2, "nvfp4b200_mx_linear", x2.data_ptr(), qw.data_ptr(), sw.data_ptr(), _ptr(bias), _ptr(qx), _ptr(sx),
+        held = None if fused else MXOperand(m, k, x2)
+        qx, sx = (None, None) if fused else held.pointers()
+        _run(x2, "nvfp4b200_mx_linear", x2.data_ptr(), qw.data_ptr(), sw.data_ptr(), _ptr(bias), qx, sx,
              y.data_ptr(), m, n, k, max(x2.stride(0), k))
     return y
 
