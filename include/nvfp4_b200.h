@@ -255,8 +255,8 @@ int nvfp4b200_mx_linear_fused(int64_t m, int64_t n, int64_t k);
 /* y = Q(x) . W^T + bias for W held in MXFP4: x bf16 [m, k] (row stride ldx) is
  * quantized along k, into qx [m, k/2] and sfx (as nvfp4b200_mx_quant's q and s;
  * may be NULL where nvfp4b200_mx_linear_fused says so), and multiplied: up to
- * 128 tokens by a kernel that streams the weights over all SMs, more by
- * nvfp4b200_mx_gemm.  qw [n, k/2], sfw: the weight; bias bf16
+ * 128 tokens (more where n is small) by a kernel that spreads the weights over
+ * all SMs, else by nvfp4b200_mx_gemm.  qw [n, k/2], sfw: the weight; bias bf16
  * [n] or NULL; y bf16 [m, n].  k % 32 == 0, n % 8 == 0. */
 int nvfp4b200_mx_linear(const void* x, const void* qw, const void* sfw, const void* bias, void* qx, void* sfx,
                         void* y, int64_t m, int64_t n, int64_t k, int64_t ldx, void* stream);

@@ -1,4 +1,4 @@
-// MXFP4 linear layer for few tokens (B200, sm_100a): y = Q(x) . W^T + bias
+// MXFP4 linear layer for few tokens, or few outputs (B200, sm_100a): y = Q(x) . W^T + bias
 // with W held in MXFP4.
 //
 // With few tokens the product is a stream of the weights (17/32 byte per
@@ -9,7 +9,7 @@
 // cluster, so that 128-row tiles x K parts fill the SMs.  The parts' fp32 sums
 // meet through distributed shared memory in one fixed order.
 //
-//   grid (tiles * parts), cluster (parts): CTA rank r of a cluster takes every
+//   grid (tiles * parts, blocks of N tokens), cluster (parts): CTA rank r of a cluster takes every
 //     stage (256 k) of its share of K for 128 weight rows;
 //   warp 0      producer: weights (one 128-byte-swizzled TMA box of 128 rows x
 //               128 bytes, and their 2 scale atoms) per stage into a ring of up
@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank(), parts = (int)cluster_size();
   const int tile = blockIdx.x / parts;
+  const int tok0 = blockIdx.y * N;   // N = 128 where there is more than one block of tokens
   const int k_lo = (int)((int64_t)a.k_stages * rank / parts), k_hi = (int)((int64_t)a.k_stages * (rank + 1) / parts);
   const int steps = k_hi - k_lo;
   // weights of every stage and tokens (1024-byte aligned), then the scales; the
@@ -199,8 +200,8 @@ __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constan
     };
     auto tokens = [&](int i, int st) {
       if (FUSED) return;
-      tma_2d(s_b + st * N * BK_BYTES, &xmap, &full[st], (k_lo + i) * BK_BYTES, 0);
-      bulk::copy(s_sfb + st * SF_BYTES, a.sfx + (int64_t)2 * (k_lo + i) * 512, sf_bytes(i), &full[st]);
+      tma_2d(s_b + st * N * BK_BYTES, &xmap, &full[st], (k_lo + i) * BK_BYTES, tok0);
+      bulk::copy(s_sfb + st * SF_BYTES, a.sfx + ((int64_t)blockIdx.y * a.atoms + 2 * (k_lo + i)) * 512, sf_bytes(i), &full[st]);
     };
     const int first = min(steps, a.stages);
     // FUSED: whatever ran before may have written the weights themselves
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constan
   // ---- epilogue: this part's sums as [token][row], over the ring (every MMA has read it) ----
   __syncthreads();
   float* part = reinterpret_cast<float*>(smem);
-  const int m = (int)a.m;
+  const int m = (int)imin64(N, a.m - tok0);   // tokens of this block
   {
     const int row = 32 * (warp & 3) + lane;   // a warp reads the TMEM lanes of its quarter
     for (int t = 16 * (warp >> 2); t < m; t += 32) {
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constan
         }
       const __nv_bfloat162 lo = __floats2bfloat162_rn(s.x + bias[0], s.y + bias[1]);
       const __nv_bfloat162 hi = __floats2bfloat162_rn(s.z + bias[2], s.w + bias[3]);
-      *reinterpret_cast<uint2*>(a.y + (int64_t)t * a.n + row) =
+      *reinterpret_cast<uint2*>(a.y + (int64_t)(tok0 + t) * a.n + row) =
           make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
     }
   }
@@ -428,7 +429,7 @@ static int launch(const void* qw, const void* qx, Args a, int parts, cudaStream_
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return NVFP4B200_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * parts), 1, 1);
+  cfg.gridDim = dim3((unsigned)(tiles * parts), (unsigned)ceil_div(a.m, N), 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -460,6 +461,14 @@ int take_mxlin_device_error() {
 }  // namespace nvfp4b200
 
 using namespace nvfp4b200;
+
+// Whether the 128-row tiles, times blocks of 128 tokens, beat the 256 x 256 pair
+// tiles of the general GEMM: always for one block of tokens, and while there is
+// an SM for each of them.  Against the general GEMM (quantizer included): 256
+// tokens 18.7 / 27.2 us at 4096 x 14336 (64 tiles), 512 tokens 14.2 / 15.1 at 4096
+// x 4096 (128 tiles); 768 tokens 17.5 / 15.7 there (192 tiles), 256 tokens 18.3 /
+// 16.3 at 14336 x 4096 (224 tiles).
+static bool few_tokens(int64_t m, int64_t tiles, int sms) { return m <= 128 || tiles * ceil_div(m, 128) <= sms; }
 
 extern "C" {
 
@@ -497,14 +506,14 @@ int nvfp4b200_mx_linear(const void* x, const void* qw, const void* sfw, const vo
   a.atoms = (int)ceil_div(k, 128);
   a.k_stages = (int)ceil_div(k, mxlin::BK);
   a.stages = 0;
-  int parts = mxlin::parts_for(tiles, a.k_stages, sms);
+  int parts = mxlin::parts_for(tiles * ceil_div(m, 128), a.k_stages, sms);
   if (fused) {
     while (ceil_div(a.k_stages, parts) > mxlin::FUSED_STEPS) parts *= 2;
     return mxlin::launch<16, true>(qw, nullptr, a, parts, st);
   }
   rc = mx_quant_rows_async(x, qx, sfx, m, k, ldx, st);
   if (rc) return rc;
-  if (m > 128)
+  if (!few_tokens(m, tiles, sms))
     return nvfp4b200_mx_gemm(qx, qw, sfx, sfw, bias, nullptr, y, NVFP4B200_BF16, 0, NVFP4B200_EPI_NONE, m, n, k, n,
                              stream);
   if (m <= 16) return mxlin::launch<16, false>(qw, qx, a, parts, st);

@@ -78,6 +78,20 @@ def test_clip_in_place_and_out(pkg, sizes, dtypes, max_norm):
         assert all(torch.equal(a, b) for a, b in zip(grads, keep))
 
 
+def test_offsets_past_32_bits(pkg):
+    """One gradient of more than 2^31 elements, misaligned and not."""
+    big = torch.full((2 ** 31 + 4099,), 0.5, device="cuda", dtype=BF)
+    for g in (big, big[1:]):
+        ref = 0.5 * math.sqrt(g.numel())
+        n = pkg.ops.clip_grad_norm(g, ref / 4, out=[g.new_empty(g.shape)])
+        assert abs(n.item() - ref) <= REL * ref
+    big[-1] = 2000.0
+    n = pkg.ops.clip_grad_norm(big, 1e9, math.inf)
+    assert n.item() == 2000.0
+    pkg.ops.clip_grad_norm(big, 1000.0, math.inf)          # halves every value exactly, to within the 1e-6
+    assert big[-1].item() == 1000.0 and big[0].item() == 0.25 and big[2 ** 31 + 7].item() == 0.25
+
+
 def test_misaligned_views_and_layouts(pkg):
     """Views at odd offsets of one buffer, transposed and permuted gradients."""
     flat = tensors([10_007], [BF])[0]

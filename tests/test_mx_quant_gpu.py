@@ -136,8 +136,7 @@ def test_out_tensors_and_no_rows(pkg):
 
 
 def test_wide_and_long(pkg):
-    """More than 2^31 elements' worth of offsets is out of a test's reach; rows
-    past 2^16 tiles and odd tails are not: sampled rows of 70000 x 1056 against the restatement."""
+    """Many row tiles and odd tails: sampled rows of 70001 x 1056 against the restatement."""
     x = make(70001, 1056, torch.bfloat16, 3)
     q, s, qt, st = pkg.ops.mx_quantize_both(x)
     d = pkg.ops.mx_dequantize(q, s)
@@ -149,6 +148,24 @@ def test_wide_and_long(pkg):
     sub = f64(x[:, cols])
     ref = orc.dequant_mxfp4(*mxo.quantize_t(sub), len(cols), 70016)
     assert np.array_equal(f64(dt[cols]), ref)
+
+
+def test_offsets_past_32_bits(pkg):
+    """More than 2^31 elements: sampled rows and columns of both orientations."""
+    r, c = 66000, 32768
+    x = torch.empty(r, c, device="cuda", dtype=torch.bfloat16)
+    for lo in range(0, r, 11000):
+        x[lo:lo + 11000] = make(11000, c, torch.bfloat16, lo)
+    rows = torch.tensor([0, 65535, 65536, 65999], device="cuda")
+    cols = torch.tensor([0, 17, 32767], device="cuda")
+    q, s, qt, st = pkg.ops.mx_quantize_both(x)
+    xr, xc = f64(x[rows]), f64(x[:, cols])
+    del x
+    d = pkg.ops.mx_dequantize(q, s)
+    assert np.array_equal(f64(d[rows]), orc.dequant_mxfp4(*mxo.quantize(xr), len(rows), c))
+    del d, q, s
+    d = pkg.ops.mx_dequantize(qt, st)
+    assert np.array_equal(f64(d[cols]), orc.dequant_mxfp4(*mxo.quantize_t(xc), len(cols), d.shape[1]))
 
 
 def product(qa, sa, qb, sb, m, n, k):
@@ -165,7 +182,8 @@ def check(d, ref, mag, bf16=True):
 
 @pytest.mark.parametrize("m,n,k", [(1, 8, 32), (1, 4096, 1024), (2, 264, 96), (3, 520, 4096), (7, 1000, 352), (8, 2048, 2048),
                                    (9, 128, 14336), (16, 136, 512), (17, 640, 1056), (31, 256, 256), (33, 384, 640),
-                                   (64, 1032, 288), (65, 136, 1024), (129, 256, 96), (300, 520, 1024)])
+                                   (64, 1032, 288), (65, 136, 1024), (129, 256, 96), (300, 520, 1024), (257, 4096, 2048), (1000, 1024, 512),
+                                                   (700, 4608, 256)])
 @pytest.mark.parametrize("with_bias", [False, True])
 def test_mx_linear(pkg, m, n, k, with_bias):
     ops = pkg.ops

@@ -333,3 +333,26 @@ def test_layer_step_together(pkg, f4):
         pkg.ops.adamw_step(p.data.view(-1), g.view(-1), m, v, lr=1e-2, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0, step=1)
     assert all(not torch.equal(p, q) and torch.isfinite(p).all() for p, q in zip(params, before))
     assert pkg.ops.device_error() == 0
+
+
+def test_offsets_past_32_bits(pkg):
+    """More than 2^31 elements, forward and backward: the last rows against the same
+    rows alone."""
+    ops = pkg.ops
+    t, d = 133000, 16384
+    b = torch.empty(t, d, device="cuda", dtype=BF)
+    for lo in range(0, t, 13300):
+        b[lo:lo + 13300] = rnd((13300, d), lo, BF)
+    x, gp, gn = b.flip(0), rnd((d,), 1, BF), rnd((d,), 2, BF)
+    gate = rnd((2, d), 3, BF)
+    y, n, ib, iy = ops.sandwich_norm(b, x, gp, gate, gn)
+    last = slice(t - 40, t)
+    y2, n2, ib2, iy2 = ops.sandwich_norm(b[last], x[last], gp, gate[1:], gn)
+    for a, r in ((y, y2), (n, n2), (ib, ib2), (iy, iy2)):
+        assert torch.equal(a[last], r)
+    del n
+    g = ops.sandwich_norm_bwd(x, b, ib, gp, gate, dn=b, y=y, inv_y=iy, gamma_pre=gn)
+    g2 = ops.sandwich_norm_bwd(x[last], b[last], ib2, gp, gate[1:], dn=b[last], y=y2, inv_y=iy2, gamma_pre=gn)
+    for k in ("dx", "db"):
+        assert torch.equal(g[k][last], g2[k])
+    assert all(torch.isfinite(g[k]).all() for k in ("dgamma_post", "dgate", "dgamma_pre"))
