@@ -7,7 +7,7 @@ under the name ``nvfp4_b200`` (``__graft_entry__.import_package()`` or
 ``importlib`` with ``submodule_search_locations``).  All compute goes through
 the CUDA library ``lib/libnvfp4b200.so``; there is no CPU fallback.
 """
-from . import _build, _lib, ops  # noqa: F401
+from . import _bind, _build, _lib, ops  # noqa: F401
 from ._lib import NVFP4Error  # noqa: F401
 
 __version__ = "0.1.0"

@@ -3,7 +3,9 @@
 nvcc compiles each ``csrc/*.cu`` for ``-gencode arch=compute_100a,code=sm_100a``
 into ``_build/`` and links one shared object with the CUDA runtime linked
 statically, so the library depends only on the driver (libcuda) at run time
-and can be loaded next to any PyTorch build.
+and can be loaded next to any PyTorch build.  ``build_binding`` compiles the
+torch extension module on top of it (csrc/torch_binding.cpp, host code only)
+against the installed PyTorch.
 """
 from __future__ import annotations
 
@@ -18,6 +20,8 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libnvfp4b200.so")
+BINDING_NAME = "_nvfp4b200_torch"
+BINDING_PATH = os.path.join(LIB_DIR, BINDING_NAME + ".so")
 SOURCES = ["quant.cu", "gemm.cu", "train.cu", "noalloc.cu", "mx.cu", "mxlin.cu", "clip.cu", "norm.cu"]
 HEADERS = [os.path.join(CSRC, "common.cuh"), os.path.join(CSRC, "vec.cuh"), os.path.join(CSRC, "bulk.cuh"), os.path.join(CSRC, "mx.cuh"),
            os.path.join(REPO_DIR, "include", "nvfp4_b200.h")]
@@ -61,7 +65,40 @@ def build(force: bool = False, verbose: bool = False) -> str:
             print(" ".join(cmd), file=sys.stderr)
         subprocess.run(cmd, check=True)
         os.replace(tmp, LIB_PATH)
+    build_binding(force, verbose)
     return LIB_PATH
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> str:
+    """Compile (if needed) the torch extension module next to the library."""
+    src = os.path.join(CSRC, "torch_binding.cpp")
+    header = os.path.join(REPO_DIR, "include", "nvfp4_b200.h")
+    if not force and not _stale(BINDING_PATH, [src, header]):
+        return BINDING_PATH
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
+    include = cpp_extension.include_paths() + [cuda, sysconfig.get_paths()["include"]]
+    tmp = BINDING_PATH + ".tmp"
+    # the system compiler, whose C++ runtime is the shared one that libtorch uses: with a
+    # second copy linked in, an exception that crosses the two crashes the process
+    cxx = next((c for c in ("/usr/bin/g++", shutil.which("g++")) if c and os.path.exists(c)), None)
+    if cxx is None:
+        raise RuntimeError("g++ not found: the torch binding must be compiled with the system's C++ compiler")
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", src, "-o", tmp,
+           f"-DTORCH_EXTENSION_NAME={BINDING_NAME}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for path in include:
+        cmd += ["-isystem", path]
+    cmd += ["-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+            "-ltorch", "-ltorch_python", "-L" + LIB_DIR, "-lnvfp4b200", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, BINDING_PATH)
+    return BINDING_PATH
 
 
 if __name__ == "__main__":

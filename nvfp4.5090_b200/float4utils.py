@@ -24,7 +24,7 @@ from typing import Optional, Tuple
 import torch
 import torch.nn as nn
 
-from . import ops
+from . import _bind, ops
 from .gn_kernels import cutlass_nvfp4_mm, cutlass_nvfp4_mm_relu, cutlass_nvfp4_mm_relu_2
 
 
@@ -407,54 +407,25 @@ class MXFP4LinearFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
-        require(input.is_cuda and input.dtype in (torch.bfloat16, torch.float32),
-                "mxfp4_linear expects a CUDA bf16 or fp32 input.")
-        n, k = weight.shape
-        require(input.shape[-1] == k, f"K mismatch: input has {input.shape[-1]}, weight has {k}")
-        x = input.reshape(-1, k)
-        t = x.shape[0]
-        need_x, need_w = ctx.needs_input_grad[:2]
-        require(not (need_x or need_w) or n % 32 == 0, "training needs out_features divisible by 32")
-        qx, qxt = ops.mx_operands(x, True, need_w)
-        qw, qwt = ops.mx_operands(weight, True, need_x)
-        if bias is not None:
-            require(bias.numel() == n and bias.is_cuda, "bias is a CUDA tensor [N]")
-            ctx.bdtype, bias = bias.dtype, bias.to(torch.bfloat16).contiguous()
-        else:
-            ctx.bdtype = None
-        require(n % 8 == 0, "out_features must be divisible by 8")
-        y = ops.mx_product(qx, qw, input.dtype, bias)
-        ctx.save_for_backward(qxt.buf if need_w else None, qwt.buf if need_x else None)
-        ctx.shape, ctx.tokens, ctx.n, ctx.wdtype = input.shape, t, n, weight.dtype
-        if input.dim() == 2:
-            return y
-        # not a view, so that users may change the result in place
-        return torch.ops.aten._unsafe_view(y, [*input.shape[:-1], n])
+        y, xt, wt = _bind.ext.linear_forward(input, weight, bias, *ctx.needs_input_grad[:2])
+        ctx.save_for_backward(xt, wt)
+        ctx.shape, ctx.n, ctx.wdtype = input.shape, weight.shape[0], weight.dtype
+        ctx.bdtype = None if bias is None else bias.dtype
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output: torch.Tensor):
         xt, wt = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
-        n, k, t = ctx.n, ctx.shape[-1], ctx.tokens
-        dy = grad_output if grad_output.dim() == 2 else grad_output.reshape(-1, n)
         dx = dw = db = None
         if need_x or need_w:
-            qd, qdt = ops.mx_operands(dy, need_x, need_w)
-        if need_x:
-            dx = ops.mx_product(qd, ops.MXOperand(k, n, dy, wt), grad_output.dtype)
-            if len(ctx.shape) != 2:
-                dx = dx.view(ctx.shape)
-        if need_w:
-            if t:
-                out_dtype = torch.float32 if ctx.wdtype == torch.float32 else torch.bfloat16
-                dw = ops.mx_product(qdt, ops.MXOperand(k, (t + 31) // 32 * 32, dy, xt), out_dtype)
-                if dw.dtype != ctx.wdtype:
-                    dw = dw.to(ctx.wdtype)
-            else:
-                dw = torch.zeros((n, k), device=dy.device, dtype=ctx.wdtype)
+            dx, dw = _bind.ext.linear_backward(grad_output, xt, wt, ctx.shape, ctx.n, need_x, need_w,
+                                               ctx.wdtype == torch.float32)
+            if dw is not None and dw.dtype != ctx.wdtype:
+                dw = dw.to(ctx.wdtype)
         if ctx.bdtype is not None and ctx.needs_input_grad[2]:
-            db = dy.sum(dim=0, dtype=torch.float32).to(ctx.bdtype)
+            db = grad_output.reshape(-1, ctx.n).sum(dim=0, dtype=torch.float32).to(ctx.bdtype)
         return dx, dw, db
 
 

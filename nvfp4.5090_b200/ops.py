@@ -1,5 +1,8 @@
 """Torch-tensor wrappers over the C ABI: allocation, validation, stream.
 
+The MXFP4, clipping and sandwich-norm functions do these in C++
+(csrc/torch_binding.cpp), the others here.
+
 Every function enqueues on the current CUDA stream of the input's device
 (the reference's GEMM op does the same, cutlass_mm_fp4.cu:266; unlike the
 reference's CuPy quantizer launches, nothing here runs on a second stream
@@ -9,19 +12,15 @@ system).  Packed E2M1 tensors are returned as ``uint8``; the
 """
 from __future__ import annotations
 
-import array
-import functools
 import math
-import operator
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
-from . import _lib
+from . import _bind, _lib
 
 EPI_NONE, EPI_RELU, EPI_RELU2 = 0, 1, 2
 _DT_BF16, _DT_F32 = 0, 1
-_DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 
 
 def round_up(x: int, m: int) -> int:
@@ -57,22 +56,6 @@ def _scalar_f32(g: Optional[torch.Tensor], device) -> Optional[torch.Tensor]:
              "global scales are 1-element float32 CUDA tensors")
     _require(g.device == device, "global scale on a different device")
     return g
-
-
-# The current device and its current stream's handle, without building the
-# device and stream objects of torch.cuda (0.2 us a call in place of 3.4 us).
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: torch.cuda.current_stream(dev).cuda_stream)
-
-
-def _run(t: torch.Tensor, name: str, *args) -> None:
-    """Call an entry point on the device of ``t`` and that device's current stream."""
-    dev = t.get_device()
-    if dev == _current_device():
-        _lib.call(name, *args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            _lib.call(name, *args, _raw_stream(dev))
 
 
 _WS = {}
@@ -284,62 +267,6 @@ def gemm(qa: torch.Tensor, sa: torch.Tensor, qb: torch.Tensor, sb: torch.Tensor,
 # ----------------------------------------------------------------------------
 
 
-def _float_matrix(x: torch.Tensor) -> torch.Tensor:
-    """x as the MXFP4 quantizers read it: 2-D, unit column stride, 16-byte
-    aligned rows; copied when it is laid out otherwise."""
-    if not (x.is_cuda and x.dtype in _DTYPES and x.dim() == 2):
-        raise RuntimeError("MXFP4 quantizers expect a 2-D CUDA bf16, fp16 or fp32 tensor")
-    if x.data_ptr() % 16 == 0:
-        rs, cs = x.stride()
-        if cs == 1 and rs >= x.shape[1] and rs % 8 == 0:
-            return x
-    return x.clone(memory_format=torch.contiguous_format)
-
-
-def _mx_factors(x: torch.Tensor, row_scale, gamma):
-    r, c = x.shape
-    if row_scale is not None:
-        _require(row_scale.dtype == torch.float32 and row_scale.numel() == r and row_scale.device == x.device,
-                 "row_scale is float32 [R] on the input's device")
-        row_scale = row_scale.contiguous()
-    if gamma is not None:
-        _check_bf16(gamma, "gamma")
-        _require(gamma.numel() == c and gamma.device == x.device, "gamma is bf16 [K] on the input's device")
-        gamma = gamma.contiguous()
-        if gamma.data_ptr() % 16:
-            gamma = gamma.clone()
-    return row_scale, gamma
-
-
-def _mx_pair(rows: int, k: int, device, out):
-    """(q, s) tensors of an MXFP4 operand of ``rows`` rows along k."""
-    if out is not None:
-        return _outputs(out, (rows, k // 2), mx_scale_shape(rows, k), device)
-    return (torch.empty((rows, k // 2), device=device, dtype=torch.uint8),
-            torch.empty(mx_scale_shape(rows, k), device=device, dtype=torch.uint8))
-
-
-def _mx_quant(x, row_scale, gamma, rows: bool, cols: bool, out):
-    x = _float_matrix(x)
-    r, c = x.shape
-    if rows and c % 32:
-        raise RuntimeError("K must be divisible by 32 for MXFP4 1x32 scaling.")
-    if c == 0 or c % 8:
-        raise RuntimeError("MXFP4 quantizers need columns divisible by 8")
-    if row_scale is not None or gamma is not None:
-        row_scale, gamma = _mx_factors(x, row_scale, gamma)
-    q = s = qt = st = None
-    dev = x.device
-    if rows:
-        q, s = _mx_pair(r, c, dev, out)
-    if cols:
-        qt, st = _mx_pair(c, (r + 31) // 32 * 32, dev, None if rows else out)
-    if r:
-        _run(x, "nvfp4b200_mx_quant", x.data_ptr(), _DTYPES[x.dtype], _ptr(row_scale), _ptr(gamma), _ptr(q), _ptr(s),
-             _ptr(qt), _ptr(st), r, c, max(x.stride(0), c))
-    return q, s, qt, st
-
-
 def mx_quantize(x: torch.Tensor, row_scale: Optional[torch.Tensor] = None, gamma: Optional[torch.Tensor] = None,
                 out=None):
     """MXFP4-quantize x [R, K] (bf16, fp16 or fp32; K % 32 == 0) along K ->
@@ -350,7 +277,7 @@ def mx_quantize(x: torch.Tensor, row_scale: Optional[torch.Tensor] = None, gamma
     [R]) and ``gamma`` (bf16 [K]) are multiplied in first; a block with an
     infinity or a NaN becomes NaN as a whole.  ``out=(q, s)`` writes into given
     tensors of those shapes."""
-    return _mx_quant(x, row_scale, gamma, True, False, out)[:2]
+    return _bind.ext.mx_quantize(x, row_scale, gamma, out)
 
 
 def mx_quantize_t(x: torch.Tensor, row_scale: Optional[torch.Tensor] = None, gamma: Optional[torch.Tensor] = None,
@@ -358,28 +285,19 @@ def mx_quantize_t(x: torch.Tensor, row_scale: Optional[torch.Tensor] = None, gam
     """MXFP4-quantize x^T (x [R, C], C % 8 == 0) along R -> (q u8 [C, P/2], s
     swizzled for (C, P)), P = R rounded up to 32: the rows past the last count
     as zeros, so a product over P is the product over R."""
-    return _mx_quant(x, row_scale, gamma, False, True, out)[2:]
+    return _bind.ext.mx_quantize_t(x, row_scale, gamma, out)
 
 
 def mx_quantize_both(x: torch.Tensor, row_scale: Optional[torch.Tensor] = None, gamma: Optional[torch.Tensor] = None):
     """Both orientations of x [R, K] from one read: the pairs of ``mx_quantize``
     and ``mx_quantize_t`` as (q, s, qt, st)."""
-    return _mx_quant(x, row_scale, gamma, True, True, None)
+    return _bind.ext.mx_quantize_both(x, row_scale, gamma)
 
 
 def mx_dequantize(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values [R, K] (bf16 or fp32) that an MXFP4 matrix stands for."""
-    _require(q.is_cuda and q.element_size() == 1 and q.dim() == 2, "mx_dequantize expects packed bytes [R, K/2]")
-    r, k = q.shape[0], 2 * q.shape[1]
-    _require(k % 32 == 0, "K must be divisible by 32 for MXFP4 1x32 scaling.")
     _require(dtype in (torch.bfloat16, torch.float32), "output dtype must be bf16 or fp32")
-    _require(s.device == q.device and s.element_size() == 1 and s.numel() == math.prod(mx_scale_shape(r, k)),
-             "MXFP4 scale tensors must be the padded swizzled [round_up(rows,128), round_up(k/32,4)] layout")
-    q, s = q.contiguous(), s.contiguous()
-    y = torch.empty((r, k), device=q.device, dtype=dtype)
-    if r and k:
-        _run(q, "nvfp4b200_mx_dequant", q.data_ptr(), s.data_ptr(), y.data_ptr(), _DTYPES[dtype], r, k)
-    return y
+    return _bind.ext.mx_dequantize(q, s, dtype == torch.float32)
 
 
 def mx_gemm(qa: torch.Tensor, sa: torch.Tensor, qb: torch.Tensor, sb: torch.Tensor, *,
@@ -390,123 +308,14 @@ def mx_gemm(qa: torch.Tensor, sa: torch.Tensor, qb: torch.Tensor, sb: torch.Tens
     ``gemm`` for 1x32 blocks with UE8M0 scales.
 
     qa: [m, k/2], qb: [n, k/2] packed bytes; fp32 outputs can accumulate."""
-    dev = qa.get_device()
-    if not qa.is_cuda or sa.get_device() != dev or qb.get_device() != dev or sb.get_device() != dev:
-        raise RuntimeError("mx_gemm requires CUDA tensors of one device")
-    if qa.element_size() != 1 or qb.element_size() != 1 or sa.element_size() != 1 or sb.element_size() != 1:
-        raise RuntimeError("mx_gemm expects packed bytes and one-byte scales")
-    m, kh = qa.shape
-    n, kh2 = qb.shape
-    k = 2 * kh
-    if kh != kh2:
-        raise RuntimeError(f"K mismatch: A has {k}, B has {2 * kh2}")
-    if k == 0 or k % 32:
-        raise RuntimeError("K must be divisible by 32 for MXFP4 1x32 scaling.")
-    if not (qa.is_contiguous() and qb.is_contiguous() and sa.is_contiguous() and sb.is_contiguous()):
-        raise RuntimeError("gemm operands must be contiguous")
-    cols = (k + 127) // 128 * 4
-    if sa.numel() != (m + 127) // 128 * 128 * cols or sb.numel() != (n + 127) // 128 * 128 * cols:
-        raise RuntimeError("MXFP4 scale tensors must be the padded swizzled "
-                           "[round_up(rows,128), round_up(k/32,4)] layout")
-    if out is None:
-        _require(not accumulate, "accumulate needs an existing output")
-        _require(out_dtype in (torch.bfloat16, torch.float32), "output dtype must be bf16 or fp32")
-        out = torch.empty((m, n), device=qa.device, dtype=out_dtype)
-    else:
-        _require(out.dtype in (torch.bfloat16, torch.float32) and out.get_device() == dev,
-                 "output must be bf16 or fp32 on the operands' device")
-        _require(out.dim() == 2 and out.shape == (m, n) and out.stride(1) == 1,
-                 "output must be [m, n] with unit column stride")
-        _require(not accumulate or out.dtype == torch.float32, "accumulate needs an fp32 output")
-    if bias is not None:
-        _check_bf16(bias, "bias")
-        _require(bias.numel() == n and bias.get_device() == dev, "bias is bf16 [n]")
-        bias = bias.contiguous()
-    if residual is not None:
-        _check_bf16(residual, "residual")
-        _require(out.dtype == torch.bfloat16 and residual.shape == (m, n) and residual.stride() == out.stride(),
-                 "residual must match a bf16 output's layout")
-    if m == 0 or n == 0:
-        return out
-    _run(qa, "nvfp4b200_mx_gemm", qa.data_ptr(), qb.data_ptr(), sa.data_ptr(), sb.data_ptr(), _ptr(bias),
-         _ptr(residual), out.data_ptr(), _DTYPES[out.dtype], int(bool(accumulate)), int(epilogue), m, n, k,
-         out.stride(0))
-    return out
-
-
-class MXOperand:
-    """One orientation of an MXFP4 matrix in one allocation: nibbles [rows, k/2],
-    then swizzled scales.  For callers that hold operands between a forward and
-    a backward; the fewer allocations halve the wrappers' host time there."""
-    __slots__ = ("buf", "rows", "k")
-
-    def __init__(self, rows: int, k: int, like: torch.Tensor, buf: Optional[torch.Tensor] = None):
-        self.rows, self.k = rows, k
-        # k % 32 == 0: the nibbles end on a 16-byte boundary
-        self.buf = like.new_empty(rows * k // 2 + math.prod(mx_scale_shape(rows, k)),
-                                  dtype=torch.uint8) if buf is None else buf
-
-    def pointers(self) -> Tuple[int, int]:
-        p = self.buf.data_ptr()
-        return p, p + self.rows * self.k // 2
-
-
-def mx_operands(x: torch.Tensor, rows: bool, cols: bool) -> Tuple[Optional[MXOperand], Optional[MXOperand]]:
-    """x [R, K] quantized along K (``rows``) and / or, transposed, along R
-    (``cols``), from one read, as ``MXOperand``s."""
-    x = _float_matrix(x)
-    r, c = x.shape
-    if c == 0 or c % 32:
-        raise RuntimeError("K must be divisible by 32 for MXFP4 1x32 scaling.")
-    a = MXOperand(r, c, x) if rows else None
-    b = MXOperand(c, (r + 31) // 32 * 32, x) if cols else None
-    if r:
-        q, s = a.pointers() if rows else (None, None)
-        qt, st = b.pointers() if cols else (None, None)
-        _run(x, "nvfp4b200_mx_quant", x.data_ptr(), _DTYPES[x.dtype], None, None, q, s, qt, st, r, c,
-             max(x.stride(0), c))
-    return a, b
-
-
-def mx_product(a: MXOperand, b: MXOperand, out_dtype: torch.dtype, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """a . b^T + bias of two operands along the same k (bias bf16 [b.rows], checked by the caller)."""
-    if a.k != b.k or a.k == 0 or a.buf.get_device() != b.buf.get_device():
-        raise RuntimeError("the operands must share their contraction length and device")
-    out = a.buf.new_empty((a.rows, b.rows), dtype=out_dtype)
-    if a.rows and b.rows:
-        (qa, sa), (qb, sb) = a.pointers(), b.pointers()
-        _run(out, "nvfp4b200_mx_gemm", qa, qb, sa, sb, _ptr(bias), None, out.data_ptr(), _DTYPES[out_dtype], 0,
-             EPI_NONE, a.rows, b.rows, a.k, b.rows)
-    return out
+    _require(out_dtype in (torch.bfloat16, torch.float32), "output dtype must be bf16 or fp32")
+    return _bind.ext.mx_gemm(qa, sa, qb, sb, bias, residual, out, out_dtype == torch.float32, accumulate, epilogue)
 
 
 def mx_linear(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = x . W^T + bias with W held in MXFP4 (qw [n, k/2], sw; ``mx_quantize``):
     x bf16 [..., k] is quantized along k, y is bf16 [..., n].  n % 8 == 0."""
-    _check_bf16(x, "mx_linear")
-    n, k = qw.shape[0], 2 * qw.shape[1]
-    _require(x.shape[-1] == k, f"K mismatch: x has {x.shape[-1]}, W has {k}")
-    if k == 0 or k % 32 or n % 8:
-        raise RuntimeError("mx_linear needs K divisible by 32 and N by 8")
-    dev = x.get_device()
-    if (qw.get_device() != dev or sw.get_device() != dev or qw.element_size() != 1 or sw.element_size() != 1 or not qw.is_contiguous() or not sw.is_contiguous()
-            or sw.numel() != (n + 127) // 128 * 128 * ((k + 127) // 128 * 4)):
-        raise RuntimeError("the weight is contiguous q [n, k/2] and its padded swizzled scales on x's device")
-    if bias is not None:
-        _check_bf16(bias, "bias")
-        _require(bias.numel() == n and bias.get_device() == dev, "bias is bf16 [n]")
-        bias = bias.contiguous()
-    x2 = _float_matrix(x if x.dim() == 2 else x.reshape(-1, k))
-    m = x2.shape[0]
-    y = torch.empty((*x.shape[:-1], n), device=x.device, dtype=torch.bfloat16)
-    if m and n:
-        # few tokens are quantized inside the product: no workspace
-        fused = m <= 12 and _lib.load().nvfp4b200_mx_linear_fused(m, n, k)
-        held = None if fused else MXOperand(m, k, x2)
-        qx, sx = (None, None) if fused else held.pointers()
-        _run(x2, "nvfp4b200_mx_linear", x2.data_ptr(), qw.data_ptr(), sw.data_ptr(), _ptr(bias), qx, sx,
-             y.data_ptr(), m, n, k, max(x2.stride(0), k))
-    return y
+    return _bind.ext.mx_linear(x, qw, sw, bias)
 
 
 # ----------------------------------------------------------------------------
@@ -514,71 +323,8 @@ def mx_linear(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, bias: Optiona
 # ----------------------------------------------------------------------------
 
 
-def _dense(t: torch.Tensor) -> bool:
-    """Every element once in one stretch of memory, in whatever order of dimensions."""
-    if t.is_contiguous():
-        return True
-    expect = 1
-    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
-        if st != expect:
-            return False
-        expect *= n
-    return True
-
-
-_dtype_of = operator.attrgetter("dtype")
-
-
-def _grad_call(grads, outs, norm_type, grad_scale, max_norm, want):
-    """Run nvfp4b200_grad_norm; ``want`` names the outputs: n(orm), c(oef), t(otal)."""
-    if isinstance(grads, torch.Tensor):
-        grads = (grads,)
-    grads = list(grads)
-    if norm_type != 2 and norm_type != math.inf:
-        raise RuntimeError("norm_type must be 2 or inf")
-    if not max_norm >= 0.0:
-        raise RuntimeError("max_norm must not be negative")
-    dev = grads[0].get_device() if grads else _current_device()
-    count = len(grads)
-    # whole-list passes through map: about a third of the host time of a loop
-    T = torch.Tensor
-    try:
-        dts = array.array("i", map(_DTYPES.__getitem__, map(_dtype_of, grads)))
-    except KeyError:
-        dts = None
-    if dts is None or dev < 0 or set(map(T.get_device, grads)) - {dev}:
-        raise RuntimeError("gradients are bf16, fp16 or fp32 CUDA tensors of one device")
-    contiguous = all(map(T.is_contiguous, grads))
-    if not contiguous and not all(map(_dense, grads)):
-        raise RuntimeError("gradients must be dense: every element once in one stretch of memory")
-    ptrs, lens = array.array("Q", map(T.data_ptr, grads)), array.array("q", map(T.numel, grads))
-    outp = outd = None
-    if outs is grads:
-        outp, outd = ptrs, dts
-    elif outs is not None:
-        outs = [outs] if isinstance(outs, torch.Tensor) else list(outs)
-        try:
-            outd = array.array("i", map(_DTYPES.__getitem__, map(_dtype_of, outs)))
-        except KeyError:
-            outd = None
-        if (outd is None or len(outs) != count or set(map(T.get_device, outs)) - {dev}
-                or array.array("q", map(T.numel, outs)) != lens
-                or not (contiguous and all(map(T.is_contiguous, outs)))
-                and any(o.shape != t.shape or o.stride() != t.stride() for o, t in zip(outs, grads)
-                        if not (o.is_contiguous() and t.is_contiguous()))):
-            raise RuntimeError("out holds one bf16, fp16 or fp32 tensor per gradient, contiguous and of its number "
-                               "of elements, or of its shape and strides")
-        outp = array.array("Q", map(T.data_ptr, outs))
-    device = torch.device("cuda", dev)
-    words = 1024 * (1 + count // 112)
-    ws = torch.empty(words, device=device, dtype=torch.float64)
-    norm = torch.empty(1, device=device, dtype=torch.float32) if "n" in want else None
-    coef = torch.empty(1, device=device, dtype=torch.float32) if "c" in want else None
-    total = torch.empty(1, device=device, dtype=torch.float64) if "t" in want else None
-    addr = lambda a: None if a is None else a.buffer_info()[0]
-    _run(ws, "nvfp4b200_grad_norm", addr(ptrs), addr(dts), addr(outp), addr(outd), addr(lens), count,
-         2 if norm_type == 2 else 0, grad_scale, max_norm, ws.data_ptr(), words, _ptr(norm), _ptr(coef), _ptr(total))
-    return norm, coef, total
+def _listed(grads) -> list:
+    return [grads] if isinstance(grads, torch.Tensor) else grads if isinstance(grads, list) else list(grads)
 
 
 def grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], norm_type: float = 2.0,
@@ -586,7 +332,7 @@ def grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], norm_type: flo
     """Norm of all gradients together (2 or inf), of grad * grad_scale, as a
     1-element fp32 tensor.  The list may mix bf16, fp16 and fp32 and hold empty
     tensors; the sum is carried in fp64 and does not depend on timing."""
-    return _grad_call(grads, None, norm_type, grad_scale, math.inf, "n")[0]
+    return _bind.ext.grad_norm(_listed(grads), None, False, norm_type, grad_scale, math.inf, 1)[0]
 
 
 def grad_norm_coef(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
@@ -594,26 +340,20 @@ def grad_norm_coef(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm:
     """(norm, coef) with coef = min(1, max_norm / (norm + 1e-6)), both 1-element
     fp32 tensors: hand coef to ``adamw_step`` / ``adamw_master_step`` as
     ``clip`` and the gradients are clipped without a pass of their own."""
-    return _grad_call(grads, None, norm_type, grad_scale, max_norm, "nc")[:2]
+    return _bind.ext.grad_norm(_listed(grads), None, False, norm_type, grad_scale, max_norm, 3)[:2]
 
 
 def grad_norm_total(grads: Union[torch.Tensor, Sequence[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
     """The sum of squares (or the largest magnitude) as a 1-element fp64 tensor:
     what a rank holding a shard of the gradients sends to a sum (maximum) over
     the ranks before ``grad_norm_finish``."""
-    return _grad_call(grads, None, norm_type, 1.0, math.inf, "t")[2]
+    return _bind.ext.grad_norm(_listed(grads), None, False, norm_type, 1.0, math.inf, 4)[2]
 
 
 def grad_norm_finish(totals: torch.Tensor, max_norm: float, norm_type: float = 2.0,
                      grad_scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
     """(norm, coef) from one or more ``grad_norm_total`` values."""
-    _require(totals.is_cuda and totals.dtype == torch.float64 and totals.is_contiguous(),
-             "totals are a contiguous float64 CUDA tensor")
-    _require(norm_type == 2 or norm_type == math.inf, "norm_type must be 2 or inf")
-    res = torch.empty(2, device=totals.device, dtype=torch.float32)
-    _run(totals, "nvfp4b200_grad_norm_finish", totals.data_ptr(), totals.numel(), 2 if norm_type == 2 else 0,
-         float(grad_scale), float(max_norm), res.data_ptr(), res.data_ptr() + 4)
-    return res[:1], res[1:]
+    return _bind.ext.grad_norm_finish(totals, norm_type, grad_scale, max_norm)
 
 
 def clip_grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
@@ -628,52 +368,13 @@ def clip_grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm:
     to scale, nothing is written.  Outputs must not overlap one another or
     another gradient.  A NaN gradient makes every output NaN, an infinite norm
     makes them 0 (NaN where the gradient was infinite)."""
-    if isinstance(grads, torch.Tensor):
-        grads = (grads,)
-    grads = list(grads)
-    return _grad_call(grads, grads if out is None else out, norm_type, grad_scale, max_norm, "n")[0]
+    return _bind.ext.grad_norm(_listed(grads), None if out is None else _listed(out), out is None, norm_type, grad_scale,
+                               max_norm, 1)[0]
 
 
 # ----------------------------------------------------------------------------
 # norms after and before a block, with gate and residual scale
 # ----------------------------------------------------------------------------
-
-
-def _rows_of(t: torch.Tensor) -> torch.Tensor:
-    """A [T, D] tensor with unit column stride (rows may be strided), copied otherwise."""
-    if t.is_contiguous() or (t.stride(1) == 1 and t.stride(0) >= t.shape[1]):
-        return t
-    return t.contiguous()
-
-
-def _ld(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1])
-
-
-def _norm_params(x: torch.Tensor, gamma_post, gate, gamma_pre):
-    """Checked contiguous parameters and the number of gate groups."""
-    t, d = x.shape
-    dev, dt = x.get_device(), x.dtype
-    for g in (gamma_post, gamma_pre):
-        if g is not None and (g.numel() != d or g.dtype != dt or g.get_device() != dev):
-            raise RuntimeError("gamma_post and gamma_pre must be [D] of the activations' dtype and device")
-    groups = 0
-    if gate is not None:
-        if gate.dtype != dt or gate.get_device() != dev or gate.shape[-1] != d:
-            raise RuntimeError("gate must be [D] or [G, D] of the activations' dtype and device")
-        groups = gate.numel() // d
-        if groups == 0 or t % groups:
-            raise RuntimeError("the rows must split evenly over the gate's groups")
-        gate = gate.contiguous()
-    return (None if gamma_post is None else gamma_post.contiguous(), gate,
-            None if gamma_pre is None else gamma_pre.contiguous(), groups)
-
-
-def _norm_input(b: torch.Tensor) -> None:
-    if not (b.is_cuda and b.dtype in _DTYPES and b.dim() == 2):
-        raise RuntimeError("the norms expect CUDA bf16, fp16 or fp32 [T, D]")
-    if not 0 < b.shape[1] <= 16384:
-        raise RuntimeError("the norms take 1 to 16384 columns")
 
 
 def sandwich_norm(b: torch.Tensor, x: torch.Tensor, gamma_post: Optional[torch.Tensor] = None,
@@ -690,41 +391,7 @@ def sandwich_norm(b: torch.Tensor, x: torch.Tensor, gamma_post: Optional[torch.T
     taking rows [g T/G, (g+1) T/G).  n is computed when ``gamma_pre`` is given
     or ``pre=True`` (then with weight 1).  Returns (y, n, inv_b, inv_y), the
     last two fp32 [T]; n and inv_y are None without n.  D <= 16384."""
-    _norm_input(b)
-    if x.dtype != b.dtype or x.get_device() != b.get_device() or x.shape != b.shape:
-        raise RuntimeError("b and x must match in shape, dtype and device")
-    gamma_post, gate, gamma_pre, groups = _norm_params(b, gamma_post, gate, gamma_pre)
-    t, d = b.shape
-    b, x = _rows_of(b), _rows_of(x)
-    pre = gamma_pre is not None if pre is None else pre
-    if gamma_pre is not None and not pre:
-        raise RuntimeError("gamma_pre without the norm it belongs to")
-    y = b.new_empty((t, d))
-    inv = torch.empty((2 if pre else 1, t), device=b.device, dtype=torch.float32)
-    n = inv_y = None
-    if pre:
-        n = torch.empty_like(y)
-        inv_b, inv_y = inv.unbind()
-    else:
-        inv_b = inv.view(t)
-    if t:
-        _run(b, "nvfp4b200_sandwich_norm", b.data_ptr(), x.data_ptr(), _ptr(gamma_post), _ptr(gate), _ptr(gamma_pre),
-             y.data_ptr(), _ptr(n), inv_b.data_ptr(), _ptr(inv_y), _DTYPES[b.dtype], t, d, groups, _ld(b), _ld(x),
-             residual_scale, branch_scale, eps)
-    return y, n, inv_b, inv_y
-
-
-@functools.lru_cache(maxsize=1024)
-def _bwd_words(dev: int, t: int, d: int, groups: int) -> int:
-    """fp32 words of workspace of the backward on a device: a function of the sizes alone."""
-    floats = _lib.c_i64(0)
-    args = ("nvfp4b200_sandwich_norm_bwd_ws", t, d, groups, _lib.ctypes.byref(floats))
-    if dev == _current_device():
-        _lib.call(*args)
-    else:
-        with torch.cuda.device(dev):
-            _lib.call(*args)
-    return floats.value
+    return _bind.ext.sandwich_norm(b, x, gamma_post, gate, gamma_pre, residual_scale, branch_scale, eps, pre)
 
 
 def sandwich_norm_bwd(dy: Optional[torch.Tensor], b: torch.Tensor, inv_b: torch.Tensor,
@@ -738,41 +405,9 @@ def sandwich_norm_bwd(dy: Optional[torch.Tensor], b: torch.Tensor, inv_b: torch.
     Returns a dict: dx, db [T, D] in the activations' dtype; dgamma_post [D],
     dgate [G, D], dgamma_pre [D] in fp32 (None without dn, and dgate without a
     gate).  Column sums are added up in a fixed order."""
-    if dy is None and dn is None:
-        raise RuntimeError("sandwich_norm_bwd needs dy or dn")
-    _norm_input(b)
-    if (dn is None) != (y is None) or (dn is None) != (inv_y is None):
-        raise RuntimeError("dn comes with y and inv_y")
-    if dn is None and gamma_pre is not None:
-        raise RuntimeError("gamma_pre without the norm it belongs to")
-    dt, dev, shape = b.dtype, b.get_device(), b.shape
-    for g in (dy, dn, y):
-        if g is not None and (g.dtype != dt or g.get_device() != dev or g.shape != shape):
-            raise RuntimeError("dy, dn and y must match b in shape, dtype and device")
-    t, d = shape
-    for g in (inv_b, inv_y):
-        if g is not None and (g.dtype != torch.float32 or g.numel() != t or g.get_device() != dev
-                              or not g.is_contiguous()):
-            raise RuntimeError("inv_b and inv_y are contiguous float32 [T]")
-    gamma_post, gate, gamma_pre, groups = _norm_params(b, gamma_post, gate, gamma_pre)
-    b = _rows_of(b)
-    dy, dn, y = [None if g is None else _rows_of(g) for g in (dy, dn, y)]
-    dx, db = b.new_empty((t, d)), b.new_empty((t, d))
-    # the parameters' gradients: dgamma_post, dgamma_pre (with dn), dgate
-    par = torch.empty((groups + 1 + (dn is not None), d), device=b.device, dtype=torch.float32)
-    dpost, dpre = par[0], (par[1] if dn is not None else None)
-    dgate = par[-groups:] if groups else None
-    if t == 0:
-        par.zero_()
-    else:
-        floats = _bwd_words(dev, t, d, groups)
-        ws = torch.empty(floats, device=b.device, dtype=torch.float32)
-        ld = lambda g: 0 if g is None else _ld(g)
-        _run(b, "nvfp4b200_sandwich_norm_bwd", _ptr(dy), _ptr(dn), b.data_ptr(), _ptr(y), inv_b.data_ptr(),
-             _ptr(inv_y), _ptr(gamma_post), _ptr(gate), _ptr(gamma_pre), dx.data_ptr(), db.data_ptr(),
-             dpost.data_ptr(), _ptr(dgate), _ptr(dpre), ws.data_ptr(), floats, _DTYPES[dt], t, d, groups, ld(dy),
-             ld(dn), _ld(b), ld(y), residual_scale, branch_scale)
-    return {"dx": dx, "db": db, "dgamma_post": dpost, "dgate": dgate, "dgamma_pre": dpre}
+    dx, db, dgamma_post, dgate, dgamma_pre = _bind.ext.sandwich_norm_bwd(
+        dy, b, inv_b, gamma_post, gate, dn, y, inv_y, gamma_pre, residual_scale, branch_scale)
+    return {"dx": dx, "db": db, "dgamma_post": dgamma_post, "dgate": dgate, "dgamma_pre": dgamma_pre}
 
 
 # ----------------------------------------------------------------------------

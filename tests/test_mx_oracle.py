@@ -163,3 +163,16 @@ def _bwd(L, dy=FAKE, dn=None, b=FAKE, y=None, ib=FAKE, iy=None, gate=None, gn=No
 ])
 def test_c_entry_points_refuse(pkg, call, expected):
     assert call(pkg._lib.load()) == expected
+
+
+def test_torch_binding_shares_the_cpp_runtime(pkg):
+    """libtorch throws and formats through the shared libstdc++; a binding with a copy
+    of its own crashes when a refusal's message is put together."""
+    with open(pkg._build.BINDING_PATH, "rb") as f:
+        assert b"libstdc++.so.6" in f.read()
+
+
+def test_torch_binding_fails_loudly_when_missing(pkg, monkeypatch, tmp_path):
+    monkeypatch.setattr(pkg._build, "BINDING_PATH", str(tmp_path / "missing.so"))
+    with pytest.raises(pkg.NVFP4Error):
+        pkg._bind.load()
