@@ -2,7 +2,7 @@
 // of arguments, allocation and the current stream, in C++ because a call's
 // host time is what its smallest users wait for (a decoded token, a small
 // layer): sandwich_norm 20 us through ctypes and the Python allocator calls,
-// NNN us here.  ops.py documents every function; the work is the C ABI's.
+// 9 us here.  ops.py documents every function; the work is the C ABI's.
 #include <torch/extension.h>
 
 #include <c10/cuda/CUDAGuard.h>
@@ -305,6 +305,51 @@ std::tuple<OptTensor, OptTensor> linear_backward(const Tensor& dy_, const OptTen
   return {dx, dw};
 }
 
+// The differentiable layer.  Quantization counts as the identity in the
+// backward; both orientations of an operand come from one read of it, and what
+// the backward needs of x and w is kept in MXFP4 (17/32 byte per element).  In
+// C++ so that the backward needs neither Python nor its lock (a training step
+// of 777 tokens through 1024 x 2048: 95 us with a Python function, 84 so).
+struct MXLinear : public torch::autograd::Function<MXLinear> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias,
+                        bool need_x, bool need_w) {
+    auto [y, xt, wt] = linear_forward(x, w, bias, need_x, need_w);
+    ctx->save_for_backward({xt.value_or(Tensor()), wt.value_or(Tensor())});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["n"] = w.size(0);
+    ctx->saved_data["w"] = (int64_t)w.scalar_type();
+    ctx->saved_data["b"] = bias ? (int64_t)bias->scalar_type() : (int64_t)-1;
+    ctx->saved_data["need"] = (int64_t)(need_x + 2 * need_w);
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    // its gradients are no functions that autograd could differentiate
+    TORCH_CHECK(!at::GradMode::is_enabled(), "mxfp4_linear has no second derivative (create_graph=True)");
+    const auto saved = ctx->get_saved_variables();
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    const int64_t n = ctx->saved_data["n"].toInt(), need = ctx->saved_data["need"].toInt(), b = ctx->saved_data["b"].toInt();
+    const auto wtype = (at::ScalarType)ctx->saved_data["w"].toInt();
+    const Tensor& dy = grads[0];
+    auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    torch::autograd::variable_list out(5);
+    if (!dy.defined()) return out;
+    if (need) {
+      auto [dx, dw] = linear_backward(dy, opt(saved[0]), opt(saved[1]), shape, n, need & 1, need & 2, wtype == at::kFloat);
+      if (dx) out[0] = *dx;
+      if (dw) out[1] = dw->scalar_type() == wtype ? *dw : dw->to(wtype);
+    }
+    if (b >= 0 && ctx->needs_input_grad(2))
+      out[2] = dy.reshape({-1, n}).sum(at::IntArrayRef{0}, false, at::kFloat).to((at::ScalarType)b);
+    return out;
+  }
+};
+
+Tensor mxfp4_linear(const Tensor& x, const Tensor& w, const OptTensor& bias) {
+  const bool grad = at::GradMode::is_enabled();
+  return MXLinear::apply(x, w, bias, grad && x.requires_grad(), grad && w.requires_grad());
+}
+
 // ---- gradient norm and clipping ---------------------------------------------
 
 // which: bit 0 the norm, 1 the coefficient, 2 the fp64 total.  `outs`: the
@@ -496,8 +541,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mx_dequantize", &mx_dequantize);
   m.def("mx_gemm", &mx_gemm);
   m.def("mx_linear", &mx_linear);
-  m.def("linear_forward", &linear_forward);
-  m.def("linear_backward", &linear_backward);
+  m.def("mxfp4_linear", &mxfp4_linear);
   m.def("grad_norm", &grad_norm);
   m.def("grad_norm_finish", &grad_norm_finish);
   m.def("sandwich_norm", &sandwich_norm);

@@ -398,40 +398,16 @@ def mxfp4mm(A: torch.Tensor, B: torch.Tensor, *, out_dtype: torch.dtype = torch.
     return ops.mx_gemm(qa, sa, qb, sb, out_dtype=out_dtype).reshape(*batch, B.shape[0])
 
 
-class MXFP4LinearFunction(torch.autograd.Function):
-    """X @ W^T + bias with MXFP4 operands in forward, dgrad and wgrad, each
-    quantized along its product's contraction dimension; quantization counts
-    as the identity in the backward.  Both orientations of an operand come from
-    one read of it, and what the backward needs of X and W is kept in MXFP4
-    (17/32 byte per element)."""
-
-    @staticmethod
-    def forward(ctx, input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
-        y, xt, wt = _bind.ext.linear_forward(input, weight, bias, *ctx.needs_input_grad[:2])
-        ctx.save_for_backward(xt, wt)
-        ctx.shape, ctx.n, ctx.wdtype = input.shape, weight.shape[0], weight.dtype
-        ctx.bdtype = None if bias is None else bias.dtype
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_output: torch.Tensor):
-        xt, wt = ctx.saved_tensors
-        need_x, need_w = ctx.needs_input_grad[:2]
-        dx = dw = db = None
-        if need_x or need_w:
-            dx, dw = _bind.ext.linear_backward(grad_output, xt, wt, ctx.shape, ctx.n, need_x, need_w,
-                                               ctx.wdtype == torch.float32)
-            if dw is not None and dw.dtype != ctx.wdtype:
-                dw = dw.to(ctx.wdtype)
-        if ctx.bdtype is not None and ctx.needs_input_grad[2]:
-            db = grad_output.reshape(-1, ctx.n).sum(dim=0, dtype=torch.float32).to(ctx.bdtype)
-        return dx, dw, db
-
-
 def mxfp4_linear(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """input [..., K] @ weight [N, K]^T + bias with MXFP4 products, differentiable in all three."""
-    return MXFP4LinearFunction.apply(input, weight, bias)
+    """input [..., K] @ weight [N, K]^T + bias with MXFP4 products, differentiable in all three.
+
+    Input bf16 or fp32 (the result's type), weight bf16, fp16 or fp32.  Forward,
+    dgrad and wgrad quantize each operand along the product's contraction
+    dimension, which takes K % 32 == 0 and, for gradients, N % 32 == 0 (else
+    N % 8 == 0); tokens count as filled up with zeros.  Quantization is the
+    identity in the backward, which keeps x and the weight in MXFP4 only; there
+    is no second derivative."""
+    return _bind.ext.mxfp4_linear(input, weight, bias)
 
 
 class MXFP4Linear(NVFP4Linear):
@@ -476,5 +452,4 @@ __all__ = ["round_up", "require", "FP4_DTYPE", "FP8_SCALE_DTYPE", "quant_nvfp4_f
            "rmsnorm_quant_nvfp4_fused", "nvfp4mm_torch", "nvfp4mm", "nvfp4mm_relu", "nvfp4mm_relu_2",
            "test_accuracy", "_bytes_nvfp4_quant_fused", "bench_quant_gbps", "bench_gemm_tflops",
            "NVFP4LinearFunction", "NVFP4Linear", "cutlass_nvfp4_mm", "cutlass_nvfp4_mm_relu",
-           "cutlass_nvfp4_mm_relu_2", "MX_SCALE_DTYPE", "quant_mxfp4_fused", "mxfp4mm", "MXFP4LinearFunction",
-           "mxfp4_linear", "MXFP4Linear"]
+           "cutlass_nvfp4_mm_relu_2", "MX_SCALE_DTYPE", "quant_mxfp4_fused", "mxfp4mm", "mxfp4_linear", "MXFP4Linear"]

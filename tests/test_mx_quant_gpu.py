@@ -272,6 +272,33 @@ def test_linear_module(pkg, f4):
         lin(xg)
 
 
+def test_no_second_derivative(pkg, f4):
+    x = make(32, 64, torch.bfloat16, 1).requires_grad_()
+    w = make(32, 64, torch.bfloat16, 2).requires_grad_()
+    y = f4.mxfp4_linear(x, w)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+    with torch.no_grad():
+        assert not f4.mxfp4_linear(x, w).requires_grad
+
+
+def test_backward_twice_and_saved_tensor_hooks(pkg, f4):
+    """retain_graph, and hooks that move what is kept (offloading): the same bits."""
+    x = make(40, 64, torch.bfloat16, 1).requires_grad_()
+    w = make(32, 64, torch.bfloat16, 2).requires_grad_()
+    dy = make(40, 32, torch.bfloat16, 3)
+    y = f4.mxfp4_linear(x, w)
+    first = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    again = torch.autograd.grad(y, (x, w), dy)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+        z = f4.mxfp4_linear(x, w)
+    moved = torch.autograd.grad(z, (x, w), dy)
+    for a, b, c in zip(first, again, moved):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, (x, w), dy)     # freed
+
+
 def test_gemm_forms(pkg):
     """fp32 store and accumulate, residual, ReLU epilogue, strided output."""
     ops = pkg.ops
