@@ -70,25 +70,29 @@ __device__ __forceinline__ uint32_t absmax8(const float (&f)[8]) {
   return m;
 }
 
+// Elements before the first 16-byte boundary at or after p (at most n).
+template <typename T>
+__device__ __forceinline__ int head_of(const T* p, int n) {
+  return min(n, (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / (int)sizeof(T));
+}
+
 template <int DT, bool INF>
 __device__ __forceinline__ void reduce_chunk(const void* base, int64_t lo, int64_t hi, double& sum, uint32_t& top) {
   using E = Elem<DT>;
   const typename E::Raw* p = static_cast<const typename E::Raw*>(base) + lo;
-  const int n = (int)(hi - lo);
+  const int n = (int)(hi - lo), head = head_of(p, n), nv = (n - head) >> 3;
   float f[8];
-  int done = 0;
-  if ((reinterpret_cast<uintptr_t>(base) & 15) == 0) {
-    const int nv = n >> 3;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < nv; i += THREADS) {
-      E::unpack(E::load(p + 8 * i), f);
-      if (INF) top = max(top, absmax8(f)); else sum += sumsq8(f);
-    }
-    done = nv << 3;
+  for (int i = threadIdx.x; i < nv; i += THREADS) {
+    E::unpack(E::load(p + head + 8 * i), f);
+    if (INF) top = max(top, absmax8(f)); else sum += sumsq8(f);
   }
-  for (int i = done + threadIdx.x; i < n; i += 8 * THREADS) {
+  // up to 7 elements before the first vector and 7 after the last
+  const int rest = n - 8 * nv, t = threadIdx.x;
+  if (t < rest) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = i + j * THREADS < n ? E::get(p + i + j * THREADS) : 0.0f;
+    for (int j = 1; j < 8; ++j) f[j] = 0.0f;
+    f[0] = E::get(p + (t < head ? t : 8 * nv + t));
     if (INF) top = max(top, absmax8(f)); else sum += sumsq8(f);
   }
 }
@@ -165,16 +169,25 @@ __device__ __forceinline__ float clip_factor(const Norm& a, bool writer) {
 
 __global__ void __launch_bounds__(THREADS) finish_kernel(const Norm a) { clip_factor(a, threadIdx.x == 0); }
 
+// One chunk, read and written in 16-byte vectors whatever the two tensors'
+// alignment (a bucket's views start anywhere): vectors of 8 elements are read
+// on the source's boundaries, and where the destination's boundaries fall e
+// elements later, each output vector takes its last e elements from the next
+// lane's.  A few elements at the chunk's ends go one by one.
 template <int SD, int DD>
 __device__ __forceinline__ void scale_chunk(const void* src, void* dst, int64_t lo, int64_t hi, float k) {
   using S = Elem<SD>;
   using D = Elem<DD>;
   const typename S::Raw* p = static_cast<const typename S::Raw*>(src) + lo;
   typename D::Raw* o = static_cast<typename D::Raw*>(dst) + lo;
-  const int n = (int)(hi - lo);
-  int done = 0;
-  if (((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) & 15) == 0) {
-    const int nv = n >> 3;
+  const int n = (int)(hi - lo), head = head_of(p, n), e = head_of(o + head, n - head);
+  // whole vectors of the source, and of the destination (an output vector between
+  // the source's boundaries needs two whole ones)
+  const int nv = (n - head) >> 3, ov = e == 0 ? nv : max(0, nv - 1);
+  p += head;
+  o += head + e;
+  const int lane = threadIdx.x & 31;
+  if (e == 0) {
 #pragma unroll 4
     for (int i = threadIdx.x; i < nv; i += THREADS) {
       float f[8];
@@ -183,13 +196,63 @@ __device__ __forceinline__ void scale_chunk(const void* src, void* dst, int64_t 
       for (int j = 0; j < 8; ++j) f[j] *= k;
       D::store(o + 8 * i, D::pack(f));
     }
-    done = nv << 3;
+  } else {
+#pragma unroll 1
+    for (int i0 = threadIdx.x - lane; i0 < ov; i0 += THREADS) {   // a warp's 32 output vectors
+      const int i = i0 + lane;
+      float f[8], t[8];
+      const auto own_src = i < nv ? S::load(p + 8 * i) : S::zero();
+      const auto next_src = lane == 31 && i + 1 < nv ? S::load(p + 8 * i + 8) : S::zero();
+      S::unpack(own_src, f);
+      S::unpack(next_src, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= k;
+      if constexpr (DD != NVFP4B200_F32) {
+        // 16-bit results are shifted packed: two conditional word shifts, then a half-word
+        const auto own = D::pack(f);
+        uint32_t x[8] = {own.a.x, own.a.y, own.a.z, own.a.w, 0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[4 + j] = __shfl_down_sync(0xffffffffu, x[j], 1);
+        if (lane == 31) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) t[j] *= k;
+          const auto next = D::pack(t);
+          x[4] = next.a.x; x[5] = next.a.y; x[6] = next.a.z; x[7] = next.a.w;
+        }
+#pragma unroll
+        for (int j = 0; j < 6; ++j) x[j] = (e & 4) ? x[j + 2] : x[j];
+#pragma unroll
+        for (int j = 0; j < 5; ++j) x[j] = (e & 2) ? x[j + 1] : x[j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __funnelshift_r(x[j], x[j + 1], 16 * (e & 1));
+        if (i < ov) *reinterpret_cast<uint4*>(o + 8 * i) = make_uint4(x[0], x[1], x[2], x[3]);
+      } else {   // e < 4
+        float x[11];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = f[j];
+#pragma unroll
+        for (int j = 0; j < 3; ++j) x[8 + j] = __shfl_down_sync(0xffffffffu, f[j], 1);
+        if (lane == 31) {
+#pragma unroll
+          for (int j = 0; j < 3; ++j) x[8 + j] = t[j] * k;
+        }
+#pragma unroll
+        for (int j = 0; j < 9; ++j) x[j] = (e & 2) ? x[j + 2] : x[j];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = (e & 1) ? x[j + 1] : x[j];
+        if (i < ov) D::store(o + 8 * i, D::pack(f));
+      }
+    }
   }
-#pragma unroll 4
-  for (int i = done + threadIdx.x; i < n; i += THREADS) o[i] = D::bits(S::get(p + i) * k);
+  // the elements before and after the output vectors: at most 7 + 7 and 15
+  const int before = head + e, rest = n - 8 * ov, t = threadIdx.x;
+  if (t < rest) {
+    const int j = t < before ? t - before : 8 * ov + t - before;   // relative to o
+    o[j] = D::bits(S::get(p + e + j) * k);
+  }
 }
 
-__global__ void __launch_bounds__(THREADS) scale_kernel(const __grid_constant__ Table t, const Norm a, int first) {
+__global__ void __launch_bounds__(THREADS, 5) scale_kernel(const __grid_constant__ Table t, const Norm a, int first) {
   const float k = clip_factor(a, first && blockIdx.x == 0 && threadIdx.x == 0);
   for (int j = blockIdx.x; j < t.chunks; j += gridDim.x) {
     const int c = t.chunks - 1 - j;

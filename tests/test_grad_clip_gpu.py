@@ -114,6 +114,24 @@ def test_misaligned_views_and_layouts(pkg):
     assert torch.equal(flat[~inside], rest[~inside])
 
 
+@pytest.mark.parametrize("src", [BF, HF, FL])
+@pytest.mark.parametrize("dst", [BF, HF, FL])
+def test_every_alignment(pkg, src, dst):
+    """Views at every offset within 16 bytes on either side, short and past a chunk's
+    length: each value right, nothing written beside them."""
+    for n in (1, 6, 7, 8, 9, 23, 300, 12345):
+        a, b = tensors([n + 9], [src], n)[0], torch.full((n + 18,), 7.0, device="cuda", dtype=dst)
+        for i in range(0, 9, 1 if n < 400 else 3):
+            for j in range(9):
+                b.fill_(7.0)
+                g, o = a[i:i + n], b[j + 1:j + 1 + n]
+                norm = pkg.ops.clip_grad_norm([g], 0.01, out=[o])
+                ref = ref_norm([g])
+                assert abs(norm.item() - ref) <= REL * ref
+                check_scaled([o], [g], min(1.0, 0.01 / (ref + 1e-6)))
+                assert (b[:j + 1] == 7).all() and (b[j + 1 + n:] == 7).all()
+
+
 @pytest.mark.parametrize("scale", [1e-38, 1e-30, 1e-22, 1e18, 1e30, 3e38])
 def test_extreme_magnitudes(pkg, scale):
     """Squares that fp32 cannot hold, alone and beside ordinary ones."""
