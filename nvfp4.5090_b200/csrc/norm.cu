@@ -373,6 +373,7 @@ struct BwdArgs {
   int d;
   float alpha, s;
   int stages;               // staged kernel: rows of the ring
+  int64_t safe_rows;        // staged kernel, unaligned rows: those whose 16-byte windows lie inside every tensor
   int ws16;                 // part and part_gate are 16-byte aligned
 };
 
@@ -520,7 +521,12 @@ __device__ int g_norm_error = 0;
 constexpr int BWD_STAGES = 3;   // rows of the ring, at most
 
 // One 8-element vector per thread: TPR threads cover d <= 8 * TPR columns.
-template <int DT, int TPR, bool PRE>
+// ODD: rows that do not start on 16-byte boundaries (widths that are no
+// multiple of 8, say).  The bulk copies take each row's window of whole
+// 16-byte pieces, a thread's eight columns are TPR apart and are read and
+// written one by one; the last rows, whose windows could reach past the tensor,
+// are read straight from global memory.
+template <int DT, int TPR, bool PRE, bool ODD>
 __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1024 / TPR)
     sandwich_bwd_staged_kernel(const BwdArgs a, int64_t parts_per_group) {
   using E = Elem<DT>;
@@ -536,21 +542,32 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
   const int t = threadIdx.x;
   const float inv_d = 1.0f / (float)a.d;
   const int row_bytes = a.d * (int)sizeof(Raw);
+  const int slot = ODD ? ((row_bytes + 15) & ~15) + 16 : row_bytes;   // of one tensor's row in the ring
   const int64_t g = blockIdx.x / parts_per_group, p = blockIdx.x % parts_per_group;
   const int64_t r0 = g * a.rows_per_gate + p * a.rows_per_cta;
   const int rows = (int)(imin64(r0 + a.rows_per_cta, (g + 1) * a.rows_per_gate) - r0);
 
+  const int staged = (int)imin64(rows, ODD ? (a.safe_rows > r0 ? a.safe_rows - r0 : 0) : rows);
+  auto skew = [&](int64_t r, int64_t ld) { return ODD ? (int)((uint64_t)(r * ld) * sizeof(Raw) & 15) : 0; };
+
   auto fetch = [&](int i, int stage) {   // one thread: row r0 + i into a stage
-    if (i >= rows) return;
-    uint8_t* dst = row_ring + (size_t)stage * NT * row_bytes;
-    bulk::expect(&full[stage], (uint32_t)((NT - (a.dy ? 0 : 1)) * row_bytes));
+    if (i >= staged) return;
+    uint8_t* dst = row_ring + (size_t)stage * NT * slot;
     const int64_t r = r0 + i;
-    if (a.dy) bulk::copy(dst, static_cast<const Raw*>(a.dy) + r * a.ld_dy, row_bytes, &full[stage]);
-    bulk::copy(dst + row_bytes, static_cast<const Raw*>(a.b) + r * a.ldb, row_bytes, &full[stage]);
-    if (PRE) {
-      bulk::copy(dst + 2 * row_bytes, static_cast<const Raw*>(a.dn) + r * a.ld_dn, row_bytes, &full[stage]);
-      bulk::copy(dst + 3 * row_bytes, static_cast<const Raw*>(a.y) + r * a.ldy, row_bytes, &full[stage]);
-    }
+    const void* base[4] = {a.dy, a.b, a.dn, a.y};
+    const int64_t ld[4] = {a.ld_dy, a.ldb, a.ld_dn, a.ldy};
+    uint32_t total = 0;
+#pragma unroll
+    for (int q = 0; q < NT; ++q)
+      if (base[q]) total += (uint32_t)(ODD ? (skew(r, ld[q]) + row_bytes + 15) & ~15 : row_bytes);
+    bulk::expect(&full[stage], total);
+#pragma unroll
+    for (int q = 0; q < NT; ++q)
+      if (base[q]) {
+        const int off = skew(r, ld[q]);
+        bulk::copy(dst + q * slot, static_cast<const uint8_t*>(base[q]) + r * ld[q] * (int64_t)sizeof(Raw) - off,
+                   (uint32_t)(ODD ? (off + row_bytes + 15) & ~15 : row_bytes), &full[stage]);
+      }
   };
   if (t < 3 * 4 * W4 * 2) (&red[0][0][0])[t] = 0.0f;   // warp parts past the last stay zero
   if (t == 0) {
@@ -562,14 +579,19 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
     for (int st = 0; st < ST; ++st) fetch(st, st);
 
   // column sums, each thread's own: S (2 float4) and dgamma_pre's (2 more)
-  ulonglong2* sums_at = reinterpret_cast<ulonglong2*>(row_ring + (size_t)ST * NT * row_bytes) + t;
+  ulonglong2* sums_at = reinterpret_cast<ulonglong2*>(row_ring + (size_t)ST * NT * slot) + t;
 #pragma unroll
   for (int j = 0; j < (PRE ? 4 : 2); ++j) sums_at[j * TPR] = make_ulonglong2(0ull, 0ull);
-  const int c = 8 * t;
+  const int c = ODD ? t : 8 * t;   // the thread's first column; the others follow, or (ODD) are TPR apart
   const bool in = c < a.d;
   auto weights = [&](const void* p, int64_t off, uint64_t (&w)[NP]) {
     float f[8];
-    E::unpack(in ? E::load(static_cast<const Raw*>(p) + off + c) : E::zero(), f);
+    if (ODD) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = c + j * TPR < a.d ? E::get(static_cast<const Raw*>(p) + off + c + j * TPR) : 0.0f;
+    } else {
+      E::unpack(in ? E::load(static_cast<const Raw*>(p) + off + c) : E::zero(), f);
+    }
 #pragma unroll
     for (int j = 0; j < NP; ++j) w[j] = f2mul(w[j], f2pack(f[2 * j], f[2 * j + 1]));
   };
@@ -595,10 +617,22 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
       next_b = __ldg(ib + i + 1);
       if (PRE) next_y = __ldg(iy + i + 1);
     }
-    if (!bulk::wait(&full[stage], parity)) gave_up = 1;
-    const uint8_t* src = row_ring + (size_t)stage * NT * row_bytes;
+    if (i < staged && !bulk::wait(&full[stage], parity)) gave_up = 1;
+    const uint8_t* src = row_ring + (size_t)stage * NT * slot;
     auto get = [&](int tensor, int c, uint64_t (&o)[4]) {
-      Pairs<DT>::get(reinterpret_cast<const uint4*>(src + tensor * row_bytes + c * (int)sizeof(Raw)), 1, o);
+      if (!ODD) {
+        Pairs<DT>::get(reinterpret_cast<const uint4*>(src + tensor * slot + c * (int)sizeof(Raw)), 1, o);
+        return;
+      }
+      const void* base = tensor == 0 ? a.dy : tensor == 1 ? a.b : tensor == 2 ? a.dn : a.y;
+      const int64_t at = (r0 + i) * (tensor == 0 ? a.ld_dy : tensor == 1 ? a.ldb : tensor == 2 ? a.ld_dn : a.ldy);
+      const Raw* row = i < staged ? reinterpret_cast<const Raw*>(src + tensor * slot + (int)((uint64_t)at * sizeof(Raw) & 15))
+                                  : static_cast<const Raw*>(base) + at;
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = c + j * TPR < a.d ? E::value(row[c + j * TPR]) : 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = f2pack(f[2 * j], f[2 * j + 1]);
     };
     uint64_t t0[NP], yh[PRE ? NP : 1], bh[NP];
     uint64_t A = 0ull, B = 0ull, C = 0ull;
@@ -679,7 +713,14 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
     }
     sums_at[0] = make_ulonglong2(S[0], S[1]);
     sums_at[TPR] = make_ulonglong2(S[2], S[3]);
-    if (in) {
+    if (ODD) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j * TPR < a.d) {
+          dx[c + j * TPR] = E::bits(dxv[j]);
+          db[c + j * TPR] = E::bits(dbv[j]);
+        }
+    } else if (in) {
       E::store(dx + c, E::pack(dxv));
       E::store(db + c, E::pack(dbv));
     }
@@ -702,7 +743,15 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
 #pragma unroll
   for (int j = 0; j < NP; ++j) gate[j] = f2two(1.0f);
   if (a.gate) weights(a.gate, g * a.d, gate);
-  auto put = [&](float* out, uint64_t lo, uint64_t hi) {   // d % 8 == 0: 16-byte aligned where the workspace is
+  auto put = [&](float* row, int h, uint64_t lo, uint64_t hi) {   // the thread's columns 4 h .. 4 h + 3
+    if (ODD) {
+      const float f[4] = {f2lo(lo), f2hi(lo), f2lo(hi), f2hi(hi)};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + (4 * h + j) * TPR < a.d) row[c + (4 * h + j) * TPR] = f[j];
+      return;
+    }
+    float* out = row + c + 4 * h;   // d % 8 == 0: 16-byte aligned where the workspace is
     if (a.ws16) {
       *reinterpret_cast<ulonglong2*>(out) = make_ulonglong2(lo, hi);
     } else {
@@ -713,11 +762,11 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
   for (int h = 0; h < 2; ++h) {
     const ulonglong2 sv = sums_at[h * TPR];
     const uint64_t lo = f2mul(sv.x, f2two(a.s)), hi = f2mul(sv.y, f2two(a.s));
-    if (a.gate) put(a.part_gate + (int64_t)blockIdx.x * a.d + c + 4 * h, lo, hi);
-    put(a.part + (int64_t)blockIdx.x * a.d + c + 4 * h, f2mul(lo, gate[2 * h]), f2mul(hi, gate[2 * h + 1]));
+    if (a.gate) put(a.part_gate + (int64_t)blockIdx.x * a.d, h, lo, hi);
+    put(a.part + (int64_t)blockIdx.x * a.d, h, f2mul(lo, gate[2 * h]), f2mul(hi, gate[2 * h + 1]));
     if (PRE) {
       const ulonglong2 pv = sums_at[(2 + h) * TPR];
-      put(a.part + ((int64_t)gridDim.x + blockIdx.x) * a.d + c + 4 * h, pv.x, pv.y);
+      put(a.part + ((int64_t)gridDim.x + blockIdx.x) * a.d, h, pv.x, pv.y);
     }
   }
 }
@@ -930,7 +979,7 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
   nvfp4b200_sandwich_norm_bwd_ws(rows, d, groups, &need);
   if (ws_floats < need) return NVFP4B200_ERR_BAD_SHAPE;
   norm::BwdArgs a{dy, dn, b, y, gamma_post, gate, gamma_pre, inv_b, inv_y, dx, db, ws, ws + 2 * sp.ctas * d, dgate, rows, ldb,
-                  ld_dy, ld_dn, ldy, rows / g, sp.rows_per_cta, (int)d, residual_scale, branch_scale, 0,
+                  ld_dy, ld_dn, ldy, rows / g, sp.rows_per_cta, (int)d, residual_scale, branch_scale, 0, 0,
                   aligned(ws, 16)};
   const bool vec = (d * bytes) % 16 == 0 && d % 8 == 0 && vec_ok(dy, ld_dy, bytes) && vec_ok(dn, ld_dn, bytes) &&
                    vec_ok(b, ldb, bytes) && vec_ok(y, ldy, bytes) && vec_ok(gamma_post, d, bytes) &&
@@ -942,17 +991,23 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
       constexpr int T = decltype(tpr)::value, DT = decltype(dt)::value;
       // the staged kernel where a row fits and a CTA's rows have one gate:
       // 346 -> 152 us at 16000 x 4096 bf16 with 8 gates and the next norm
-      if constexpr (decltype(v)::value && T <= 512) {
+      if constexpr (T <= 512) {
         constexpr int T2 = 2 * T;
+        constexpr bool ODD = !decltype(v)::value;
         // two CTAs' worth of threads share an SM (fewer where one is that large), and
         // so its memory: as many ring rows as fit, up to 3 (2 with the next norm's
         // tensors); one row at least, alone on the SM if need be
-        const int row = (dn ? 4 : 2) * (int)d * norm::dtype_size<DT>(), sums = (dn ? 4 : 2) * 16 * T2;
+        const int width = (int)d * bytes, row = (dn ? 4 : 2) * (ODD ? (int)round_up(width, 16) + 16 : width);
+        const int sums = (dn ? 4 : 2) * 16 * T2;
         const int share = norm::MAX_SMEM / std::max(1, 1024 / T2);
         a.stages = std::max(std::min(dn ? 2 : norm::BWD_STAGES, (share - sums) / row), 1);
         const int smem = a.stages * row + sums;
-        if (smem <= norm::MAX_SMEM && (!gate || sp.parts_per_group > 1)) {
-          auto* fn = dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true> : norm::sandwich_bwd_staged_kernel<DT, T2, false>;
+        const int64_t ld_min = std::min(std::min(dy ? ld_dy : ldb, ldb), dn ? std::min(ld_dn, ldy) : ldb);
+        a.safe_rows = std::max<int64_t>(0, rows - 1 - 15 / (ld_min * bytes));
+        const bool bases = aligned(b, 16) && (!dy || aligned(dy, 16)) && (!dn || (aligned(dn, 16) && aligned(y, 16)));
+        if (smem <= norm::MAX_SMEM && (!gate || sp.parts_per_group > 1) && (!ODD || bases)) {
+          auto* fn = dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true, ODD>
+                        : norm::sandwich_bwd_staged_kernel<DT, T2, false, ODD>;
           if (smem > 32 * 1024 &&   // with the static arrays, past the default limit
               cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
             return (int)NVFP4B200_ERR_CUDA;
