@@ -163,6 +163,9 @@ __device__ __forceinline__ float f2sum(uint64_t v) { return f2lo(v) + f2hi(v); }
 
 constexpr int STAGES = 3;
 
+// Set when a bounded wait for a copy gave up.
+__device__ int g_norm_error = 0;
+
 struct FwdArgs {
   const void *b, *x, *gamma_post, *gate, *gamma_pre;
   void *y, *n;
@@ -171,6 +174,9 @@ struct FwdArgs {
   int d;
   float alpha, s, eps;
   int pre;
+  int stages;               // unaligned rows: rows of the ring
+  int64_t safe_rows;        // those whose 16-byte windows lie inside both tensors
+  int64_t rows_per_cta;
 };
 
 template <int DT, bool VEC, int TPR>
@@ -362,6 +368,113 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, DT == NVFP4B200_F32 ? (
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
+// The forward for rows that do not start on 16-byte boundaries: one thread
+// copies each row's window of whole 16-byte pieces of b and x into a ring, as
+// in the backward below; a thread's eight columns are TPR apart and are read
+// and written one by one.  The last rows, whose windows could reach past the
+// tensors, are read straight from global memory.
+template <int DT, int TPR>
+__global__ void __launch_bounds__(TPR, 1024 / TPR) sandwich_fwd_odd_kernel(const FwdArgs a) {
+  using E = Elem<DT>;
+  using Raw = typename E::Raw;
+  extern __shared__ __align__(16) uint8_t odd_ring[];   // [stages][2][slot]
+  __shared__ float red[4][TPR / 32];
+  __shared__ __align__(8) uint64_t full[STAGES];
+  __shared__ int gave_up;
+  const int t = threadIdx.x;
+  const float inv_d = 1.0f / (float)a.d;
+  const int row_bytes = a.d * (int)sizeof(Raw), slot = ((row_bytes + 15) & ~15) + 16;
+  auto skew = [&](int64_t r, int64_t ld) { return (int)((uint64_t)(r * ld) * sizeof(Raw) & 15); };
+  const int64_t r0 = (int64_t)blockIdx.x * a.rows_per_cta, end = imin64(a.rows, r0 + a.rows_per_cta);
+  const int64_t safe = imin64(end, a.safe_rows);
+  auto fetch = [&](int64_t r, int stage) {   // one thread
+    if (r >= safe) return;
+    uint8_t* dst = odd_ring + (size_t)stage * 2 * slot;
+    const int ob = skew(r, a.ldb), ox = skew(r, a.ldx);
+    const uint32_t nb = (uint32_t)((ob + row_bytes + 15) & ~15), nx = (uint32_t)((ox + row_bytes + 15) & ~15);
+    bulk::expect(&full[stage], nb + nx);
+    bulk::copy(dst, static_cast<const uint8_t*>(a.b) + r * a.ldb * (int64_t)sizeof(Raw) - ob, nb, &full[stage]);
+    bulk::copy(dst + slot, static_cast<const uint8_t*>(a.x) + r * a.ldx * (int64_t)sizeof(Raw) - ox, nx, &full[stage]);
+  };
+  if (t == 0) {
+    gave_up = 0;
+    bulk::init(full, STAGES);
+  }
+  __syncthreads();
+  if (t == 0)
+    for (int st = 0; st < a.stages; ++st) fetch(r0 + st, st);
+  // the weights stay in registers: s * gamma_post * gate of the rows' group, gamma_pre
+  float w[8], wn[8];
+  int64_t group = -1;
+  auto times = [&](const void* p, int64_t off, float (&f)[8]) {   // past the row's end its last element
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] *= E::get(static_cast<const Raw*>(p) + off + min(t + j * TPR, a.d - 1));
+  };
+#pragma unroll
+  for (int j = 0; j < 8; ++j) wn[j] = 1.0f;
+  if (a.gamma_pre) times(a.gamma_pre, 0, wn);
+  int stage = 0, buf = 0;
+  uint32_t parity = 0;
+  for (int64_t r = r0; r < end; ++r) {
+    if (r / a.rows_per_gate != group) {
+      group = r / a.rows_per_gate;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = a.s;
+      if (a.gamma_post) times(a.gamma_post, 0, w);
+      if (a.gate) times(a.gate, group * a.d, w);
+    }
+    const bool staged = r < safe;
+    if (staged && !bulk::wait(&full[stage], parity)) gave_up = 1;
+    const uint8_t* src = odd_ring + (size_t)stage * 2 * slot;
+    const Raw* rb = staged ? reinterpret_cast<const Raw*>(src + skew(r, a.ldb)) : static_cast<const Raw*>(a.b) + r * a.ldb;
+    const Raw* rx = staged ? reinterpret_cast<const Raw*>(src + slot + skew(r, a.ldx)) : static_cast<const Raw*>(a.x) + r * a.ldx;
+    auto put = [&](void* out, const float (&f)[8]) {
+      Raw* o = static_cast<Raw*>(out) + r * a.d + t;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (t + j * TPR < a.d) o[j * TPR] = E::bits(f[j]);
+    };
+    float v[8], x[8], ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = min(t + j * TPR, a.d - 1);
+      v[j] = E::value(rb[c]);
+      x[j] = E::value(rx[c]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss = t + j * TPR < a.d ? fmaf(v[j], v[j], ss) : ss;
+    const float inv_b = rsqrtf(row_sum<TPR>(ss, red[buf], 0) * inv_d + a.eps);
+    // past the sum's barrier every thread has read the row: its place is refilled
+    if (t == 0) fetch(r + a.stages, stage);
+    if (gave_up) break;
+    ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = fmaf(v[j] * inv_b, w[j], a.alpha * x[j]);
+      ss = t + j * TPR < a.d ? fmaf(v[j], v[j], ss) : ss;
+    }
+    put(a.y, v);
+    if (t == 0) a.inv_b[r] = inv_b;
+    if (a.pre) {
+      const float inv_y = rsqrtf(row_sum<TPR>(ss, red[buf + 1], 0) * inv_d + a.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= inv_y * wn[j];
+      put(a.n, v);
+      if (t == 0) a.inv_y[r] = inv_y;
+    }
+    buf ^= 2;
+    if (++stage == a.stages) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+  if (gave_up && t == 0) {
+    // a copy did not arrive in time: report it, and leave no copy in flight behind
+    atomicExch(&g_norm_error, NVFP4B200_ERR_TIMEOUT);
+    for (int st = 0; st < a.stages; ++st) bulk::wait(&full[st], parity ^ (st < stage ? 1u : 0u));
+  }
+}
+
 struct BwdArgs {
   const void *dy, *dn, *b, *y, *gamma_post, *gate, *gamma_pre;
   const float *inv_b, *inv_y;
@@ -516,7 +629,6 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
 // The column sums live in shared memory, each thread's own words, so that a
 // thread fits 64 registers and 32 warps share an SM: with the sums in registers
 // 16 warps did, and waited for one another's barriers (147 us against 134 at 16000 x 4096).
-__device__ int g_norm_error = 0;
 
 constexpr int BWD_STAGES = 3;   // rows of the ring, at most
 
@@ -907,7 +1019,7 @@ int nvfp4b200_sandwich_norm(const void* b, const void* x, const void* gamma_post
   if (rc) return rc;
   if (rows == 0) return NVFP4B200_OK;
   norm::FwdArgs a{b, x, gamma_post, gate, gamma_pre, y, n, inv_b, inv_y, rows, ldb, ldx, groups ? rows / groups : rows,
-                  (int)d, residual_scale, branch_scale, eps, n != nullptr};
+                  (int)d, residual_scale, branch_scale, eps, n != nullptr, 0, 0, 0};
   const bool vec = (d * bytes) % 16 == 0 && d % 8 == 0 && vec_ok(b, ldb, bytes) && vec_ok(x, ldx, bytes) &&
                    vec_ok(gamma_post, d, bytes) && vec_ok(gate, d, bytes) && vec_ok(gamma_pre, d, bytes) &&
                    vec_ok(y, d, bytes) && vec_ok(n, d, bytes);
@@ -927,6 +1039,24 @@ int nvfp4b200_sandwich_norm(const void* b, const void* x, const void* gamma_post
         const int per_sm = std::max(1, std::min(norm::MAX_SMEM / smem, T < 512 ? 4 : 1024 / T));
         fn<<<(unsigned)std::min<int64_t>(want, (int64_t)sm_count_current() * per_sm), THREADS, smem, st>>>(a);
         return launch_status();
+      }
+      if constexpr (!decltype(v)::value && T >= 64 && T <= 512) {
+        // unaligned rows of more than 512 columns, 8 columns a thread: 114 -> 82 us at 8000 x
+        // 4095 bf16 with the next norm (20000 x 301: 24 us without, 28 with)
+        constexpr int T2 = 2 * T;
+        const int row = 2 * ((int)round_up(d * bytes, 16) + 16), share = norm::MAX_SMEM / std::max(1, 1024 / T2);
+        if (aligned(b, 16) && aligned(x, 16) && row <= share) {
+          a.stages = std::min(norm::STAGES, share / row);
+          a.safe_rows = std::max<int64_t>(0, rows - 1 - 15 / (std::min(ldb, ldx) * bytes));
+          auto* odd = norm::sandwich_fwd_odd_kernel<DT, T2>;
+          const int size = a.stages * row;
+          if (size > 32 * 1024 &&   // with the static arrays, past the default limit
+              cudaFuncSetAttribute(odd, cudaFuncAttributeMaxDynamicSharedMemorySize, size) != cudaSuccess)
+            return (int)NVFP4B200_ERR_CUDA;
+          a.rows_per_cta = ceil_div(rows, (int64_t)sm_count_current() * (1024 / T2));
+          odd<<<(unsigned)ceil_div(rows, a.rows_per_cta), T2, size, st>>>(a);
+          return launch_status();
+        }
       }
       const unsigned grid = (unsigned)std::min<int64_t>(want, (int64_t)sm_count_current() * (2048 / THREADS));
       norm::sandwich_fwd_kernel<decltype(dt)::value, decltype(v)::value, T><<<grid, THREADS, 0, st>>>(a);

@@ -126,7 +126,8 @@ def test_strides_and_misaligned(pkg):
     ops = pkg.ops
     t, d = 37, 264
     big = rnd((t, 3 * d), 1, BF)
-    for b, x in ((big[:, :d], big[:, 2 * d:]), (big[:, 1:d + 1], big[:, d + 3:2 * d + 3]),
+    odd = rnd((t, 3 * d + 1), 6, BF)
+    for b, x in ((odd[:, :d], odd[:, 2 * d:3 * d]), (big[:, :d], big[:, 2 * d:]), (big[:, 1:d + 1], big[:, d + 3:2 * d + 3]),
                  (rnd((d, t), 2, BF).t(), big[:, :d]), (big[:1, :d].expand(t, d), big[:, d:2 * d])):
         gp, gate, gn = rnd((d,), 3, BF), rnd((1, d), 4, BF), rnd((d,), 5, BF)
         got = ops.sandwich_norm(b, x, gp, gate, gn)
@@ -142,6 +143,38 @@ def test_strides_and_misaligned(pkg):
             close(g[k], ref[k], mg[k], BF)
         for k in ("dgamma_post", "dgate", "dgamma_pre"):
             close(g[k], ref[k], mg[k], extra=F32 + (t + 64) * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FL])
+@pytest.mark.parametrize("t,d", [(1, 3), (2, 7), (9, 1), (500, 5), (300, 67), (1000, 1001), (401, 4097), (97, 8191), (700, 2050)])
+def test_widths_of_no_multiple(pkg, t, d, dtype):
+    """Unaligned rows, many of them, the tensors ending with their storage: forward and
+    backward against float64, and nothing read beside them (neighbours are NaN)."""
+    ops = pkg.ops
+
+    def lone(seed, std=1.0):   # a [t, d] view that starts 16-byte aligned, NaN before and after
+        flat = torch.full((t * d + 32,), math.nan, device="cuda", dtype=dtype)
+        flat[16:16 + t * d] = rnd((t * d,), seed, dtype, std)
+        return flat[16:16 + t * d].view(t, d)
+
+    b, x, dy, dn = lone(1, 2.0), lone(2), lone(3, 0.1), lone(4, 0.1)
+    gp, gate, gn = rnd((d,), 5, dtype, 0.3) + 1, rnd((1, d), 6, dtype), rnd((d,), 7, dtype, 0.3) + 1
+    y, n, ib, iy = ops.sandwich_norm(b, x, gp, gate, gn, branch_scale=0.7)
+    ry, rib, mag = forward64(b, x, gp, gate, gn, 1.0, 0.7, 1e-6)
+    close(ib, rib, rib)
+    close(y, ry, mag, dtype)
+    riy = (ry.square().mean(1) + 1e-6).rsqrt()
+    off = riy * (mag.square().mean(1) + 1e-6).sqrt()
+    close(n, ry * riy[:, None] * gn.double(), (mag * (1 + off[:, None])) * riy[:, None] * gn.double().abs(), dtype)
+    for kw in (dict(dn=dn, y=y, inv_y=iy, gamma_pre=gn), {}):
+        got = ops.sandwich_norm_bwd(dy, b, ib, gp, gate, branch_scale=0.7, **kw)
+        ref, big = backward64(dy, kw.get("dn"), b, y, ib, iy, gp, gate, gn, 1.0, 0.7)
+        for k in ("dx", "db"):
+            close(got[k], ref[k], big[k], dtype)
+        for k in ("dgamma_post", "dgate", "dgamma_pre"):
+            if got[k] is not None:
+                close(got[k], ref[k], big[k], extra=F32 + (t + 64) * 2.0 ** -24)
+    assert ops.device_error() == 0
 
 
 def test_zero_rows_and_no_rows(pkg):
