@@ -205,11 +205,12 @@ class SandwichNormFunction(torch.autograd.Function):
         y, n, inv_b, inv_y = ops.sandwich_norm(b2, x.reshape(-1, d), gamma_post, gate, gamma_pre,
                                                residual_scale=residual_scale, branch_scale=branch_scale, eps=eps,
                                                pre=pre)
+        if b.dim() != 2:   # not views, so that users may change the results in place
+            y, n = (None if t is None else torch.ops.aten._unsafe_view(t, b.shape) for t in (y, n))
+        # y as it is returned: a change of it in place before the backward that reads it is refused
         ctx.save_for_backward(b2, y if n is not None else None, inv_b, inv_y, gamma_post, gate, gamma_pre)
         ctx.scales, ctx.shape = (residual_scale, branch_scale), b.shape
         ctx.set_materialize_grads(False)
-        if b.dim() != 2:   # not views, so that users may change the results in place
-            y, n = (None if t is None else torch.ops.aten._unsafe_view(t, b.shape) for t in (y, n))
         return y if n is None else (y, n)
 
     @staticmethod
@@ -219,7 +220,7 @@ class SandwichNormFunction(torch.autograd.Function):
             return (None,) * 9
         b, y, inv_b, inv_y, gamma_post, gate, gamma_pre = ctx.saved_tensors
         flat = lambda t: None if t is None else t.reshape(b.shape)
-        more = dict(dn=flat(dn), y=y, inv_y=inv_y, gamma_pre=gamma_pre) if dn is not None else {}
+        more = dict(dn=flat(dn), y=flat(y), inv_y=inv_y, gamma_pre=gamma_pre) if dn is not None else {}
         g = ops.sandwich_norm_bwd(flat(dy), b, inv_b, gamma_post, gate, residual_scale=ctx.scales[0],
                                   branch_scale=ctx.scales[1], **more)
         like = lambda v, p: None if p is None or v is None else v.reshape(p.shape).to(p.dtype)
