@@ -44,6 +44,10 @@ int code_of(const Tensor& t) {
 
 void* ptr(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
 bool on(const Tensor& t, const Tensor& like) { return t.is_cuda() && t.get_device() == like.get_device(); }
+// Counts a write into a caller's tensor, so that autograd refuses a backward that saved it before.
+void wrote(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 int64_t scale_rows(int64_t rows) { return up(rows, 128); }
 int64_t scale_cols(int64_t k) { return up(k / 32, 4); }
@@ -113,6 +117,10 @@ std::pair<Pair, Pair> quantize(const Tensor& x_, const OptTensor& row_, const Op
   if (cols) b = operand(x, c, up(r, 32), rows ? std::nullopt : out);
   quantize_into(x, row, gamma, rows ? a.first.data_ptr() : nullptr, rows ? a.second.data_ptr() : nullptr,
                 cols ? b.first.data_ptr() : nullptr, cols ? b.second.data_ptr() : nullptr, at_.stream);
+  if (out) {
+    wrote(out->first);
+    wrote(out->second);
+  }
   return {a, b};
 }
 
@@ -186,6 +194,7 @@ Tensor mx_gemm(const Tensor& qa, const Tensor& sa, const Tensor& qb, const Tenso
                             out.data_ptr(), out.scalar_type() == at::kFloat ? NVFP4B200_F32 : NVFP4B200_BF16,
                             accumulate, epilogue, m, n, k, out.stride(0), at_.stream),
           "nvfp4b200_mx_gemm");
+  if (out_) wrote(out);
   return out;
 }
 
@@ -274,6 +283,12 @@ std::tuple<Tensor, OptTensor, OptTensor> linear_forward(const Tensor& x_, const 
   return {y, xt, wt};
 }
 
+int64_t tokens(const std::vector<int64_t>& x_shape) {
+  int64_t t = 1;
+  for (size_t i = 0; i + 1 < x_shape.size(); ++i) t *= x_shape[i];
+  return t;
+}
+
 // Its backward: dx in x's shape and dy's type, dw fp32 or bf16.
 std::tuple<OptTensor, OptTensor> linear_backward(const Tensor& dy_, const OptTensor& xt, const OptTensor& wt,
                                                  const std::vector<int64_t>& x_shape, int64_t n, bool need_x, bool need_w,
@@ -282,7 +297,7 @@ std::tuple<OptTensor, OptTensor> linear_backward(const Tensor& dy_, const OptTen
               "mxfp4_linear's gradient must be bf16 or fp32");
   const int64_t k = x_shape.back();
   On at_(dy_);
-  const Tensor dy = float_matrix(dy_.dim() == 2 ? dy_ : dy_.reshape({-1, n}));
+  const Tensor dy = float_matrix(dy_.dim() == 2 ? dy_ : dy_.reshape({tokens(x_shape), n}));
   const int64_t t = dy.size(0), tp = up(t, 32);
   TORCH_CHECK((!need_x || (wt && on(*wt, dy) && wt->numel() == operand_bytes(k, n))) &&
                   (!need_w || (xt && on(*xt, dy) && xt->numel() == operand_bytes(k, tp))),
@@ -340,7 +355,7 @@ struct MXLinear : public torch::autograd::Function<MXLinear> {
       if (dw) out[1] = dw->scalar_type() == wtype ? *dw : dw->to(wtype);
     }
     if (b >= 0 && ctx->needs_input_grad(2))
-      out[2] = dy.reshape({-1, n}).sum(at::IntArrayRef{0}, false, at::kFloat).to((at::ScalarType)b);
+      out[2] = dy.reshape({tokens(shape), n}).sum(at::IntArrayRef{0}, false, at::kFloat).to((at::ScalarType)b);
     return out;
   }
 };
@@ -407,6 +422,8 @@ std::tuple<OptTensor, OptTensor, OptTensor> grad_norm(const std::vector<Tensor>&
                             ws.data_ptr<double>(), words, static_cast<float*>(ptr(norm)), static_cast<float*>(ptr(coef)),
                             static_cast<double*>(ptr(total)), c10::cuda::getCurrentCUDAStream(dev.index()).stream()),
         "nvfp4b200_grad_norm");
+  if (write)
+    for (const Tensor& t : in_place ? grads : *outs) wrote(t);
   return {norm, coef, total};
 }
 

@@ -285,3 +285,42 @@ def test_trainer_clips(pkg, micro):
         for a, b in zip(tr.blocks, free.blocks):
             lo = d   # past gamma
             assert (a.m[lo:] - coef * b.m[lo:]).abs().max() <= 2e-4 * coef * b.m[lo:].abs().max()
+
+
+def test_writes_are_counted(pkg):
+    """A tensor that autograd saved and clipping then wrote: its backward is
+    refused, as after any change in place.  Tensors of inference mode count nothing."""
+    for out in (False, True):
+        p = torch.randn(100, device="cuda", requires_grad=True)
+        t = torch.randn(100, device="cuda")
+        loss = (p * t).sum()
+        pkg.ops.clip_grad_norm([torch.randn(100, device="cuda")] if out else [t], 0.5, out=[t] if out else None)
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+    with torch.inference_mode():
+        t = torch.randn(100, device="cuda")
+        ref = t.double().norm().item()
+        assert abs(pkg.ops.clip_grad_norm([t], 0.5).item() - ref) <= REL * ref
+    assert t.norm().item() < 0.51
+
+
+def test_two_threads(pkg):
+    """Calls from several host threads, each on its stream, as from one."""
+    import threading
+    lists = [tensors([(257, 515), 33, 100_003 * (i + 1)], [FL, BF, HF], seed=i) for i in range(4)]
+    ref = [pkg.ops.grad_norm(g) for g in lists]
+    torch.cuda.synchronize()
+    got = [[] for _ in lists]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got[i].append(pkg.ops.grad_norm(lists[i]))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(len(g) == 50 and all(torch.equal(v, r) for v in g) for g, r in zip(got, ref))

@@ -419,3 +419,15 @@ def test_linear_on_two_streams_at_once(pkg):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, ref))
     assert ops.device_error() == 0
+
+
+def test_no_output_features(pkg, f4):
+    """A weight of no rows: an empty result, and gradients of zeros."""
+    for shape in ((2, 3, 64), (5, 64), (0, 2, 64)):
+        x = torch.randn(shape, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        w = torch.empty(0, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        b = torch.empty(0, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        y = f4.mxfp4_linear(x, w, b)
+        assert y.shape == (*shape[:-1], 0)
+        y.sum().backward()
+        assert (x.grad == 0).all() and x.grad.shape == x.shape and w.grad.shape == w.shape and b.grad.shape == b.shape
