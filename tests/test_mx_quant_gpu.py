@@ -431,3 +431,34 @@ def test_no_output_features(pkg, f4):
         assert y.shape == (*shape[:-1], 0)
         y.sum().backward()
         assert (x.grad == 0).all() and x.grad.shape == x.shape and w.grad.shape == w.shape and b.grad.shape == b.shape
+
+
+@pytest.mark.parametrize("m", [1, 8, 37])
+def test_chain_in_a_graph(pkg, m):
+    """Layers one after another, captured: each result is the next call's input,
+    its memory is used again two calls later, and every call may start early."""
+    ops = pkg.ops
+    k = 2048
+    ws = [ops.mx_quantize(make(k, k, torch.bfloat16, s, 0.0) * k ** -0.5) for s in range(12)]
+    xs = [make(m, k, torch.bfloat16, 20 + s, 0.0) for s in range(3)]
+    ref = []
+    for x in xs:
+        for w in ws:
+            x = ops.mx_linear(x, *w)
+            torch.cuda.synchronize()
+        ref.append(x)
+        assert x.float().norm() > 0
+    hold = xs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = hold
+        for w in ws:
+            y = ops.mx_linear(y, *w)
+    for rep in range(30):
+        hold.copy_(xs[rep % 3])
+        graph.replay()
+        assert torch.equal(y, ref[rep % 3]), rep
+        z = xs[rep % 3]
+        for w in ws:
+            z = ops.mx_linear(z, *w)
+        assert torch.equal(z, ref[rep % 3]), rep
