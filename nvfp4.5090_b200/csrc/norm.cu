@@ -36,7 +36,9 @@ namespace norm {
 constexpr int VPT = 2;            // 8-element vectors per thread and row
 constexpr int CPT = 8 * VPT;      // columns per thread
 constexpr int MAX_D = 1024 * CPT;
-constexpr int MAX_SMEM = 220 * 1024;
+constexpr int MAX_SMEM = 225 * 1024;   // dynamic, of one CTA: 227 KB less the static arrays
+// what n CTAs of an SM can each have: its 228 KB less 1 KB per CTA that the system takes and 1 KB of static arrays
+constexpr int smem_share(int n) { return n <= 1 ? MAX_SMEM : 228 * 1024 / n - 2048; }
 
 template <int DT>
 constexpr int dtype_size() { return DT == NVFP4B200_F32 ? 4 : 2; }
@@ -638,7 +640,11 @@ constexpr int BWD_STAGES = 3;   // rows of the ring, at most
 // 16-byte pieces, a thread's eight columns are TPR apart and are read and
 // written one by one; the last rows, whose windows could reach past the tensor,
 // are read straight from global memory.
-template <int DT, int TPR, bool PRE, bool ODD>
+// MULTI: a CTA's rows are whole groups (few rows each, one at the least: a gate
+// per token).  W is set up anew at a group's start, the next group's gate having
+// been brought to L2, and S is handed over at its end; the sum of gate * S is
+// kept beside the other column sums.
+template <int DT, int TPR, bool PRE, bool ODD, bool MULTI>
 __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1024 / TPR)
     sandwich_bwd_staged_kernel(const BwdArgs a, int64_t parts_per_group) {
   using E = Elem<DT>;
@@ -656,8 +662,8 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
   const int row_bytes = a.d * (int)sizeof(Raw);
   const int slot = ODD ? ((row_bytes + 15) & ~15) + 16 : row_bytes;   // of one tensor's row in the ring
   const int64_t g = blockIdx.x / parts_per_group, p = blockIdx.x % parts_per_group;
-  const int64_t r0 = g * a.rows_per_gate + p * a.rows_per_cta;
-  const int rows = (int)(imin64(r0 + a.rows_per_cta, (g + 1) * a.rows_per_gate) - r0);
+  const int64_t r0 = MULTI ? (int64_t)blockIdx.x * a.rows_per_cta : g * a.rows_per_gate + p * a.rows_per_cta;
+  const int rows = (int)(imin64(r0 + a.rows_per_cta, MULTI ? a.rows : (g + 1) * a.rows_per_gate) - r0);
 
   const int staged = (int)imin64(rows, ODD ? (a.safe_rows > r0 ? a.safe_rows - r0 : 0) : rows);
   auto skew = [&](int64_t r, int64_t ld) { return ODD ? (int)((uint64_t)(r * ld) * sizeof(Raw) & 15) : 0; };
@@ -690,10 +696,10 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
   if (t == 0)
     for (int st = 0; st < ST; ++st) fetch(st, st);
 
-  // column sums, each thread's own: S (2 float4) and dgamma_pre's (2 more)
+  // column sums, each thread's own: S (2 float4), dgamma_pre's (2 more), gate * S over the groups (2 more)
   ulonglong2* sums_at = reinterpret_cast<ulonglong2*>(row_ring + (size_t)ST * NT * slot) + t;
 #pragma unroll
-  for (int j = 0; j < (PRE ? 4 : 2); ++j) sums_at[j * TPR] = make_ulonglong2(0ull, 0ull);
+  for (int j = 0; j < NT + (MULTI ? 2 : 0); ++j) sums_at[j * TPR] = make_ulonglong2(0ull, 0ull);
   const int c = ODD ? t : 8 * t;   // the thread's first column; the others follow, or (ODD) are TPR apart
   const bool in = c < a.d;
   auto weights = [&](const void* p, int64_t off, uint64_t (&w)[NP]) {
@@ -711,12 +717,30 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
 #pragma unroll
   for (int j = 0; j < NP; ++j) W[j] = f2two(a.s);
   if (a.gamma_post) weights(a.gamma_post, 0, W);
-  if (a.gate) weights(a.gate, g * a.d, W);
+  if (!MULTI && a.gate) weights(a.gate, g * a.d, W);
+  int64_t group = MULTI ? r0 / a.rows_per_gate - 1 : 0, left = 0;
   if constexpr (PRE) {
 #pragma unroll
     for (int j = 0; j < NP; ++j) gpre[j] = f2two(1.0f);
     if (a.gamma_pre) weights(a.gamma_pre, 0, gpre);
   }
+
+  auto put = [&](float* row, bool wide, int h, uint64_t lo, uint64_t hi) {   // the thread's columns 4 h .. 4 h + 3
+    if (ODD) {
+      const float f[4] = {f2lo(lo), f2hi(lo), f2lo(hi), f2hi(hi)};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + (4 * h + j) * TPR < a.d) row[c + (4 * h + j) * TPR] = f[j];
+      return;
+    }
+    float* out = row + c + 4 * h;   // d % 8 == 0: 16-byte aligned where the first row is
+    if (wide) {
+      *reinterpret_cast<ulonglong2*>(out) = make_ulonglong2(lo, hi);
+    } else {
+      out[0] = f2lo(lo); out[1] = f2hi(lo); out[2] = f2lo(hi); out[3] = f2hi(hi);
+    }
+  };
+  const bool aligned_dgate = MULTI && (reinterpret_cast<uintptr_t>(a.dgate) & 15) == 0;
 
   Raw *dx = static_cast<Raw*>(a.dx) + r0 * a.d, *db = static_cast<Raw*>(a.db) + r0 * a.d;
   const float *ib = a.inv_b + r0, *iy = PRE ? a.inv_y + r0 : nullptr;
@@ -728,6 +752,21 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
     if (i + 1 < rows) {   // a row ahead, so that its latency is not exposed once per row
       next_b = __ldg(ib + i + 1);
       if (PRE) next_y = __ldg(iy + i + 1);
+    }
+    if constexpr (MULTI) {
+      if (left == 0) {   // a group begins
+        left = a.rows_per_gate;
+        ++group;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) W[j] = f2two(a.s);
+        if (a.gamma_post) weights(a.gamma_post, 0, W);
+        weights(a.gate, group * a.d, W);
+        if (i + left < rows && in && t % (128 / (ODD ? (int)sizeof(Raw) : 16)) == 0)
+          for (int j = 0; j < (ODD ? 8 : 1); ++j)
+            if (c + j * TPR < a.d)
+              asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const Raw*>(a.gate) + (group + 1) * a.d + c + j * TPR));
+      }
+      --left;
     }
     if (i < staged && !bulk::wait(&full[stage], parity)) gave_up = 1;
     const uint8_t* src = row_ring + (size_t)stage * NT * slot;
@@ -823,6 +862,29 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
       dxv[2 * j] = f2lo(e); dxv[2 * j + 1] = f2hi(e);
       dbv[2 * j] = f2lo(d); dbv[2 * j + 1] = f2hi(d);
     }
+    if constexpr (MULTI) {
+      if (left == 0) {   // and ends
+        const uint64_t one = f2two(1.0f);
+        uint64_t dg[NP], gs[NP];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          dg[j] = gs[j] = f2mul(S[j], f2two(a.s));
+          S[j] = 0ull;
+        }
+        weights(a.gate, group * a.d, gs);
+        if (a.gamma_post) weights(a.gamma_post, 0, dg);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const ulonglong2 v = sums_at[(NT + h) * TPR];
+          sums_at[(NT + h) * TPR] = make_ulonglong2(f2fma(gs[2 * h], one, v.x), f2fma(gs[2 * h + 1], one, v.y));
+        }
+        if (a.dgate && in) {
+          float* out = a.dgate + group * a.d;
+          put(out, aligned_dgate, 0, dg[0], dg[1]);
+          put(out, aligned_dgate, 1, dg[2], dg[3]);
+        }
+      }
+    }
     sums_at[0] = make_ulonglong2(S[0], S[1]);
     sums_at[TPR] = make_ulonglong2(S[2], S[3]);
     if (ODD) {
@@ -854,31 +916,21 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
   uint64_t gate[NP];
 #pragma unroll
   for (int j = 0; j < NP; ++j) gate[j] = f2two(1.0f);
-  if (a.gate) weights(a.gate, g * a.d, gate);
-  auto put = [&](float* row, int h, uint64_t lo, uint64_t hi) {   // the thread's columns 4 h .. 4 h + 3
-    if (ODD) {
-      const float f[4] = {f2lo(lo), f2hi(lo), f2lo(hi), f2hi(hi)};
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (c + (4 * h + j) * TPR < a.d) row[c + (4 * h + j) * TPR] = f[j];
-      return;
-    }
-    float* out = row + c + 4 * h;   // d % 8 == 0: 16-byte aligned where the workspace is
-    if (a.ws16) {
-      *reinterpret_cast<ulonglong2*>(out) = make_ulonglong2(lo, hi);
-    } else {
-      out[0] = f2lo(lo); out[1] = f2hi(lo); out[2] = f2lo(hi); out[3] = f2hi(hi);
-    }
-  };
+  if (!MULTI && a.gate) weights(a.gate, g * a.d, gate);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const ulonglong2 sv = sums_at[h * TPR];
-    const uint64_t lo = f2mul(sv.x, f2two(a.s)), hi = f2mul(sv.y, f2two(a.s));
-    if (a.gate) put(a.part_gate + (int64_t)blockIdx.x * a.d, h, lo, hi);
-    put(a.part + (int64_t)blockIdx.x * a.d, h, f2mul(lo, gate[2 * h]), f2mul(hi, gate[2 * h + 1]));
+    if constexpr (MULTI) {
+      const ulonglong2 v = sums_at[(NT + h) * TPR];
+      put(a.part + (int64_t)blockIdx.x * a.d, a.ws16, h, v.x, v.y);
+    } else {
+      const ulonglong2 sv = sums_at[h * TPR];
+      const uint64_t lo = f2mul(sv.x, f2two(a.s)), hi = f2mul(sv.y, f2two(a.s));
+      if (a.gate) put(a.part_gate + (int64_t)blockIdx.x * a.d, a.ws16, h, lo, hi);
+      put(a.part + (int64_t)blockIdx.x * a.d, a.ws16, h, f2mul(lo, gate[2 * h]), f2mul(hi, gate[2 * h + 1]));
+    }
     if (PRE) {
       const ulonglong2 pv = sums_at[(2 + h) * TPR];
-      put(a.part + ((int64_t)gridDim.x + blockIdx.x) * a.d, h, pv.x, pv.y);
+      put(a.part + ((int64_t)gridDim.x + blockIdx.x) * a.d, a.ws16, h, pv.x, pv.y);
     }
   }
 }
@@ -964,23 +1016,31 @@ struct Split {
   int64_t rows_per_cta, parts_per_group, ctas;
 };
 
+constexpr int START_ROWS = 4;
+
 static Split split_rows(int64_t rows, int64_t groups, int64_t d, int sms) {
   // 512 threads' worth of CTAs per SM (128 registers a thread), narrow rows in
   // more, smaller CTAs
   int64_t tpr = 32;
   while (tpr * CPT < d) tpr *= 2;
   const int64_t per = rows / groups, target = std::max<int64_t>(1, 512 / tpr) * sms;
-  Split s;
-  if (groups >= target || per == 1) {             // whole groups per CTA
-    const int64_t g = std::max<int64_t>(1, ceil_div(groups, target));
-    s.rows_per_cta = g * per;
-    s.parts_per_group = 1;
-    s.ctas = ceil_div(groups, g);
-  } else {
-    const int64_t parts = std::min(per, std::max<int64_t>(1, target / groups));
-    s.rows_per_cta = ceil_div(per, parts);
-    s.parts_per_group = ceil_div(per, s.rows_per_cta);
-    s.ctas = groups * s.parts_per_group;
+  // A CTA takes a part of a group's rows, or whole groups.  The cost is counted in
+  // rows: waves of CTAs times the rows of one and some more for its start.
+  Split s{0, 1, 0};
+  int64_t best = INT64_MAX;
+  for (int64_t waves = 1; waves <= 4; ++waves) {
+    const int64_t fit = waves * target / groups;      // parts of a group
+    const int64_t whole = ceil_div(groups, waves * target);
+    for (const int64_t rows_per : {fit > 1 && per > 1 ? ceil_div(per, fit) : int64_t(0), whole * per}) {
+      if (rows_per == 0) continue;
+      const int64_t parts = rows_per < per ? ceil_div(per, rows_per) : 1;
+      const int64_t ctas = rows_per < per ? groups * parts : ceil_div(groups, rows_per / per);
+      const int64_t cost = ceil_div(ctas, target) * (rows_per + START_ROWS);
+      if (cost < best) {
+        best = cost;
+        s = {rows_per, parts, ctas};
+      }
+    }
   }
   return s;
 }
@@ -1036,7 +1096,7 @@ int nvfp4b200_sandwich_norm(const void* b, const void* x, const void* gamma_post
         if (smem > 32 * 1024 &&   // with the static arrays, past the default limit
             cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
           return (int)NVFP4B200_ERR_CUDA;
-        const int per_sm = std::max(1, std::min(norm::MAX_SMEM / smem, T < 512 ? 4 : 1024 / T));
+        const int per_sm = std::max(1, std::min(228 * 1024 / (smem + 2048), T < 512 ? 4 : 1024 / T));
         fn<<<(unsigned)std::min<int64_t>(want, (int64_t)sm_count_current() * per_sm), THREADS, smem, st>>>(a);
         return launch_status();
       }
@@ -1044,7 +1104,7 @@ int nvfp4b200_sandwich_norm(const void* b, const void* x, const void* gamma_post
         // unaligned rows of more than 512 columns, 8 columns a thread: 114 -> 82 us at 8000 x
         // 4095 bf16 with the next norm (20000 x 301: 24 us without, 28 with)
         constexpr int T2 = 2 * T;
-        const int row = 2 * ((int)round_up(d * bytes, 16) + 16), share = norm::MAX_SMEM / std::max(1, 1024 / T2);
+        const int row = 2 * ((int)round_up(d * bytes, 16) + 16), share = norm::smem_share(1024 / T2);
         if (aligned(b, 16) && aligned(x, 16) && row <= share) {
           a.stages = std::min(norm::STAGES, share / row);
           a.safe_rows = std::max<int64_t>(0, rows - 1 - 15 / (std::min(ldb, ldx) * bytes));
@@ -1128,16 +1188,19 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
         // so its memory: as many ring rows as fit, up to 3 (2 with the next norm's
         // tensors); one row at least, alone on the SM if need be
         const int width = (int)d * bytes, row = (dn ? 4 : 2) * (ODD ? (int)round_up(width, 16) + 16 : width);
-        const int sums = (dn ? 4 : 2) * 16 * T2;
-        const int share = norm::MAX_SMEM / std::max(1, 1024 / T2);
+        const bool multi = gate && sp.parts_per_group == 1;   // a CTA's rows are whole groups
+        const int sums = ((dn ? 4 : 2) + (multi ? 2 : 0)) * 16 * T2;
+        const int share = norm::smem_share(1024 / T2);
         a.stages = std::max(std::min(dn ? 2 : norm::BWD_STAGES, (share - sums) / row), 1);
         const int smem = a.stages * row + sums;
         const int64_t ld_min = std::min(std::min(dy ? ld_dy : ldb, ldb), dn ? std::min(ld_dn, ldy) : ldb);
         a.safe_rows = std::max<int64_t>(0, rows - 1 - 15 / (ld_min * bytes));
         const bool bases = aligned(b, 16) && (!dy || aligned(dy, 16)) && (!dn || (aligned(dn, 16) && aligned(y, 16)));
-        if (smem <= norm::MAX_SMEM && (!gate || sp.parts_per_group > 1) && (!ODD || bases)) {
-          auto* fn = dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true, ODD>
-                        : norm::sandwich_bwd_staged_kernel<DT, T2, false, ODD>;
+        if (smem <= norm::MAX_SMEM && (!ODD || bases)) {
+          auto* fn = multi ? (dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true, ODD, true>
+                                 : norm::sandwich_bwd_staged_kernel<DT, T2, false, ODD, true>)
+                           : (dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true, ODD, false>
+                                 : norm::sandwich_bwd_staged_kernel<DT, T2, false, ODD, false>);
           if (smem > 32 * 1024 &&   // with the static arrays, past the default limit
               cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
             return (int)NVFP4B200_ERR_CUDA;

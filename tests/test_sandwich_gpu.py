@@ -177,6 +177,30 @@ def test_widths_of_no_multiple(pkg, t, d, dtype):
     assert ops.device_error() == 0
 
 
+@pytest.mark.parametrize("dtype", [BF, FL])
+@pytest.mark.parametrize("per,d", [(1, 4096), (1, 1001), (3, 1001), (2, 96), (7, 520), (1, 7), (5, 4104), (1, 8191), (40, 2048)])
+def test_many_gates(pkg, per, d, dtype):
+    """More groups of rows than CTAs: a CTA walks several groups, and the last one fewer."""
+    ops = pkg.ops
+    groups = (5000 if d < 100 else 1900 if d < 1100 else 701) // (1 if per < 8 else 4)
+    t = groups * per
+    b, y, dy, dn = (rnd((t, d), i, dtype, s) for i, s in ((1, 2.0), (2, 1.0), (3, 0.1), (4, 0.1)))
+    gp, gate, gn = rnd((d,), 5, dtype, 0.3) + 1, rnd((groups, d), 6, dtype), rnd((d,), 7, dtype, 0.3) + 1
+    ib, iy = rnd((t,), 8).abs() + 0.1, rnd((t,), 9).abs() + 0.1
+    for kw in (dict(dn=dn, y=y, inv_y=iy, gamma_pre=gn), {}):
+        for w in (gp, None):
+            got = ops.sandwich_norm_bwd(dy, b, ib, w, gate, residual_scale=0.5, branch_scale=-0.7, **kw)
+            ref, big = backward64(dy, kw.get("dn"), b, y, ib, iy, w, gate, gn, 0.5, -0.7)
+            for k in ("dx", "db"):
+                close(got[k], ref[k], big[k], dtype)
+            for k in ("dgamma_post", "dgate", "dgamma_pre"):
+                if got[k] is not None:
+                    close(got[k], ref[k], big[k], extra=F32 + (t + 64) * 2.0 ** -24)
+            again = ops.sandwich_norm_bwd(dy, b, ib, w, gate, residual_scale=0.5, branch_scale=-0.7, **kw)
+            assert all(got[k] is None or torch.equal(got[k], again[k]) for k in got)
+    assert ops.device_error() == 0
+
+
 def test_zero_rows_and_no_rows(pkg):
     ops = pkg.ops
     b = torch.zeros(3, 64, device="cuda", dtype=BF)
