@@ -626,8 +626,8 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
 //     m1 = A / d,    m2 = (B - inv_y * m1 * C) / d
 //     t = t0 - inv_y * m1 * yh,    db = inv_b * (W t - m2 bh).
 // Arithmetic is on packed pairs of floats.  A CTA's rows lie in one group (W
-// stays in registers), so dgamma_post's part is gate * S at the end.  The
-// column sums S leave out s; it is multiplied in at the end.
+// stays in registers) but in the MULTI form, so dgamma_post's part is gate * S
+// at the end.  The column sums S leave out s; it is multiplied in at the end.
 // The column sums live in shared memory, each thread's own words, so that a
 // thread fits 64 registers and 32 warps share an SM: with the sums in registers
 // 16 warps did, and waited for one another's barriers (147 us against 134 at 16000 x 4096).
@@ -643,7 +643,8 @@ constexpr int BWD_STAGES = 3;   // rows of the ring, at most
 // MULTI: a CTA's rows are whole groups (few rows each, one at the least: a gate
 // per token).  W is set up anew at a group's start, the next group's gate having
 // been brought to L2, and S is handed over at its end; the sum of gate * S is
-// kept beside the other column sums.
+// kept beside the other column sums.  (With gate, gamma_post and that sum in
+// registers 16 warps share an SM: 316 us at 16000 x 4096 with a gate per row, 246 so.)
 template <int DT, int TPR, bool PRE, bool ODD, bool MULTI>
 __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1024 / TPR)
     sandwich_bwd_staged_kernel(const BwdArgs a, int64_t parts_per_group) {
@@ -1019,13 +1020,15 @@ struct Split {
 constexpr int START_ROWS = 4;
 
 static Split split_rows(int64_t rows, int64_t groups, int64_t d, int sms) {
-  // 512 threads' worth of CTAs per SM (128 registers a thread), narrow rows in
+  // CTAs that run at a time: 1024 threads per SM, 8 columns each; narrow rows in
   // more, smaller CTAs
   int64_t tpr = 32;
   while (tpr * CPT < d) tpr *= 2;
   const int64_t per = rows / groups, target = std::max<int64_t>(1, 512 / tpr) * sms;
   // A CTA takes a part of a group's rows, or whole groups.  The cost is counted in
-  // rows: waves of CTAs times the rows of one and some more for its start.
+  // rows: waves of CTAs times the rows of one and some more for its start.  (As many
+  // whole groups, or parts of one, as fill one wave: 16000 x 4096 with 160 gates 242
+  // us against 170 so, 100 gates 195 / 167, 320 gates 244 / 185.)
   Split s{0, 1, 0};
   int64_t best = INT64_MAX;
   for (int64_t waves = 1; waves <= 4; ++waves) {
@@ -1179,8 +1182,8 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
   return norm::by_type(dtype, vec, [&](auto dt, auto v) {
     const int r = norm::by_width((int)d, [&](auto tpr) {
       constexpr int T = decltype(tpr)::value, DT = decltype(dt)::value;
-      // the staged kernel where a row fits and a CTA's rows have one gate:
-      // 346 -> 152 us at 16000 x 4096 bf16 with 8 gates and the next norm
+      // the staged kernel where a row fits: 346 -> 152 us at 16000 x 4096 bf16 with 8
+      // gates and the next norm, 611 -> 246 with a gate per row
       if constexpr (T <= 512) {
         constexpr int T2 = 2 * T;
         constexpr bool ODD = !decltype(v)::value;
