@@ -29,23 +29,35 @@ __device__ __forceinline__ void copy(void* dst, const void* src, uint32_t bytes,
                : "memory");
 }
 
+// CLUSTER: for what another CTA of the cluster wrote.
+template <bool CLUSTER>
 __device__ __forceinline__ bool test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(addr(bar)), "r"(parity)
-      : "memory");
+  if (CLUSTER)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(addr(bar)), "r"(parity)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(addr(bar)), "r"(parity)
+        : "memory");
   return ok != 0;
 }
 
 // False when the phase did not complete within the limit.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
-  if (test(bar, parity)) return true;
+  if (test<CLUSTER>(bar, parity)) return true;
   const long long t0 = clock64();
-  while (!test(bar, parity))
+  while (!test<CLUSTER>(bar, parity))
     if (clock64() - t0 > WAIT_CYCLES) return false;
   return true;
 }

@@ -28,6 +28,7 @@
 #include "vec.cuh"
 
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 namespace nvfp4b200 {
@@ -245,88 +246,100 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) sandwich_fwd_kernel(con
 // barrier and the loads of the next rows run while a row waits for its two
 // reductions.  (The second sum is not folded into the first exchange: y's
 // square sum from those of its parts cancels where y is small.)
-template <int DT, int TPR>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, DT == NVFP4B200_F32 ? (TPR < 512 ? 2 : 1) : TPR < 512 ? 4 : 1024 / TPR)
+template <int DT, int TPR, int V>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR < 512 ? 4 : 1024 / TPR)
     sandwich_fwd_staged_kernel(const FwdArgs a) {
   using E = Elem<DT>;
   using Raw = typename E::Raw;
   constexpr int Q = (int)sizeof(Raw) * 8 / 16;
-  constexpr int NP = CPT / 2;
+  constexpr int NP = 4 * V;
   constexpr int THREADS = TPR < 256 ? 256 : TPR, GROUPS = THREADS / TPR;
-  extern __shared__ __align__(16) uint4 ring[];   // [STAGES][2][VPT * Q][THREADS]
+  extern __shared__ __align__(16) uint4 ring[];   // [STAGES][2][V * Q][THREADS]
   __shared__ float red[4][GROUPS * (TPR / 32)];
   const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
   const float inv_d = 1.0f / (float)a.d;
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   auto slot = [&](int stage, int tensor, int piece) {
-    return ring + ((stage * 2 + tensor) * (VPT * Q) + piece) * THREADS + threadIdx.x;
+    return ring + ((stage * 2 + tensor) * (V * Q) + piece) * THREADS + threadIdx.x;
   };
+  // first column of a 16-byte piece: neighbouring lanes' pieces are neighbours (fp32 8192 x 4096:
+  // 146 us with a thread's two pieces side by side, half a sector each, 88 so)
+  auto at = [&](int i, int q) { return ((i * Q + q) * TPR + t) * (8 / Q); };
   auto fetch = [&](int64_t r, int stage) {
     if (r < a.rows) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const Raw* row = k ? static_cast<const Raw*>(a.x) + r * a.ldx : static_cast<const Raw*>(a.b) + r * a.ldb;
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-          const int c = column<true, TPR>(t, 8 * i);
-          if (c < a.d) {
+        for (int i = 0; i < V; ++i) {
 #pragma unroll
-            for (int q = 0; q < Q; ++q)
-              cp_async16(slot(stage, k, i * Q + q), reinterpret_cast<const uint4*>(row + c) + q);
-          }
+          for (int q = 0; q < Q; ++q)
+            if (at(i, q) < a.d) cp_async16(slot(stage, k, i * Q + q), row + at(i, q));
         }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int i = 0; i < VPT; ++i)   // columns past the end stay zero in every stage
-    if (column<true, TPR>(t, 8 * i) >= a.d)
-      for (int k = 0; k < STAGES * 2; ++k)
-        for (int q = 0; q < Q; ++q) *slot(k >> 1, k & 1, i * Q + q) = make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < V; ++i)   // columns past the end stay zero in every stage
+    for (int q = 0; q < Q; ++q)
+      if (at(i, q) >= a.d)
+        for (int k = 0; k < STAGES * 2; ++k) *slot(k >> 1, k & 1, i * Q + q) = make_uint4(0, 0, 0, 0);
   int64_t r = (int64_t)blockIdx.x * GROUPS + group;
 #pragma unroll
   for (int st = 0; st < STAGES - 1; ++st) fetch(r + st * step, st);
 
   // a weight vector's pairs times v, or v where there is none
-  auto weigh = [&](const typename E::Vec8 (&w)[VPT], uint64_t (&v)[NP]) {
+  auto weigh = [&](const typename E::Vec8 (&w)[V], uint64_t (&v)[NP]) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
+    for (int i = 0; i < V; ++i) {
       float f[8];
       E::unpack(w[i], f);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[4 * i + j] = f2mul(v[4 * i + j], f2pack(f[2 * j], f[2 * j + 1]));
     }
   };
-  auto load_w = [&](const void* p, int64_t off, typename E::Vec8 (&w)[VPT]) {
+  auto load_w = [&](const void* p, int64_t off, typename E::Vec8 (&w)[V]) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = column<true, TPR>(t, 8 * i);
-      w[i] = c < a.d ? E::load(static_cast<const Raw*>(p) + off + c) : E::zero();
+    for (int i = 0; i < V; ++i) {
+      w[i] = E::zero();
+      const Raw* row = static_cast<const Raw*>(p) + off;
+      if constexpr (Q == 1) {
+        if (at(i, 0) < a.d) w[i] = E::load(row + at(i, 0));
+      } else {
+        if (at(i, 0) < a.d) w[i].a = *reinterpret_cast<const float4*>(row + at(i, 0));
+        if (at(i, 1) < a.d) w[i].b = *reinterpret_cast<const float4*>(row + at(i, 1));
+      }
     }
   };
   auto put = [&](void* base, int64_t r, const uint64_t (&v)[NP]) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = column<true, TPR>(t, 8 * i);
+    for (int i = 0; i < V; ++i) {
       float f[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         f[2 * j] = f2lo(v[4 * i + j]);
         f[2 * j + 1] = f2hi(v[4 * i + j]);
       }
-      if (c < a.d) E::store(static_cast<Raw*>(base) + r * a.d + c, E::pack(f));
+      Raw* row = static_cast<Raw*>(base) + r * a.d;
+      if constexpr (Q == 1) {
+        if (at(i, 0) < a.d) E::store(row + at(i, 0), E::pack(f));
+      } else {
+        const auto v8 = E::pack(f);
+        if (at(i, 0) < a.d) *reinterpret_cast<float4*>(row + at(i, 0)) = v8.a;
+        if (at(i, 1) < a.d) *reinterpret_cast<float4*>(row + at(i, 1)) = v8.b;
+      }
     }
   };
   int stage = 0, buf = 0;
   for (; r < a.rows; r += step) {
-    typename E::Vec8 wp[VPT], wg[VPT], wn[VPT];   // read (from L1 after the first row) ahead of the reductions
+    typename E::Vec8 wp[V], wg[V], wn[V];   // read (from L1 after the first row) ahead of the reductions
     if (a.gamma_post) load_w(a.gamma_post, 0, wp);
     if (a.gate) load_w(a.gate, (r / a.rows_per_gate) * a.d, wg);
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     uint64_t v[NP], ss = 0ull;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
+    for (int i = 0; i < V; ++i) {
       uint64_t p[4];
       Pairs<DT>::get(slot(stage, 0, i * Q), THREADS, p);
 #pragma unroll
@@ -344,7 +357,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, DT == NVFP4B200_F32 ? (
     if (a.gamma_pre) load_w(a.gamma_pre, 0, wn);
     ss = 0ull;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
+    for (int i = 0; i < V; ++i) {
       uint64_t x[4];
       Pairs<DT>::get(slot(stage, 1, i * Q), THREADS, x);
 #pragma unroll
@@ -382,7 +395,7 @@ __global__ void __launch_bounds__(TPR, 1024 / TPR) sandwich_fwd_odd_kernel(const
   extern __shared__ __align__(16) uint8_t odd_ring[];   // [stages][2][slot]
   __shared__ float red[4][TPR / 32];
   __shared__ __align__(8) uint64_t full[STAGES];
-  __shared__ int gave_up;
+  __shared__ int gave_up;   // the row whose copy did not arrive in time
   const int t = threadIdx.x;
   const float inv_d = 1.0f / (float)a.d;
   const int row_bytes = a.d * (int)sizeof(Raw), slot = ((row_bytes + 15) & ~15) + 16;
@@ -399,7 +412,7 @@ __global__ void __launch_bounds__(TPR, 1024 / TPR) sandwich_fwd_odd_kernel(const
     bulk::copy(dst + slot, static_cast<const uint8_t*>(a.x) + r * a.ldx * (int64_t)sizeof(Raw) - ox, nx, &full[stage]);
   };
   if (t == 0) {
-    gave_up = 0;
+    gave_up = INT_MAX;
     bulk::init(full, STAGES);
   }
   __syncthreads();
@@ -426,7 +439,7 @@ __global__ void __launch_bounds__(TPR, 1024 / TPR) sandwich_fwd_odd_kernel(const
       if (a.gate) times(a.gate, group * a.d, w);
     }
     const bool staged = r < safe;
-    if (staged && !bulk::wait(&full[stage], parity)) gave_up = 1;
+    if (staged && !bulk::wait(&full[stage], parity)) gave_up = (int)(r - r0);
     const uint8_t* src = odd_ring + (size_t)stage * 2 * slot;
     const Raw* rb = staged ? reinterpret_cast<const Raw*>(src + skew(r, a.ldb)) : static_cast<const Raw*>(a.b) + r * a.ldb;
     const Raw* rx = staged ? reinterpret_cast<const Raw*>(src + slot + skew(r, a.ldx)) : static_cast<const Raw*>(a.x) + r * a.ldx;
@@ -448,7 +461,7 @@ __global__ void __launch_bounds__(TPR, 1024 / TPR) sandwich_fwd_odd_kernel(const
     const float inv_b = rsqrtf(row_sum<TPR>(ss, red[buf], 0) * inv_d + a.eps);
     // past the sum's barrier every thread has read the row: its place is refilled
     if (t == 0) fetch(r + a.stages, stage);
-    if (gave_up) break;
+    if (gave_up <= r - r0) break;
     ss = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -470,7 +483,7 @@ __global__ void __launch_bounds__(TPR, 1024 / TPR) sandwich_fwd_odd_kernel(const
       parity ^= 1u;
     }
   }
-  if (gave_up && t == 0) {
+  if (gave_up != INT_MAX && t == 0) {
     // a copy did not arrive in time: report it, and leave no copy in flight behind
     atomicExch(&g_norm_error, NVFP4B200_ERR_TIMEOUT);
     for (int st = 0; st < a.stages; ++st) bulk::wait(&full[st], parity ^ (st < stage ? 1u : 0u));
@@ -634,7 +647,10 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
 
 constexpr int BWD_STAGES = 3;   // rows of the ring, at most
 
-// One 8-element vector per thread: TPR threads cover d <= 8 * TPR columns.
+// Eight elements per thread: TPR threads cover d <= 8 * TPR columns.  In fp32
+// they are two pieces of four, a half of the row apart, so that neighbouring
+// lanes' 16 bytes are neighbours (8192 x 4096: 186 us with the pieces side by side, 170
+// so; 4096 x 8192 190 and 144).
 // ODD: rows that do not start on 16-byte boundaries (widths that are no
 // multiple of 8, say).  The bulk copies take each row's window of whole
 // 16-byte pieces, a thread's eight columns are TPR apart and are read and
@@ -645,7 +661,13 @@ constexpr int BWD_STAGES = 3;   // rows of the ring, at most
 // been brought to L2, and S is handed over at its end; the sum of gate * S is
 // kept beside the other column sums.  (With gate, gamma_post and that sum in
 // registers 16 warps share an SM: 316 us at 16000 x 4096 with a gate per row, 246 so.)
-template <int DT, int TPR, bool PRE, bool ODD, bool MULTI>
+// SPLIT: rows of more than 8192 columns, which no SM's shared memory holds
+// together with their column sums.  The two CTAs of a cluster take half the
+// columns each; every warp sends its parts of the row's sums to the other CTA,
+// on a barrier that counts their bytes.  (With the cluster's own barrier in
+// every row 250 us at 4096 x 16384 bf16 with the next
+// norm, 229 so; 1016 with rows read straight from global memory.)
+template <int DT, int TPR, bool PRE, bool ODD, bool MULTI, bool SPLIT>
 __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1024 / TPR)
     sandwich_bwd_staged_kernel(const BwdArgs a, int64_t parts_per_group) {
   using E = Elem<DT>;
@@ -653,17 +675,24 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
   constexpr int NT = PRE ? 4 : 2;                 // tensors: dy, b [, dn, y]
   constexpr int NP = 4;                           // packed pairs per thread
   const int ST = a.stages;
-  constexpr int W4 = (TPR / 32 + 3) / 4;          // 16-byte words of one sum's warp parts
+  constexpr int W4 = (TPR / 32 + 3) / 4 * (SPLIT ? 2 : 1);   // 16-byte words of one sum's warp parts
   extern __shared__ __align__(16) uint8_t row_ring[];   // [ST][NT][d], then the column sums
   __shared__ __align__(16) float red[2][3][4 * W4];
-  __shared__ __align__(8) uint64_t full[BWD_STAGES];
-  __shared__ int gave_up;
+  __shared__ __align__(8) uint64_t full[BWD_STAGES], theirs[SPLIT ? 2 : 1];
+  __shared__ int gave_up;   // the row whose copy did not arrive in time
   const int t = threadIdx.x;
   const float inv_d = 1.0f / (float)a.d;
-  const int row_bytes = a.d * (int)sizeof(Raw);
+  // this CTA's columns: [c0, c0 + d) of the row
+  const int rank = SPLIT ? (int)blockIdx.x & 1 : 0, half = SPLIT ? ((a.d + 1) / 2 + 7) & ~7 : a.d;
+  const int c0 = rank * half, d = SPLIT ? min(half, a.d - c0) : a.d;
+  const int64_t unit = SPLIT ? blockIdx.x >> 1 : blockIdx.x, units = SPLIT ? gridDim.x >> 1 : gridDim.x;
+  auto pair_barrier = []() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  };
+  const int row_bytes = d * (int)sizeof(Raw);
   const int slot = ODD ? ((row_bytes + 15) & ~15) + 16 : row_bytes;   // of one tensor's row in the ring
-  const int64_t g = blockIdx.x / parts_per_group, p = blockIdx.x % parts_per_group;
-  const int64_t r0 = MULTI ? (int64_t)blockIdx.x * a.rows_per_cta : g * a.rows_per_gate + p * a.rows_per_cta;
+  const int64_t g = unit / parts_per_group, p = unit % parts_per_group;
+  const int64_t r0 = MULTI ? unit * a.rows_per_cta : g * a.rows_per_gate + p * a.rows_per_cta;
   const int rows = (int)(imin64(r0 + a.rows_per_cta, MULTI ? a.rows : (g + 1) * a.rows_per_gate) - r0);
 
   const int staged = (int)imin64(rows, ODD ? (a.safe_rows > r0 ? a.safe_rows - r0 : 0) : rows);
@@ -684,16 +713,18 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
     for (int q = 0; q < NT; ++q)
       if (base[q]) {
         const int off = skew(r, ld[q]);
-        bulk::copy(dst + q * slot, static_cast<const uint8_t*>(base[q]) + r * ld[q] * (int64_t)sizeof(Raw) - off,
+        bulk::copy(dst + q * slot, static_cast<const uint8_t*>(base[q]) + (r * ld[q] + c0) * (int64_t)sizeof(Raw) - off,
                    (uint32_t)(ODD ? (off + row_bytes + 15) & ~15 : row_bytes), &full[stage]);
       }
   };
   if (t < 3 * 4 * W4 * 2) (&red[0][0][0])[t] = 0.0f;   // warp parts past the last stay zero
   if (t == 0) {
-    gave_up = 0;
+    gave_up = INT_MAX;
     bulk::init(full, ST);
+    if (SPLIT) bulk::init(theirs, 2);
   }
-  __syncthreads();
+  if (SPLIT) pair_barrier();
+  else __syncthreads();
   if (t == 0)
     for (int st = 0; st < ST; ++st) fetch(st, st);
 
@@ -701,15 +732,23 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
   ulonglong2* sums_at = reinterpret_cast<ulonglong2*>(row_ring + (size_t)ST * NT * slot) + t;
 #pragma unroll
   for (int j = 0; j < NT + (MULTI ? 2 : 0); ++j) sums_at[j * TPR] = make_ulonglong2(0ull, 0ull);
-  const int c = ODD ? t : 8 * t;   // the thread's first column; the others follow, or (ODD) are TPR apart
-  const bool in = c < a.d;
+  // the thread's first column; the others follow, or are TPR apart (ODD), or half h of them starts at col(h)
+  constexpr bool WIDE = !ODD && DT == NVFP4B200_F32;
+  const int c = ODD ? t : WIDE ? 4 * t : 8 * t;
+  const bool in = c < d;
+  auto col = [&](int h) { return WIDE ? 4 * (h * TPR + t) : c + 4 * h; };
   auto weights = [&](const void* p, int64_t off, uint64_t (&w)[NP]) {
     float f[8];
     if (ODD) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = c + j * TPR < a.d ? E::get(static_cast<const Raw*>(p) + off + c + j * TPR) : 0.0f;
+      for (int j = 0; j < 8; ++j) f[j] = c + j * TPR < d ? E::get(static_cast<const Raw*>(p) + off + c0 + c + j * TPR) : 0.0f;
+    } else if constexpr (WIDE) {
+      auto v = E::zero();
+      if (col(0) < d) v.a = __ldg(reinterpret_cast<const float4*>(static_cast<const Raw*>(p) + off + c0 + col(0)));
+      if (col(1) < d) v.b = __ldg(reinterpret_cast<const float4*>(static_cast<const Raw*>(p) + off + c0 + col(1)));
+      E::unpack(v, f);
     } else {
-      E::unpack(in ? E::load(static_cast<const Raw*>(p) + off + c) : E::zero(), f);
+      E::unpack(in ? E::load(static_cast<const Raw*>(p) + off + c0 + c) : E::zero(), f);
     }
 #pragma unroll
     for (int j = 0; j < NP; ++j) w[j] = f2mul(w[j], f2pack(f[2 * j], f[2 * j + 1]));
@@ -731,10 +770,11 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
       const float f[4] = {f2lo(lo), f2hi(lo), f2lo(hi), f2hi(hi)};
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (c + (4 * h + j) * TPR < a.d) row[c + (4 * h + j) * TPR] = f[j];
+        if (c + (4 * h + j) * TPR < d) row[c0 + c + (4 * h + j) * TPR] = f[j];
       return;
     }
-    float* out = row + c + 4 * h;   // d % 8 == 0: 16-byte aligned where the first row is
+    if (WIDE && col(h) >= d) return;
+    float* out = row + c0 + col(h);   // d % 8 == 0: 16-byte aligned where the first row is
     if (wide) {
       *reinterpret_cast<ulonglong2*>(out) = make_ulonglong2(lo, hi);
     } else {
@@ -743,7 +783,7 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
   };
   const bool aligned_dgate = MULTI && (reinterpret_cast<uintptr_t>(a.dgate) & 15) == 0;
 
-  Raw *dx = static_cast<Raw*>(a.dx) + r0 * a.d, *db = static_cast<Raw*>(a.db) + r0 * a.d;
+  Raw *dx = static_cast<Raw*>(a.dx) + r0 * a.d + c0, *db = static_cast<Raw*>(a.db) + r0 * a.d + c0;
   const float *ib = a.inv_b + r0, *iy = PRE ? a.inv_y + r0 : nullptr;
   float next_b = __ldg(ib), next_y = PRE ? __ldg(iy) : 0.0f;
   int stage = 0, buf = 0;
@@ -763,26 +803,28 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
         if (a.gamma_post) weights(a.gamma_post, 0, W);
         weights(a.gate, group * a.d, W);
         if (i + left < rows && in && t % (128 / (ODD ? (int)sizeof(Raw) : 16)) == 0)
-          for (int j = 0; j < (ODD ? 8 : 1); ++j)
-            if (c + j * TPR < a.d)
-              asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const Raw*>(a.gate) + (group + 1) * a.d + c + j * TPR));
+          for (int j = 0; j < (ODD ? 8 : WIDE ? 2 : 1); ++j)
+            if (ODD ? c + j * TPR < d : col(j) < d)
+              asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const Raw*>(a.gate) + (group + 1) * a.d + c0 + (ODD ? c + j * TPR : col(j))));
       }
       --left;
     }
-    if (i < staged && !bulk::wait(&full[stage], parity)) gave_up = 1;
+    if (i < staged && !bulk::wait(&full[stage], parity)) gave_up = i;
     const uint8_t* src = row_ring + (size_t)stage * NT * slot;
     auto get = [&](int tensor, int c, uint64_t (&o)[4]) {
       if (!ODD) {
-        Pairs<DT>::get(reinterpret_cast<const uint4*>(src + tensor * slot + c * (int)sizeof(Raw)), 1, o);
+        const uint4* at = reinterpret_cast<const uint4*>(src + tensor * slot + c * (int)sizeof(Raw));
+        Pairs<DT>::get(at, !WIDE || col(1) < d ? (WIDE ? TPR : 1) : 0, o);
+        if (WIDE && col(1) >= d) o[2] = o[3] = 0ull;
         return;
       }
       const void* base = tensor == 0 ? a.dy : tensor == 1 ? a.b : tensor == 2 ? a.dn : a.y;
       const int64_t at = (r0 + i) * (tensor == 0 ? a.ld_dy : tensor == 1 ? a.ldb : tensor == 2 ? a.ld_dn : a.ldy);
       const Raw* row = i < staged ? reinterpret_cast<const Raw*>(src + tensor * slot + (int)((uint64_t)at * sizeof(Raw) & 15))
-                                  : static_cast<const Raw*>(base) + at;
+                                  : static_cast<const Raw*>(base) + at + c0;
       float f[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = c + j * TPR < a.d ? E::value(row[c + j * TPR]) : 0.0f;
+      for (int j = 0; j < 8; ++j) f[j] = c + j * TPR < d ? E::value(row[c + j * TPR]) : 0.0f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] = f2pack(f[2 * j], f[2 * j + 1]);
     };
@@ -829,11 +871,25 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
     for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
       for (int k = 0; k < (PRE ? 3 : 1); ++k) sums[k] += __shfl_xor_sync(0xffffffffu, sums[k], o);
-    if ((t & 31) == 0) {
+    if (SPLIT) {   // three lanes, a sum each
+      if ((t & 31) < (PRE ? 3 : 1)) {
+        const int k = t & 31;
+        const float v = k == 0 ? sums[0] : k == 1 ? sums[1] : sums[2];
+        float* at = &red[buf][k][rank * (TPR / 32) + (t >> 5)];
+        *at = v;
+        asm volatile(
+            "{\n\t.reg .b32 a, b;\n\tmapa.shared::cluster.u32 a, %0, %2;\n\tmapa.shared::cluster.u32 b, %1, %2;\n\t"
+            "st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [a], %3, [b];\n\t}" ::"r"(bulk::addr(at)),
+            "r"(bulk::addr(&theirs[buf])), "r"(rank ^ 1), "r"(__float_as_uint(v))
+            : "memory");
+      }
+      if (t == 0) bulk::expect(&theirs[buf], (PRE ? 3 : 1) * (TPR / 32) * 4);
+    } else if ((t & 31) == 0) {
 #pragma unroll
       for (int k = 0; k < (PRE ? 3 : 1); ++k) red[buf][k][t >> 5] = sums[k];
     }
     __syncthreads();
+    if (SPLIT && !bulk::wait<true>(&theirs[buf], (uint32_t)(i >> 1) & 1u)) gave_up = i;
     if (t == 0) fetch(i + ST, stage);
     if (TPR > 32) {
 #pragma unroll
@@ -848,7 +904,7 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
       }
     }
     buf ^= 1;
-    if (gave_up) break;   // set before the barrier: every thread sees it
+    if (gave_up <= i) break;   // set before the barrier: every thread sees it
     const float m1 = PRE ? sums[1] * inv_d : 0.0f;
     const float m2 = (PRE ? fmaf(-inv_y * m1, sums[2], sums[0]) : sums[0]) * inv_d;
     const ulonglong2 s0 = sums_at[0], s1 = sums_at[TPR];
@@ -858,10 +914,10 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
     for (int j = 0; j < NP; ++j) {
       const uint64_t tt = PRE ? f2fma(yh[j], f2two(-inv_y * m1), t0[j]) : t0[j];
       S[j] = f2fma(tt, bh[j], S[j]);
-      const uint64_t d = f2mul(f2fma(bh[j], f2two(-m2), f2mul(W[j], tt)), f2two(inv_b));
+      const uint64_t e_b = f2mul(f2fma(bh[j], f2two(-m2), f2mul(W[j], tt)), f2two(inv_b));
       const uint64_t e = f2mul(tt, f2two(a.alpha));
       dxv[2 * j] = f2lo(e); dxv[2 * j + 1] = f2hi(e);
-      dbv[2 * j] = f2lo(d); dbv[2 * j + 1] = f2hi(d);
+      dbv[2 * j] = f2lo(e_b); dbv[2 * j + 1] = f2hi(e_b);
     }
     if constexpr (MULTI) {
       if (left == 0) {   // and ends
@@ -891,10 +947,20 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
     if (ODD) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (c + j * TPR < a.d) {
+        if (c + j * TPR < d) {
           dx[c + j * TPR] = E::bits(dxv[j]);
           db[c + j * TPR] = E::bits(dbv[j]);
         }
+    } else if constexpr (WIDE) {
+      const auto px = E::pack(dxv), pb = E::pack(dbv);
+      if (col(0) < d) {
+        *reinterpret_cast<float4*>(dx + col(0)) = px.a;
+        *reinterpret_cast<float4*>(db + col(0)) = pb.a;
+      }
+      if (col(1) < d) {
+        *reinterpret_cast<float4*>(dx + col(1)) = px.b;
+        *reinterpret_cast<float4*>(db + col(1)) = pb.b;
+      }
     } else if (in) {
       E::store(dx + c, E::pack(dxv));
       E::store(db + c, E::pack(dbv));
@@ -906,11 +972,13 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
       parity ^= 1u;
     }
   }
-  if (gave_up && t == 0) {
+  if (gave_up != INT_MAX && t == 0) {
     // a copy did not arrive in time: report it, and leave no copy in flight behind
     atomicExch(&g_norm_error, NVFP4B200_ERR_TIMEOUT);
     for (int st = 0; st < ST; ++st) bulk::wait(&full[st], parity ^ (st < stage ? 1u : 0u));
   }
+
+  if (SPLIT) pair_barrier();   // no CTA leaves while the other may still send to it
 
   // partial column sums: s * S, gate * s * S and dgamma_pre
   if (!in) return;
@@ -922,16 +990,16 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
   for (int h = 0; h < 2; ++h) {
     if constexpr (MULTI) {
       const ulonglong2 v = sums_at[(NT + h) * TPR];
-      put(a.part + (int64_t)blockIdx.x * a.d, a.ws16, h, v.x, v.y);
+      put(a.part + unit * a.d, a.ws16, h, v.x, v.y);
     } else {
       const ulonglong2 sv = sums_at[h * TPR];
       const uint64_t lo = f2mul(sv.x, f2two(a.s)), hi = f2mul(sv.y, f2two(a.s));
-      if (a.gate) put(a.part_gate + (int64_t)blockIdx.x * a.d, a.ws16, h, lo, hi);
-      put(a.part + (int64_t)blockIdx.x * a.d, a.ws16, h, f2mul(lo, gate[2 * h]), f2mul(hi, gate[2 * h + 1]));
+      if (a.gate) put(a.part_gate + unit * a.d, a.ws16, h, lo, hi);
+      put(a.part + unit * a.d, a.ws16, h, f2mul(lo, gate[2 * h]), f2mul(hi, gate[2 * h + 1]));
     }
     if (PRE) {
       const ulonglong2 pv = sums_at[(2 + h) * TPR];
-      put(a.part + ((int64_t)gridDim.x + blockIdx.x) * a.d, a.ws16, h, pv.x, pv.y);
+      put(a.part + (units + unit) * a.d, a.ws16, h, pv.x, pv.y);
     }
   }
 }
@@ -1024,7 +1092,8 @@ static Split split_rows(int64_t rows, int64_t groups, int64_t d, int sms) {
   // more, smaller CTAs
   int64_t tpr = 32;
   while (tpr * CPT < d) tpr *= 2;
-  const int64_t per = rows / groups, target = std::max<int64_t>(1, 512 / tpr) * sms;
+  // rows of more than 8192 columns take two SMs
+  const int64_t per = rows / groups, target = tpr > 512 ? std::max(1, sms / 2) : 512 / tpr * sms;
   // A CTA takes a part of a group's rows, or whole groups.  The cost is counted in
   // rows: waves of CTAs times the rows of one and some more for its start.  (As many
   // whole groups, or parts of one, as fill one wave: 16000 x 4096 with 160 gates 242
@@ -1092,15 +1161,19 @@ int nvfp4b200_sandwich_norm(const void* b, const void* x, const void* gamma_post
       constexpr int T = decltype(tpr)::value, THREADS = T < 256 ? 256 : T, GROUPS = THREADS / T;
       constexpr int DT = decltype(dt)::value;
       const int64_t want = ceil_div(rows, GROUPS);
-      // the staged kernel where its ring fits: 195 -> 176 us at 16384 x 8192 bf16 with the next norm
-      constexpr int smem = norm::STAGES * 2 * THREADS * norm::CPT * norm::dtype_size<DT>();
+      // the staged kernel where its ring fits: 195 -> 168 us at 16384 x 8192 bf16 with the next norm.
+      // fp32: 8 columns a thread, so that 32 warps share an SM (8192 x 4096: 88 us, 141 with 16
+      // columns; bf16 at 16384 x 4096 93 with 16 columns, 109 with 8)
+      constexpr int V = DT == NVFP4B200_F32 && T <= 512 ? 1 : norm::VPT, TV = T * norm::VPT / V;
+      constexpr int THREADS_V = TV < 256 ? 256 : TV;
+      constexpr int smem = norm::STAGES * 2 * THREADS_V * 8 * V * norm::dtype_size<DT>();
       if constexpr (decltype(v)::value && smem <= norm::MAX_SMEM) {
-        auto* fn = norm::sandwich_fwd_staged_kernel<DT, T>;
+        auto* fn = norm::sandwich_fwd_staged_kernel<DT, TV, V>;
         if (smem > 32 * 1024 &&   // with the static arrays, past the default limit
             cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
           return (int)NVFP4B200_ERR_CUDA;
-        const int per_sm = std::max(1, std::min(228 * 1024 / (smem + 2048), T < 512 ? 4 : 1024 / T));
-        fn<<<(unsigned)std::min<int64_t>(want, (int64_t)sm_count_current() * per_sm), THREADS, smem, st>>>(a);
+        const int per_sm = std::max(1, std::min(228 * 1024 / (smem + 2048), TV < 512 ? 4 : 1024 / TV));
+        fn<<<(unsigned)std::min<int64_t>(ceil_div(rows, THREADS_V / TV), (int64_t)sm_count_current() * per_sm), THREADS_V, smem, st>>>(a);
         return launch_status();
       }
       if constexpr (!decltype(v)::value && T >= 64 && T <= 512) {
@@ -1184,13 +1257,14 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
       constexpr int T = decltype(tpr)::value, DT = decltype(dt)::value;
       // the staged kernel where a row fits: 346 -> 152 us at 16000 x 4096 bf16 with 8
       // gates and the next norm, 611 -> 246 with a gate per row
-      if constexpr (T <= 512) {
-        constexpr int T2 = 2 * T;
+      {
+        constexpr bool SPLIT = T > 512;
+        constexpr int T2 = SPLIT ? T : 2 * T;
         constexpr bool ODD = !decltype(v)::value;
         // two CTAs' worth of threads share an SM (fewer where one is that large), and
         // so its memory: as many ring rows as fit, up to 3 (2 with the next norm's
         // tensors); one row at least, alone on the SM if need be
-        const int width = (int)d * bytes, row = (dn ? 4 : 2) * (ODD ? (int)round_up(width, 16) + 16 : width);
+        const int width = (int)(SPLIT ? round_up(ceil_div(d, 2), 8) : d) * bytes, row = (dn ? 4 : 2) * (ODD ? (int)round_up(width, 16) + 16 : width);
         const bool multi = gate && sp.parts_per_group == 1;   // a CTA's rows are whole groups
         const int sums = ((dn ? 4 : 2) + (multi ? 2 : 0)) * 16 * T2;
         const int share = norm::smem_share(1024 / T2);
@@ -1200,14 +1274,32 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
         a.safe_rows = std::max<int64_t>(0, rows - 1 - 15 / (ld_min * bytes));
         const bool bases = aligned(b, 16) && (!dy || aligned(dy, 16)) && (!dn || (aligned(dn, 16) && aligned(y, 16)));
         if (smem <= norm::MAX_SMEM && (!ODD || bases)) {
-          auto* fn = multi ? (dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true, ODD, true>
-                                 : norm::sandwich_bwd_staged_kernel<DT, T2, false, ODD, true>)
-                           : (dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true, ODD, false>
-                                 : norm::sandwich_bwd_staged_kernel<DT, T2, false, ODD, false>);
+          auto* fn = multi ? (dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true, ODD, true, SPLIT>
+                                 : norm::sandwich_bwd_staged_kernel<DT, T2, false, ODD, true, SPLIT>)
+                           : (dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true, ODD, false, SPLIT>
+                                 : norm::sandwich_bwd_staged_kernel<DT, T2, false, ODD, false, SPLIT>);
           if (smem > 32 * 1024 &&   // with the static arrays, past the default limit
               cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
             return (int)NVFP4B200_ERR_CUDA;
-          fn<<<(unsigned)sp.ctas, T2, smem, st>>>(a, sp.parts_per_group);
+          if (!SPLIT) {
+            fn<<<(unsigned)sp.ctas, T2, smem, st>>>(a, sp.parts_per_group);
+            return launch_status();
+          }
+          cudaLaunchConfig_t cfg = {};
+          cfg.gridDim = dim3((unsigned)(2 * sp.ctas), 1, 1);
+          cfg.blockDim = dim3(T2, 1, 1);
+          cfg.dynamicSmemBytes = smem;
+          cfg.stream = st;
+          cudaLaunchAttribute pair;
+          pair.id = cudaLaunchAttributeClusterDimension;
+          pair.val.clusterDim.x = 2;
+          pair.val.clusterDim.y = pair.val.clusterDim.z = 1;
+          cfg.attrs = &pair;
+          cfg.numAttrs = 1;
+          if (cudaLaunchKernelEx(&cfg, fn, a, sp.parts_per_group) != cudaSuccess) {
+            cudaGetLastError();
+            return (int)NVFP4B200_ERR_LAUNCH;
+          }
           return launch_status();
         }
       }

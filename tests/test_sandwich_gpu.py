@@ -78,7 +78,8 @@ CASES = [  # t, d, groups, gamma_post, gamma_pre/pre
     (1, 1, 0, True, True), (1, 4096, 1, True, True), (5, 64, 5, True, True), (3, 333, 1, True, True),
     (16, 520, 4, False, True), (77, 1000, 7, True, False), (130, 2048, 1, True, True), (64, 4096, 16, True, True),
     (33, 5000, 0, True, True), (20, 8192, 2, True, True), (9, 16384, 3, True, True), (7, 16383, 1, True, True),
-    (2000, 96, 1000, True, True), (1200, 256, 2, True, True), (4099, 40, 1, True, True), (600, 512, 600, False, False)]
+    (2000, 96, 1000, True, True), (1200, 256, 2, True, True), (1500, 8200, 1, True, True), (700, 12296, 7, True, True),
+    (400, 16384, 0, True, False), (4099, 40, 1, True, True), (600, 512, 600, False, False)]
 
 
 @pytest.mark.parametrize("dtype", [BF, HF, FL])
@@ -146,7 +147,8 @@ def test_strides_and_misaligned(pkg):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF, FL])
-@pytest.mark.parametrize("t,d", [(1, 3), (2, 7), (9, 1), (500, 5), (300, 67), (1000, 1001), (401, 4097), (97, 8191), (700, 2050)])
+@pytest.mark.parametrize("t,d", [(1, 3), (2, 7), (9, 1), (500, 5), (300, 67), (1000, 1001), (401, 4097), (97, 8191), (700, 2050),
+                                 (500, 9001), (311, 16383), (2, 8193)])
 def test_widths_of_no_multiple(pkg, t, d, dtype):
     """Unaligned rows, many of them, the tensors ending with their storage: forward and
     backward against float64, and nothing read beside them (neighbours are NaN)."""
@@ -178,11 +180,11 @@ def test_widths_of_no_multiple(pkg, t, d, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, FL])
-@pytest.mark.parametrize("per,d", [(1, 4096), (1, 1001), (3, 1001), (2, 96), (7, 520), (1, 7), (5, 4104), (1, 8191), (40, 2048)])
+@pytest.mark.parametrize("per,d", [(1, 4096), (1, 1001), (3, 1001), (2, 96), (7, 520), (1, 7), (5, 4104), (1, 8191), (40, 2048), (1, 12288), (3, 16384), (2, 9001)])
 def test_many_gates(pkg, per, d, dtype):
     """More groups of rows than CTAs: a CTA walks several groups, and the last one fewer."""
     ops = pkg.ops
-    groups = (5000 if d < 100 else 1900 if d < 1100 else 701) // (1 if per < 8 else 4)
+    groups = (5000 if d < 100 else 1900 if d < 1100 else 701 if d < 8192 else 233) // (1 if per < 8 else 4)
     t = groups * per
     b, y, dy, dn = (rnd((t, d), i, dtype, s) for i, s in ((1, 2.0), (2, 1.0), (3, 0.1), (4, 0.1)))
     gp, gate, gn = rnd((d,), 5, dtype, 0.3) + 1, rnd((groups, d), 6, dtype), rnd((d,), 7, dtype, 0.3) + 1
