@@ -41,6 +41,9 @@ constexpr int MAX_SMEM = 225 * 1024;   // dynamic, of one CTA: 227 KB less the s
 // what n CTAs of an SM can each have: its 228 KB less 1 KB per CTA that the system takes and 1 KB of static arrays
 constexpr int smem_share(int n) { return n <= 1 ? MAX_SMEM : 228 * 1024 / n - 2048; }
 
+// Threads of a CTA of the forward: rows of TPR threads each, 256 threads or a little more.
+constexpr int threads_of(int tpr) { return (tpr < 256 ? (255 + tpr) / tpr : 1) * tpr; }
+
 template <int DT>
 constexpr int dtype_size() { return DT == NVFP4B200_F32 ? 4 : 2; }
 
@@ -183,9 +186,9 @@ struct FwdArgs {
 };
 
 template <int DT, bool VEC, int TPR>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) sandwich_fwd_kernel(const FwdArgs a) {
+__global__ void __launch_bounds__(threads_of(TPR)) sandwich_fwd_kernel(const FwdArgs a) {
   using Raw = typename Elem<DT>::Raw;
-  constexpr int GROUPS = TPR < 256 ? 256 / TPR : 1;
+  constexpr int GROUPS = threads_of(TPR) / TPR;
   __shared__ float red[4][GROUPS * (TPR / 32)];
   const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
   const Raw *B = static_cast<const Raw*>(a.b), *X = static_cast<const Raw*>(a.x);
@@ -247,13 +250,13 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) sandwich_fwd_kernel(con
 // reductions.  (The second sum is not folded into the first exchange: y's
 // square sum from those of its parts cancels where y is small.)
 template <int DT, int TPR, int V>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR < 512 ? 4 : 1024 / TPR)
+__global__ void __launch_bounds__(threads_of(TPR), 1024 / threads_of(TPR))
     sandwich_fwd_staged_kernel(const FwdArgs a) {
   using E = Elem<DT>;
   using Raw = typename E::Raw;
   constexpr int Q = (int)sizeof(Raw) * 8 / 16;
   constexpr int NP = 4 * V;
-  constexpr int THREADS = TPR < 256 ? 256 : TPR, GROUPS = THREADS / TPR;
+  constexpr int THREADS = threads_of(TPR), GROUPS = THREADS / TPR;
   extern __shared__ __align__(16) uint4 ring[];   // [STAGES][2][V * Q][THREADS]
   __shared__ float red[4][GROUPS * (TPR / 32)];
   const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
@@ -1059,14 +1062,17 @@ __global__ void __launch_bounds__(32 * FINISH_WARPS) sandwich_bwd_finish_kernel(
   }
 }
 
-template <typename F>
+// Threads per row, 16 columns each: the least of a few numbers of warps.  (With
+// powers of two alone 13107 x 5120 bf16 took 119 us in the forward and 240 in the
+// backward, 94 and 167 so; 43690 x 1536 129 and 166, 92 and 155.  160 gained nothing.)
+constexpr int WIDTHS[] = {32, 64, 96, 128, 256, 320, 384, 512, 1024};
+
+template <int I = 0, typename F>
 static int by_width(int d, F f) {
-  if (d <= 32 * CPT) return f(std::integral_constant<int, 32>());
-  if (d <= 64 * CPT) return f(std::integral_constant<int, 64>());
-  if (d <= 128 * CPT) return f(std::integral_constant<int, 128>());
-  if (d <= 256 * CPT) return f(std::integral_constant<int, 256>());
-  if (d <= 512 * CPT) return f(std::integral_constant<int, 512>());
-  return f(std::integral_constant<int, 1024>());
+  if constexpr (I + 1 < (int)(sizeof(WIDTHS) / sizeof(int))) {
+    if (d > WIDTHS[I] * CPT) return by_width<I + 1>(d, f);
+  }
+  return f(std::integral_constant<int, WIDTHS[I]>());
 }
 
 template <typename F>
@@ -1090,10 +1096,10 @@ constexpr int START_ROWS = 4;
 static Split split_rows(int64_t rows, int64_t groups, int64_t d, int sms) {
   // CTAs that run at a time: 1024 threads per SM, 8 columns each; narrow rows in
   // more, smaller CTAs
-  int64_t tpr = 32;
-  while (tpr * CPT < d) tpr *= 2;
+  int64_t tpr = 0;
+  by_width((int)d, [&](auto t) { tpr = t; return 0; });
   // rows of more than 8192 columns take two SMs
-  const int64_t per = rows / groups, target = tpr > 512 ? std::max(1, sms / 2) : 512 / tpr * sms;
+  const int64_t per = rows / groups, target = tpr > 512 ? std::max(1, sms / 2) : 1024 / (2 * tpr) * sms;
   // A CTA takes a part of a group's rows, or whole groups.  The cost is counted in
   // rows: waves of CTAs times the rows of one and some more for its start.  (As many
   // whole groups, or parts of one, as fill one wave: 16000 x 4096 with 160 gates 242
@@ -1158,21 +1164,21 @@ int nvfp4b200_sandwich_norm(const void* b, const void* x, const void* gamma_post
   cudaStream_t st = (cudaStream_t)stream;
   return norm::by_type(dtype, vec, [&](auto dt, auto v) {
     return norm::by_width((int)d, [&](auto tpr) {
-      constexpr int T = decltype(tpr)::value, THREADS = T < 256 ? 256 : T, GROUPS = THREADS / T;
+      constexpr int T = decltype(tpr)::value, THREADS = norm::threads_of(T), GROUPS = THREADS / T;
       constexpr int DT = decltype(dt)::value;
       const int64_t want = ceil_div(rows, GROUPS);
       // the staged kernel where its ring fits: 195 -> 168 us at 16384 x 8192 bf16 with the next norm.
       // fp32: 8 columns a thread, so that 32 warps share an SM (8192 x 4096: 88 us, 141 with 16
       // columns; bf16 at 16384 x 4096 93 with 16 columns, 109 with 8)
       constexpr int V = DT == NVFP4B200_F32 && T <= 512 ? 1 : norm::VPT, TV = T * norm::VPT / V;
-      constexpr int THREADS_V = TV < 256 ? 256 : TV;
+      constexpr int THREADS_V = norm::threads_of(TV);
       constexpr int smem = norm::STAGES * 2 * THREADS_V * 8 * V * norm::dtype_size<DT>();
       if constexpr (decltype(v)::value && smem <= norm::MAX_SMEM) {
         auto* fn = norm::sandwich_fwd_staged_kernel<DT, TV, V>;
         if (smem > 32 * 1024 &&   // with the static arrays, past the default limit
             cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
           return (int)NVFP4B200_ERR_CUDA;
-        const int per_sm = std::max(1, std::min(228 * 1024 / (smem + 2048), TV < 512 ? 4 : 1024 / TV));
+        const int per_sm = std::max(1, std::min(228 * 1024 / (smem + 2048), 1024 / THREADS_V));
         fn<<<(unsigned)std::min<int64_t>(ceil_div(rows, THREADS_V / TV), (int64_t)sm_count_current() * per_sm), THREADS_V, smem, st>>>(a);
         return launch_status();
       }

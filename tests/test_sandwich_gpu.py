@@ -79,7 +79,8 @@ CASES = [  # t, d, groups, gamma_post, gamma_pre/pre
     (16, 520, 4, False, True), (77, 1000, 7, True, False), (130, 2048, 1, True, True), (64, 4096, 16, True, True),
     (33, 5000, 0, True, True), (20, 8192, 2, True, True), (9, 16384, 3, True, True), (7, 16383, 1, True, True),
     (2000, 96, 1000, True, True), (1200, 256, 2, True, True), (1500, 8200, 1, True, True), (700, 12296, 7, True, True),
-    (400, 16384, 0, True, False), (4099, 40, 1, True, True), (600, 512, 600, False, False)]
+    (400, 16384, 0, True, False), (333, 1536, 3, True, True), (901, 2560, 1, True, True), (640, 5120, 1, True, True),
+    (320, 5888, 0, True, True), (77, 1480, 1, True, False), (50, 2488, 50, True, True), (4099, 40, 1, True, True), (600, 512, 600, False, False)]
 
 
 @pytest.mark.parametrize("dtype", [BF, HF, FL])
@@ -148,7 +149,7 @@ def test_strides_and_misaligned(pkg):
 
 @pytest.mark.parametrize("dtype", [BF, HF, FL])
 @pytest.mark.parametrize("t,d", [(1, 3), (2, 7), (9, 1), (500, 5), (300, 67), (1000, 1001), (401, 4097), (97, 8191), (700, 2050),
-                                 (500, 9001), (311, 16383), (2, 8193)])
+                                 (500, 9001), (311, 16383), (2, 8193), (450, 1501), (301, 5003), (290, 6001)])
 def test_widths_of_no_multiple(pkg, t, d, dtype):
     """Unaligned rows, many of them, the tensors ending with their storage: forward and
     backward against float64, and nothing read beside them (neighbours are NaN)."""
