@@ -690,6 +690,7 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
   const int c0 = rank * half, d = SPLIT ? min(half, a.d - c0) : a.d;
   const int64_t unit = SPLIT ? blockIdx.x >> 1 : blockIdx.x, units = SPLIT ? gridDim.x >> 1 : gridDim.x;
   auto pair_barrier = []() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   };
   const int row_bytes = d * (int)sizeof(Raw);
