@@ -1065,8 +1065,9 @@ __global__ void __launch_bounds__(32 * FINISH_WARPS) sandwich_bwd_finish_kernel(
 
 // Threads per row, 16 columns each: the least of a few numbers of warps.  (With
 // powers of two alone 13107 x 5120 bf16 took 119 us in the forward and 240 in the
-// backward, 94 and 167 so; 43690 x 1536 129 and 166, 92 and 155.  160 gained nothing.)
-constexpr int WIDTHS[] = {32, 64, 96, 128, 256, 320, 384, 512, 1024};
+// backward, 88 and 163 so; 43690 x 1536 129 and 166, 92 and 155; 26214 x 2560 125 and 198,
+// 122 and 154.)
+constexpr int WIDTHS[] = {32, 64, 96, 128, 160, 256, 320, 384, 512, 1024};
 
 template <int I = 0, typename F>
 static int by_width(int d, F f) {
