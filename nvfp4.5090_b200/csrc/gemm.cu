@@ -48,6 +48,7 @@
 // returns, so a broken pipeline cannot hang the GPU.  No TMA load uses
 // cluster multicast.
 #include "common.cuh"
+#include "sched_slots.h"
 
 #include <cuda.h>
 #include <algorithm>
@@ -97,7 +98,8 @@ static_assert(ACC1_COL + ACC_COLS <= SF_COL && SF_COL + SF_COLS <= TMEM_COLS, "T
 constexpr int TILE_RING = 4;
 // readers of every ring slot: leader MMA warp + 8 epilogue warps, peer producer + 8 epilogue warps
 constexpr int RING_READERS = 2 * (1 + EPI_WARPS);
-constexpr int SCHED_SLOTS = 256;                      // per-launch tile counters, used round robin
+constexpr int STREAM_SLOTS = 256, GRAPH_SLOTS = 8192;  // tile counters of streams and of captured launches
+constexpr int SCHED_SLOTS = STREAM_SLOTS + GRAPH_SLOTS;
 constexpr int NUM_BARS = 2 * STAGES + 3 + EPI_WARPS + 2 * TILE_RING;  // + ring full / empty
 constexpr int BAR_BYTES = 512;                        // mbarriers + TMEM address slot + abort flag + tile ring
 static_assert(NUM_BARS * 8 + 8 + 4 * TILE_RING <= BAR_BYTES, "barrier area");
@@ -145,14 +147,15 @@ struct Params {
   int stages;                // pipeline stages in use (STAGES, or DSW_STAGES with dswiglu)
   int out_bytes;             // epilogue staging bytes (OUT_BYTES or DSW_OUT_BYTES)
   int mx;                    // MXFP4 operands: 1x32 blocks, UE8M0 scales (kind::mxf4)
-  int sched_slot;            // this launch's tile counter: g_tile_sched[sched_slot]
+  int sched_slot;            // this launch's tile counter: g_tile_sched[sched_slot]; -1: a fixed walk
 };
 
-// Per-launch tile counters: [0] tiles claimed beyond the first wave, [1]
-// clusters that have finished claiming.  The last cluster to finish resets
-// both to zero, so a slot is clean for the launch that reuses it (launches
-// take slots round robin).  Every wait in the kernel is bounded, so even a
-// launch that gives up reaches the reset.
+// Tile counters: [0] tiles claimed beyond the first wave, [1] clusters that
+// have finished claiming.  The last cluster to finish resets both to zero, so
+// a slot is clean for the launch that takes it next; which launch has which
+// slot, and that no two that run at once have the same, is sched_slots.h.
+// Every wait in the kernel is bounded, so even a launch that gives up reaches
+// the reset.  Without a slot a cluster takes every num_clusters-th tile.
 __device__ uint32_t g_tile_sched[SCHED_SLOTS][2];
 
 // ---------------------------------------------------------------------------
@@ -570,7 +573,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     uint32_t phase = 0;
     uint32_t armed = 0, armed_parity = 0;  // leader: stages whose barrier expects bytes, and the phase armed
     bool ok = true;
-    uint32_t* sched = g_tile_sched[p.sched_slot];
+    uint32_t* sched = p.sched_slot < 0 ? nullptr : g_tile_sched[p.sched_slot];
     int tile = cluster_id, next = -1;
     for (int i = 0; ok; ++i) {
       if (leader) {
@@ -589,11 +592,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
         __syncwarp();
         if (tile < 0) break;
         // claim the tile after this one now: the atomic's latency hides behind this tile's loads
-        if (lane == 0) {
-          const uint32_t c = atomicAdd(&sched[0], 1u);
-          next = c < (uint32_t)(total_tiles - num_clusters) ? num_clusters + (int)c : -1;
+        if (sched) {
+          if (lane == 0) {
+            const uint32_t c = atomicAdd(&sched[0], 1u);
+            next = c < (uint32_t)(total_tiles - num_clusters) ? num_clusters + (int)c : -1;
+          }
+          next = __shfl_sync(0xffffffffu, next, 0);
+        } else {
+          next = tile < total_tiles - num_clusters ? tile + num_clusters : -1;
         }
-        next = __shfl_sync(0xffffffffu, next, 0);
       } else {
         if (!ring_read(i, tile)) {
           ok = false;
@@ -632,7 +639,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
       }
       tile = next;
     }
-    if (leader && lane == 0) {
+    if (leader && lane == 0 && sched) {
       // this cluster claims no more tiles; the last cluster to get here resets the counters
       if (atomicAdd(&sched[1], 1u) == (uint32_t)num_clusters - 1u) {
         atomicExch(&sched[0], 0u);
@@ -1286,6 +1293,55 @@ struct DswigluIn {
   float* g_out;
 };
 
+using Slots = SchedSlots<STREAM_SLOTS, GRAPH_SLOTS>;
+
+static Slots& slots_of(int dev) {
+  static Slots* all = new Slots[64];   // never freed: graphs may go after static objects have
+  return all[dev & 63];
+}
+
+// A captured launch's counter goes back with the last graph that holds it.
+static void CUDART_CB give_back_slot(void* p) {
+  const uintptr_t v = reinterpret_cast<uintptr_t>(p);
+  slots_of((int)(v & 63)).give_back((int)(v >> 6));
+}
+
+// The counter of a launch on `stream`, -1 when none is to be had.
+static int take_slot(cudaStream_t stream) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  cudaGraph_t graph = nullptr;
+  if (cudaStreamGetCaptureInfo(stream, &status, nullptr, &graph) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  if (status == cudaStreamCaptureStatusNone) {
+    unsigned long long id = 0;
+    if (cudaStreamGetId(stream, &id) != cudaSuccess) {
+      cudaGetLastError();
+      return -1;
+    }
+    return slots_of(dev).of_stream(id);
+  }
+  if (status != cudaStreamCaptureStatusActive || !graph) return -1;
+  const int slot = slots_of(dev).take();
+  if (slot < 0) return -1;
+  cudaUserObject_t obj;
+  void* payload = reinterpret_cast<void*>(((uintptr_t)slot << 6) | (uintptr_t)dev);
+  if (cudaUserObjectCreate(&obj, payload, give_back_slot, 1, cudaUserObjectNoDestructorSync) != cudaSuccess) {
+    cudaGetLastError();
+    slots_of(dev).give_back(slot);
+    return -1;
+  }
+  if (cudaGraphRetainUserObject(graph, obj, 1, cudaGraphUserObjectMove) != cudaSuccess) {
+    cudaGetLastError();
+    cudaUserObjectRelease(obj, 1);   // gives the slot back
+    return -1;
+  }
+  return slot;
+}
+
 static int run(const void* a, const void* b, const void* sfa, const void* sfb, const float* scale_a,
                const float* scale_b, const void* bias, const void* residual, void* d, int d_dtype, int accumulate,
                int epilogue, int64_t m, int64_t n, int64_t k, int64_t ldd, cudaStream_t stream,
@@ -1367,12 +1423,7 @@ static int run(const void* a, const void* b, const void* sfa, const void* sfb, c
   const int max_sms = g_gemm_max_sms.load(std::memory_order_relaxed);
   if (max_sms > 0) cap = std::max(1, std::min(cap, max_sms / 2));
   const int clusters = (int)std::min<int64_t>(tiles, cap);
-  {
-    static std::atomic<uint32_t> seq[64];
-    int dev = 0;
-    cudaGetDevice(&dev);
-    p.sched_slot = (int)(seq[dev & 63].fetch_add(1u, std::memory_order_relaxed) % SCHED_SLOTS);
-  }
+  p.sched_slot = tiles > clusters ? take_slot(stream) : -1;   // one tile each: nothing to claim
   if (cudaFuncSetAttribute(nvfp4_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) !=
       cudaSuccess)
     return NVFP4B200_ERR_CUDA;
@@ -1410,8 +1461,10 @@ int nvfp4b200_get_device_error(int* out) {
     if (*out == 0) *out = e;
   }
   if (*out != 0) {   // a launch gave up: make sure no tile counter is left dirty (the device is idle here)
-    static const uint32_t zeros[gemm::SCHED_SLOTS][2] = {};
-    if (cudaMemcpyToSymbol(gemm::g_tile_sched, zeros, sizeof(zeros)) != cudaSuccess) return NVFP4B200_ERR_CUDA;
+    void* counters = nullptr;
+    if (cudaGetSymbolAddress(&counters, gemm::g_tile_sched) != cudaSuccess ||
+        cudaMemset(counters, 0, sizeof(gemm::g_tile_sched)) != cudaSuccess)
+      return NVFP4B200_ERR_CUDA;
   }
   return NVFP4B200_OK;
 }
