@@ -25,7 +25,7 @@ BINDING_NAME = "_nvfp4b200_torch"
 BINDING_PATH = os.path.join(LIB_DIR, BINDING_NAME + ".so")
 SOURCES = ["quant.cu", "gemm.cu", "train.cu", "noalloc.cu", "mx.cu", "mxlin.cu", "clip.cu", "norm.cu"]
 HEADERS = [os.path.join(CSRC, "common.cuh"), os.path.join(CSRC, "vec.cuh"), os.path.join(CSRC, "bulk.cuh"), os.path.join(CSRC, "mx.cuh"),
-           os.path.join(CSRC, "sched_slots.h"), os.path.join(REPO_DIR, "include", "nvfp4_b200.h")]
+           os.path.join(CSRC, "sched_slots.h"), os.path.join(CSRC, "row_stop.h"), os.path.join(REPO_DIR, "include", "nvfp4_b200.h")]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"] + ARCH
 

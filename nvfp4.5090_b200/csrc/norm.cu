@@ -25,6 +25,7 @@
 //
 // Bound: HBM, one read of each input and one write of each output.
 #include "bulk.cuh"
+#include "row_stop.h"
 #include "vec.cuh"
 
 #include <algorithm>
@@ -649,6 +650,7 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
 // 16 warps did, and waited for one another's barriers (147 us against 134 at 16000 x 4096).
 
 constexpr int BWD_STAGES = 3;   // rows of the ring, at most
+constexpr long long SETTLE_CYCLES = 1000000;   // about 0.5 ms: far longer than a store between two CTAs takes
 
 // Eight elements per thread: TPR threads cover d <= 8 * TPR columns.  In fp32
 // they are two pieces of four, a half of the row apart, so that neighbouring
@@ -682,7 +684,7 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
   extern __shared__ __align__(16) uint8_t row_ring[];   // [ST][NT][d], then the column sums
   __shared__ __align__(16) float red[2][3][4 * W4];
   __shared__ __align__(8) uint64_t full[BWD_STAGES], theirs[SPLIT ? 2 : 1];
-  __shared__ int gave_up;   // the row whose copy did not arrive in time
+  __shared__ int stop;   // row_stop.h: set where a wait ran out
   const int t = threadIdx.x;
   const float inv_d = 1.0f / (float)a.d;
   // this CTA's columns: [c0, c0 + d) of the row
@@ -723,7 +725,7 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
   };
   if (t < 3 * 4 * W4 * 2) (&red[0][0][0])[t] = 0.0f;   // warp parts past the last stay zero
   if (t == 0) {
-    gave_up = INT_MAX;
+    stop = row_stop::NEVER;
     bulk::init(full, ST);
     if (SPLIT) bulk::init(theirs, 2);
   }
@@ -813,7 +815,7 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
       }
       --left;
     }
-    if (i < staged && !bulk::wait(&full[stage], parity)) gave_up = i;
+    if (i < staged && !bulk::wait(&full[stage], parity)) atomicMin(&stop, row_stop::before_barrier(i));
     const uint8_t* src = row_ring + (size_t)stage * NT * slot;
     auto get = [&](int tensor, int c, uint64_t (&o)[4]) {
       if (!ODD) {
@@ -893,7 +895,9 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
       for (int k = 0; k < (PRE ? 3 : 1); ++k) red[buf][k][t >> 5] = sums[k];
     }
     __syncthreads();
-    if (SPLIT && !bulk::wait<true>(&theirs[buf], (uint32_t)(i >> 1) & 1u)) gave_up = i;
+    const bool leave = row_stop::leaves(stop, i);   // the same in every thread
+    if (SPLIT && !leave && !bulk::wait<true>(&theirs[buf], (uint32_t)(i >> 1) & 1u))
+      atomicMin(&stop, row_stop::after_barrier(i));
     if (t == 0) fetch(i + ST, stage);
     if (TPR > 32) {
 #pragma unroll
@@ -908,7 +912,7 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
       }
     }
     buf ^= 1;
-    if (gave_up <= i) break;   // set before the barrier: every thread sees it
+    if (leave) break;
     const float m1 = PRE ? sums[1] * inv_d : 0.0f;
     const float m2 = (PRE ? fmaf(-inv_y * m1, sums[2], sums[0]) : sums[0]) * inv_d;
     const ulonglong2 s0 = sums_at[0], s1 = sums_at[TPR];
@@ -976,13 +980,16 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
       parity ^= 1u;
     }
   }
-  if (gave_up != INT_MAX && t == 0) {
-    // a copy did not arrive in time: report it, and leave no copy in flight behind
+  if (SPLIT) pair_barrier();   // no CTA leaves while the other may still send to it
+  if (stop != row_stop::NEVER && t == 0) {
+    // a copy, or the other CTA's sums, did not arrive in time: report it, and leave
+    // nothing in flight behind.  Nothing tells when the other CTA's last sums have landed.
     atomicExch(&g_norm_error, NVFP4B200_ERR_TIMEOUT);
     for (int st = 0; st < ST; ++st) bulk::wait(&full[st], parity ^ (st < stage ? 1u : 0u));
+    if (SPLIT)
+      for (const long long t0 = clock64(); clock64() - t0 < SETTLE_CYCLES;) {
+      }
   }
-
-  if (SPLIT) pair_barrier();   // no CTA leaves while the other may still send to it
 
   // partial column sums: s * S, gate * s * S and dgamma_pre
   if (!in) return;
