@@ -29,7 +29,6 @@
 #include "vec.cuh"
 
 #include <algorithm>
-#include <climits>
 #include <type_traits>
 
 namespace nvfp4b200 {
@@ -399,7 +398,7 @@ __global__ void __launch_bounds__(TPR, 1024 / TPR) sandwich_fwd_odd_kernel(const
   extern __shared__ __align__(16) uint8_t odd_ring[];   // [stages][2][slot]
   __shared__ float red[4][TPR / 32];
   __shared__ __align__(8) uint64_t full[STAGES];
-  __shared__ int gave_up;   // the row whose copy did not arrive in time
+  __shared__ int stop;   // row_stop.h: set where a wait ran out
   const int t = threadIdx.x;
   const float inv_d = 1.0f / (float)a.d;
   const int row_bytes = a.d * (int)sizeof(Raw), slot = ((row_bytes + 15) & ~15) + 16;
@@ -416,7 +415,7 @@ __global__ void __launch_bounds__(TPR, 1024 / TPR) sandwich_fwd_odd_kernel(const
     bulk::copy(dst + slot, static_cast<const uint8_t*>(a.x) + r * a.ldx * (int64_t)sizeof(Raw) - ox, nx, &full[stage]);
   };
   if (t == 0) {
-    gave_up = INT_MAX;
+    stop = row_stop::NEVER;
     bulk::init(full, STAGES);
   }
   __syncthreads();
@@ -443,7 +442,7 @@ __global__ void __launch_bounds__(TPR, 1024 / TPR) sandwich_fwd_odd_kernel(const
       if (a.gate) times(a.gate, group * a.d, w);
     }
     const bool staged = r < safe;
-    if (staged && !bulk::wait(&full[stage], parity)) gave_up = (int)(r - r0);
+    if (staged && !bulk::wait(&full[stage], parity)) atomicMin(&stop, row_stop::before_barrier((int)(r - r0)));
     const uint8_t* src = odd_ring + (size_t)stage * 2 * slot;
     const Raw* rb = staged ? reinterpret_cast<const Raw*>(src + skew(r, a.ldb)) : static_cast<const Raw*>(a.b) + r * a.ldb;
     const Raw* rx = staged ? reinterpret_cast<const Raw*>(src + slot + skew(r, a.ldx)) : static_cast<const Raw*>(a.x) + r * a.ldx;
@@ -463,9 +462,10 @@ __global__ void __launch_bounds__(TPR, 1024 / TPR) sandwich_fwd_odd_kernel(const
 #pragma unroll
     for (int j = 0; j < 8; ++j) ss = t + j * TPR < a.d ? fmaf(v[j], v[j], ss) : ss;
     const float inv_b = rsqrtf(row_sum<TPR>(ss, red[buf], 0) * inv_d + a.eps);
-    // past the sum's barrier every thread has read the row: its place is refilled
+    // past the sum's barrier every thread has read the row: its place is refilled,
+    // where its copies arrived (a barrier whose phase is open takes no second ones)
+    if (row_stop::leaves(stop, (int)(r - r0))) break;
     if (t == 0) fetch(r + a.stages, stage);
-    if (gave_up <= r - r0) break;
     ss = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(TPR, 1024 / TPR) sandwich_fwd_odd_kernel(const
       parity ^= 1u;
     }
   }
-  if (gave_up != INT_MAX && t == 0) {
+  if (stop != row_stop::NEVER && t == 0) {
     // a copy did not arrive in time: report it, and leave no copy in flight behind
     atomicExch(&g_norm_error, NVFP4B200_ERR_TIMEOUT);
     for (int st = 0; st < a.stages; ++st) bulk::wait(&full[st], parity ^ (st < stage ? 1u : 0u));
@@ -895,9 +895,9 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
       for (int k = 0; k < (PRE ? 3 : 1); ++k) red[buf][k][t >> 5] = sums[k];
     }
     __syncthreads();
-    const bool leave = row_stop::leaves(stop, i);   // the same in every thread
-    if (SPLIT && !leave && !bulk::wait<true>(&theirs[buf], (uint32_t)(i >> 1) & 1u))
-      atomicMin(&stop, row_stop::after_barrier(i));
+    if (row_stop::leaves(stop, i)) break;   // the same in every thread
+    if (SPLIT && !bulk::wait<true>(&theirs[buf], (uint32_t)(i >> 1) & 1u)) atomicMin(&stop, row_stop::after_barrier(i));
+    // refilled only where the row's own copies arrived: a barrier whose phase is open takes no second one
     if (t == 0) fetch(i + ST, stage);
     if (TPR > 32) {
 #pragma unroll
@@ -912,7 +912,6 @@ __global__ void __launch_bounds__(TPR, DT == NVFP4B200_F32 && TPR >= 512 ? 1 : 1
       }
     }
     buf ^= 1;
-    if (leave) break;
     const float m1 = PRE ? sums[1] * inv_d : 0.0f;
     const float m2 = (PRE ? fmaf(-inv_y * m1, sums[2], sums[0]) : sums[0]) * inv_d;
     const ulonglong2 s0 = sums_at[0], s1 = sums_at[TPR];

@@ -94,3 +94,63 @@ def test_the_schedules_find_a_rule_that_is_not_uniform(rule):
     got = [run(rng, rng.randint(2, 6), rng.randint(1, 6), 0.05, lambda i: i, lambda i: i, rule.leaves, rule.never(), False)
            for _ in range(3000)]
     assert any(g == "hang" or len(set(g.values())) > 1 for g in got)
+
+
+class Ring:
+    """A ring of single-arrival transaction barriers.  Arming one whose phase is still
+    open would be its second arrival in the phase: the hardware leaves that undefined."""
+
+    def __init__(self, stages):
+        self.open, self.parity = [False] * stages, [0] * stages
+
+    def arm(self, st):
+        assert not self.open[st], "armed twice in one phase"
+        self.open[st] = True
+
+    def land(self, st):
+        self.open[st] = False
+        self.parity[st] ^= 1
+
+
+@pytest.mark.parametrize("refill_first", [False, True])
+def test_refill_behind_the_check(refill_first):
+    """A row whose copies are late: the loop leaves before its place is refilled, and
+    every place is then waited for in the phase that is still open.  The other order
+    arms a barrier twice."""
+    def walk():
+        for stages in (1, 2, 3):
+            for late in range(6):
+                ring, stage, parity, rows = Ring(stages), 0, 0, 6
+                for st in range(stages):
+                    ring.arm(st)
+                for i in range(rows):
+                    if i != late:
+                        ring.land(stage)
+                    arrived = ring.parity[stage] != parity
+                    if refill_first and i + stages < rows:
+                        ring.arm(stage)
+                    if not arrived:
+                        break
+                    if not refill_first and i + stages < rows:
+                        ring.arm(stage)
+                    stage += 1
+                    if stage == stages:
+                        stage, parity = 0, parity ^ 1
+                for st in range(stages):               # what is still open is waited for in its own phase
+                    assert not ring.open[st] or ring.parity[st] == parity ^ (st < stage)
+
+    if refill_first:
+        with pytest.raises(AssertionError, match="twice"):
+            walk()
+    else:
+        walk()
+
+
+def test_kernels_refill_behind_the_check():
+    """The order in the sources: each row loop leaves before it refills."""
+    text = open(os.path.join(os.path.dirname(HEADER), "norm.cu")).read()
+    parts = text.split("row_stop::leaves(")
+    assert len(parts) == 3                             # the two loops that wait for copies
+    for before, after in zip(parts, parts[1:]):
+        loop = before[before.rindex("row_stop::before_barrier("):]
+        assert "fetch(" not in loop and after.index("break;") < after.index("fetch(")
