@@ -81,7 +81,9 @@ __device__ __forceinline__ uint32_t cluster_size() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
+// The barrier's aligned form takes whole warps: lanes that parted before it meet first.
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ float4 ld_cluster(uint32_t local_addr, uint32_t rank) {
@@ -325,6 +327,7 @@ __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constan
   __syncthreads();
   float* part = reinterpret_cast<float*>(smem);
   const int m = (int)imin64(N, a.m - tok0);   // tokens of this block
+  __syncwarp();
   {
     const int row = 32 * (warp & 3) + lane;   // a warp reads the TMEM lanes of its quarter
     for (int t = 16 * (warp >> 2); t < m; t += 32) {
@@ -336,9 +339,9 @@ __global__ void __launch_bounds__(THREADS) mx_linear_kernel(const __grid_constan
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  __syncwarp();
   if (warp == 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols<N>()) : "memory");
-  __syncwarp();
   if (parts > 1) cluster_sync();
   const int64_t row = (int64_t)tile * TILE_ROWS + 4 * lane;   // n % 8 == 0: all four rows or none
   if (row < a.n && !gave_up) {
