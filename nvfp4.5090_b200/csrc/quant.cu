@@ -24,6 +24,23 @@ namespace nvfp4b200 {
 // device check (shared by every entry point)
 // ---------------------------------------------------------------------------
 
+// Tensor maps are encoded by the driver, which wants a context current in the
+// calling thread.  A host thread whose first CUDA call is one of ours has none.
+static bool bind_context(int dev) {
+  typedef CUresult (*GetFn)(CUcontext*);
+  static const GetFn get = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                   q == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<GetFn>(p)
+               : nullptr;
+  }();
+  CUcontext ctx = nullptr;
+  if (get && get(&ctx) == CUDA_SUCCESS && ctx) return true;
+  return cudaSetDevice(dev) == cudaSuccess;
+}
+
 int check_device() {
   static std::mutex mu;
   static int cached[64];
@@ -40,6 +57,7 @@ int check_device() {
     cached[dev] = (major == 10 && minor == 0) ? NVFP4B200_OK : NVFP4B200_ERR_UNSUPPORTED_DEVICE;
     init[dev] = true;
   }
+  if (cached[dev] == NVFP4B200_OK && !bind_context(dev)) return NVFP4B200_ERR_CUDA;
   return cached[dev];
 }
 
