@@ -37,6 +37,15 @@ inline int launch_status() {
   return e == cudaSuccess ? NVFP4B200_OK : NVFP4B200_ERR_LAUNCH;
 }
 
+// Lets a kernel have up to `most` bytes of dynamic shared memory.  The limit
+// belongs to the kernel and the device, not to one launch: `most` is the largest
+// that any launch of the kernel takes, so that calls of several sizes, from
+// several host threads, all set the same.
+template <typename F>
+inline bool allow_smem(F* kernel, int most) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most) == cudaSuccess;
+}
+
 __host__ __device__ __forceinline__ int64_t imin64(int64_t a, int64_t b) { return a < b ? a : b; }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }

@@ -1246,8 +1246,7 @@ static DeviceInfo device_info() {
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaFuncSetAttribute(nvfp4_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) ==
-            cudaSuccess &&
+    if (allow_smem(nvfp4_gemm_kernel, SMEM_BYTES) &&
         cudaOccupancyMaxActiveClusters(&n, nvfp4_gemm_kernel, &cfg) == cudaSuccess && n > 0)
       d.max_clusters = n;
     else
@@ -1426,9 +1425,7 @@ static int run(const void* a, const void* b, const void* sfa, const void* sfb, c
   if (max_sms > 0) cap = std::max(1, std::min(cap, max_sms / 2));
   const int clusters = (int)std::min<int64_t>(tiles, cap);
   p.sched_slot = tiles > clusters ? take_slot(stream) : -1;   // one tile each: nothing to claim
-  if (cudaFuncSetAttribute(nvfp4_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) !=
-      cudaSuccess)
-    return NVFP4B200_ERR_CUDA;
+  if (!allow_smem(nvfp4_gemm_kernel, SMEM_BYTES)) return NVFP4B200_ERR_CUDA;
   nvfp4_gemm_kernel<<<2 * clusters, NUM_THREADS, smem_bytes, stream>>>(ma, mb, msa, msb, md, mh, p);
   uint32_t* ws = sw ? sw->ws : (dsw ? dsw->ws : nullptr);
   if (ws) {

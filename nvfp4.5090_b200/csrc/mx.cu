@@ -287,12 +287,10 @@ __global__ void __launch_bounds__(QTHREADS, DT == NVFP4B200_F32 && (COLS || SCAL
 
 template <int DT, bool ROWS, bool COLS, bool SCALED>
 static int launch_quant(const QuantArgs& a, cudaStream_t st) {
-  const int smem = COLS ? tile_bytes<DT>() + TILE * STAGE_LD : 0;
+  constexpr int SMEM = COLS ? tile_bytes<DT>() + TILE * STAGE_LD : 0;
   auto* fn = mx_quant_kernel<DT, ROWS, COLS, SCALED>;
-  if (smem > 32 * 1024 &&   // with the static arrays, past the default limit
-      cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return NVFP4B200_ERR_CUDA;
-  fn<<<(unsigned)(a.row_tiles * a.col_tiles), QTHREADS, smem, st>>>(a);
+  if (SMEM > 32 * 1024 && !allow_smem(fn, SMEM)) return NVFP4B200_ERR_CUDA;   // with the static arrays, past the default limit
+  fn<<<(unsigned)(a.row_tiles * a.col_tiles), QTHREADS, SMEM, st>>>(a);
   return launch_status();
 }
 

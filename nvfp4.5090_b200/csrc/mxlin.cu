@@ -428,9 +428,11 @@ static int launch(const void* qw, const void* qx, Args a, int parts, cudaStream_
   const int fit = (SMEM_SM / 2 - 2048 - held) / stage_bytes<N, FUSED>();
   a.stages = std::max(1, std::min({most, fit, MAX_STAGES}));
   const int smem = std::max(a.stages * stage_bytes<N, FUSED>() + held, N * TILE_ROWS * 4) + 1024;
+  constexpr int MOST = SMEM_SM / 2;   // of the ring (above) and of the sums
+  static_assert(N * TILE_ROWS * 4 + 1024 <= MOST && stage_bytes<N, FUSED>() + (FUSED ? FUSED_STEPS * (N * BK_BYTES + SF_BYTES) : 0) + 1024 <= MOST,
+                "shared memory of one CTA of two");
   auto* fn = mx_linear_kernel<N, FUSED>;
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return NVFP4B200_ERR_CUDA;
+  if (!allow_smem(fn, MOST)) return NVFP4B200_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * parts), (unsigned)ceil_div(a.m, N), 1);
   cfg.blockDim = dim3(THREADS, 1, 1);

@@ -37,7 +37,7 @@ namespace norm {
 constexpr int VPT = 2;            // 8-element vectors per thread and row
 constexpr int CPT = 8 * VPT;      // columns per thread
 constexpr int MAX_D = 1024 * CPT;
-constexpr int MAX_SMEM = 225 * 1024;   // dynamic, of one CTA: 227 KB less the static arrays
+constexpr int MAX_SMEM = 225 * 1024;   // dynamic, of one CTA: 227 KB less the static arrays; every kernel's limit
 // what n CTAs of an SM can each have: its 228 KB less 1 KB per CTA that the system takes and 1 KB of static arrays
 constexpr int smem_share(int n) { return n <= 1 ? MAX_SMEM : 228 * 1024 / n - 2048; }
 
@@ -1183,8 +1183,7 @@ int nvfp4b200_sandwich_norm(const void* b, const void* x, const void* gamma_post
       constexpr int smem = norm::STAGES * 2 * THREADS_V * 8 * V * norm::dtype_size<DT>();
       if constexpr (decltype(v)::value && smem <= norm::MAX_SMEM) {
         auto* fn = norm::sandwich_fwd_staged_kernel<DT, TV, V>;
-        if (smem > 32 * 1024 &&   // with the static arrays, past the default limit
-            cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        if (smem > 32 * 1024 && !allow_smem(fn, norm::MAX_SMEM))   // with the static arrays, past the default limit
           return (int)NVFP4B200_ERR_CUDA;
         const int per_sm = std::max(1, std::min(228 * 1024 / (smem + 2048), 1024 / THREADS_V));
         fn<<<(unsigned)std::min<int64_t>(ceil_div(rows, THREADS_V / TV), (int64_t)sm_count_current() * per_sm), THREADS_V, smem, st>>>(a);
@@ -1200,9 +1199,7 @@ int nvfp4b200_sandwich_norm(const void* b, const void* x, const void* gamma_post
           a.safe_rows = std::max<int64_t>(0, rows - 1 - 15 / (std::min(ldb, ldx) * bytes));
           auto* odd = norm::sandwich_fwd_odd_kernel<DT, T2>;
           const int size = a.stages * row;
-          if (size > 32 * 1024 &&   // with the static arrays, past the default limit
-              cudaFuncSetAttribute(odd, cudaFuncAttributeMaxDynamicSharedMemorySize, size) != cudaSuccess)
-            return (int)NVFP4B200_ERR_CUDA;
+          if (size > 32 * 1024 && !allow_smem(odd, norm::MAX_SMEM)) return (int)NVFP4B200_ERR_CUDA;
           a.rows_per_cta = ceil_div(rows, (int64_t)sm_count_current() * (1024 / T2));
           odd<<<(unsigned)ceil_div(rows, a.rows_per_cta), T2, size, st>>>(a);
           return launch_status();
@@ -1292,9 +1289,7 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
                                  : norm::sandwich_bwd_staged_kernel<DT, T2, false, ODD, true, SPLIT>)
                            : (dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true, ODD, false, SPLIT>
                                  : norm::sandwich_bwd_staged_kernel<DT, T2, false, ODD, false, SPLIT>);
-          if (smem > 32 * 1024 &&   // with the static arrays, past the default limit
-              cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-            return (int)NVFP4B200_ERR_CUDA;
+          if (smem > 32 * 1024 && !allow_smem(fn, norm::MAX_SMEM)) return (int)NVFP4B200_ERR_CUDA;
           if (!SPLIT) {
             fn<<<(unsigned)sp.ctas, T2, smem, st>>>(a, sp.parts_per_group);
             return launch_status();

@@ -961,8 +961,7 @@ int nvfp4b200_quant_nvfp4_t(const void* x, const float* row_scale, const void* g
   const int n_tiles = (int)(n_tiles_t * n_tiles_d);
   auto run = [&](auto kern) -> int {
     const int smem = (int)sizeof(TqSmem);
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-      return NVFP4B200_ERR_CUDA;
+    if (!allow_smem(kern, (int)sizeof(TqSmem))) return NVFP4B200_ERR_CUDA;
     int per_sm = 0, dev = 0, sms = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, 256, smem) != cudaSuccess || per_sm < 1)
       return NVFP4B200_ERR_CUDA;
