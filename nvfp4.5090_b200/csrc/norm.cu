@@ -513,7 +513,8 @@ struct BwdArgs {
 // divides rows_per_gate or is a multiple of it, so a CTA's rows lie in one
 // group or are whole groups.  (Groups of rows that end early are handled by
 // the host: parts of a group are cut at its end.)
-template <int DT, bool VEC, int TPR, int V>
+// For tensors that start off a 16-byte boundary: single elements, straight from global memory.
+template <int DT, int TPR, int V>
 __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int64_t parts_per_group) {
   using Raw = typename Elem<DT>::Raw;
   constexpr int C = 8 * V;   // columns per thread
@@ -535,7 +536,7 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
   for (int j = 0; j < C; ++j) S[j] = post[j] = pre[j] = 0.0f;
   int buf = 0;
   for (; r < end; ++r) {
-    Row<DT, VEC, TPR, V> row, rb, rw;
+    Row<DT, false, TPR, V> row, rb, rw;
     float tt[C], z[C], w[C], v[C];
     if (a.dy) row.load(static_cast<const Raw*>(a.dy) + r * a.ld_dy, t, a.d);
     rb.load(static_cast<const Raw*>(a.b) + r * a.ldb, t, a.d);
@@ -546,7 +547,7 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
       for (int j = 0; j < C; ++j) tt[j] = 0.0f;
     }
     if (a.dn) {
-      Row<DT, VEC, TPR, V> rn, ry;
+      Row<DT, false, TPR, V> rn, ry;
       rn.load(static_cast<const Raw*>(a.dn) + r * a.ld_dn, t, a.d);
       ry.load(static_cast<const Raw*>(a.y) + r * a.ldy, t, a.d);
       rn.values(v);
@@ -596,10 +597,10 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
     const float mean = row_sum<TPR>(dot, red[buf + 1], 0) * inv_d;
 #pragma unroll
     for (int j = 0; j < C; ++j) z[j] = inv * fmaf(-mean, z[j], v[j]);
-    store_row<DT, VEC, TPR, V>(static_cast<Raw*>(a.db) + r * a.d, t, a.d, z);
+    store_row<DT, false, TPR, V>(static_cast<Raw*>(a.db) + r * a.d, t, a.d, z);
 #pragma unroll
     for (int j = 0; j < C; ++j) tt[j] *= a.alpha;
-    store_row<DT, VEC, TPR, V>(static_cast<Raw*>(a.dx) + r * a.d, t, a.d, tt);
+    store_row<DT, false, TPR, V>(static_cast<Raw*>(a.dx) + r * a.d, t, a.d, tt);
     buf ^= 2;
     // the last row of a group (or of this CTA's part of it): hand S over
     if (a.gate && (r + 1 == end || (r + 1) % a.rows_per_gate == 0)) {
@@ -617,7 +618,7 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
       }
 #pragma unroll
       for (int j = 0; j < C; ++j) {
-        const int c = column<VEC, TPR>(t, j);
+        const int c = column<false, TPR>(t, j);
         if (out && c < a.d) out[c] = S[j];
         S[j] = 0.0f;
       }
@@ -625,7 +626,7 @@ __global__ void __launch_bounds__(TPR) sandwich_bwd_kernel(const BwdArgs a, int6
   }
 #pragma unroll
   for (int j = 0; j < C; ++j) {
-    const int c = column<VEC, TPR>(t, j);
+    const int c = column<false, TPR>(t, j);
     if (c < a.d) {
       a.part[(int64_t)blockIdx.x * a.d + c] = a.gate ? post[j] : S[j];
       a.part[((int64_t)gridDim.x + blockIdx.x) * a.d + c] = pre[j];
@@ -1174,40 +1175,41 @@ int nvfp4b200_sandwich_norm(const void* b, const void* x, const void* gamma_post
     return norm::by_width((int)d, [&](auto tpr) {
       constexpr int T = decltype(tpr)::value, THREADS = norm::threads_of(T), GROUPS = THREADS / T;
       constexpr int DT = decltype(dt)::value;
-      const int64_t want = ceil_div(rows, GROUPS);
-      // the staged kernel where its ring fits: 195 -> 168 us at 16384 x 8192 bf16 with the next norm.
-      // fp32: 8 columns a thread, so that 32 warps share an SM (8192 x 4096: 88 us, 141 with 16
-      // columns; bf16 at 16384 x 4096 93 with 16 columns, 109 with 8)
+      constexpr bool VEC = decltype(v)::value;
+      // the staged kernel where its ring fits (all but fp32 rows of more than 8192 columns): 195 -> 168 us
+      // at 16384 x 8192 bf16 with the next norm.  fp32: 8 columns a thread, so that 32 warps share an SM
+      // (8192 x 4096: 88 us, 141 with 16 columns; bf16 at 16384 x 4096 93 with 16 columns, 109 with 8)
       constexpr int V = DT == NVFP4B200_F32 && T <= 512 ? 1 : norm::VPT, TV = T * norm::VPT / V;
       constexpr int THREADS_V = norm::threads_of(TV);
       constexpr int smem = norm::STAGES * 2 * THREADS_V * 8 * V * norm::dtype_size<DT>();
-      if constexpr (decltype(v)::value && smem <= norm::MAX_SMEM) {
+      if constexpr (VEC && smem <= norm::MAX_SMEM) {
         auto* fn = norm::sandwich_fwd_staged_kernel<DT, TV, V>;
         if (smem > 32 * 1024 && !allow_smem(fn, norm::MAX_SMEM))   // with the static arrays, past the default limit
           return (int)NVFP4B200_ERR_CUDA;
         const int per_sm = std::max(1, std::min(228 * 1024 / (smem + 2048), 1024 / THREADS_V));
         fn<<<(unsigned)std::min<int64_t>(ceil_div(rows, THREADS_V / TV), (int64_t)sm_count_current() * per_sm), THREADS_V, smem, st>>>(a);
         return launch_status();
-      }
-      if constexpr (!decltype(v)::value && T >= 64 && T <= 512) {
-        // unaligned rows of more than 512 columns, 8 columns a thread: 114 -> 82 us at 8000 x
-        // 4095 bf16 with the next norm (20000 x 301: 24 us without, 28 with)
-        constexpr int T2 = 2 * T;
-        const int row = 2 * ((int)round_up(d * bytes, 16) + 16), share = norm::smem_share(1024 / T2);
-        if (aligned(b, 16) && aligned(x, 16) && row <= share) {
-          a.stages = std::min(norm::STAGES, share / row);
-          a.safe_rows = std::max<int64_t>(0, rows - 1 - 15 / (std::min(ldb, ldx) * bytes));
-          auto* odd = norm::sandwich_fwd_odd_kernel<DT, T2>;
-          const int size = a.stages * row;
-          if (size > 32 * 1024 && !allow_smem(odd, norm::MAX_SMEM)) return (int)NVFP4B200_ERR_CUDA;
-          a.rows_per_cta = ceil_div(rows, (int64_t)sm_count_current() * (1024 / T2));
-          odd<<<(unsigned)ceil_div(rows, a.rows_per_cta), T2, size, st>>>(a);
-          return launch_status();
+      } else {
+        if constexpr (!VEC && T >= 64 && T <= 512) {
+          // unaligned rows of more than 512 columns, 8 columns a thread: 114 -> 82 us at 8000 x
+          // 4095 bf16 with the next norm (20000 x 301: 24 us without, 28 with)
+          constexpr int T2 = 2 * T;
+          const int row = 2 * ((int)round_up(d * bytes, 16) + 16), share = norm::smem_share(1024 / T2);
+          if (aligned(b, 16) && aligned(x, 16) && row <= share) {
+            a.stages = std::min(norm::STAGES, share / row);
+            a.safe_rows = std::max<int64_t>(0, rows - 1 - 15 / (std::min(ldb, ldx) * bytes));
+            auto* odd = norm::sandwich_fwd_odd_kernel<DT, T2>;
+            const int size = a.stages * row;
+            if (size > 32 * 1024 && !allow_smem(odd, norm::MAX_SMEM)) return (int)NVFP4B200_ERR_CUDA;
+            a.rows_per_cta = ceil_div(rows, (int64_t)sm_count_current() * (1024 / T2));
+            odd<<<(unsigned)ceil_div(rows, a.rows_per_cta), T2, size, st>>>(a);
+            return launch_status();
+          }
         }
+        const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(rows, GROUPS), (int64_t)sm_count_current() * (2048 / THREADS));
+        norm::sandwich_fwd_kernel<DT, VEC, T><<<grid, THREADS, 0, st>>>(a);
+        return launch_status();
       }
-      const unsigned grid = (unsigned)std::min<int64_t>(want, (int64_t)sm_count_current() * (2048 / THREADS));
-      norm::sandwich_fwd_kernel<decltype(dt)::value, decltype(v)::value, T><<<grid, THREADS, 0, st>>>(a);
-      return launch_status();
     });
   });
 }
@@ -1266,16 +1268,17 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
   return norm::by_type(dtype, vec, [&](auto dt, auto v) {
     const int r = norm::by_width((int)d, [&](auto tpr) {
       constexpr int T = decltype(tpr)::value, DT = decltype(dt)::value;
-      // the staged kernel where a row fits: 346 -> 152 us at 16000 x 4096 bf16 with 8
-      // gates and the next norm, 611 -> 246 with a gate per row
-      {
+      constexpr bool ODD = !decltype(v)::value;
+      // the staged kernel: 346 -> 152 us at 16000 x 4096 bf16 with 8 gates and the next norm, 611 -> 246 with a
+      // gate per row
+      auto staged = [&]() -> int {
         constexpr bool SPLIT = T > 512;
         constexpr int T2 = SPLIT ? T : 2 * T;
-        constexpr bool ODD = !decltype(v)::value;
         // two CTAs' worth of threads share an SM (fewer where one is that large), and
         // so its memory: as many ring rows as fit, up to 3 (2 with the next norm's
         // tensors); one row at least, alone on the SM if need be
         const int width = (int)(SPLIT ? round_up(ceil_div(d, 2), 8) : d) * bytes, row = (dn ? 4 : 2) * (ODD ? (int)round_up(width, 16) + 16 : width);
+        static_assert(4 * (8192 * norm::dtype_size<DT>() + 16) + (4 + 2) * 16 * T2 <= norm::MAX_SMEM, "one row and the column sums");
         const bool multi = gate && sp.parts_per_group == 1;   // a CTA's rows are whole groups
         const int sums = ((dn ? 4 : 2) + (multi ? 2 : 0)) * 16 * T2;
         const int share = norm::smem_share(1024 / T2);
@@ -1283,40 +1286,43 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
         const int smem = a.stages * row + sums;
         const int64_t ld_min = std::min(std::min(dy ? ld_dy : ldb, ldb), dn ? std::min(ld_dn, ldy) : ldb);
         a.safe_rows = std::max<int64_t>(0, rows - 1 - 15 / (ld_min * bytes));
-        const bool bases = aligned(b, 16) && (!dy || aligned(dy, 16)) && (!dn || (aligned(dn, 16) && aligned(y, 16)));
-        if (smem <= norm::MAX_SMEM && (!ODD || bases)) {
-          auto* fn = multi ? (dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true, ODD, true, SPLIT>
-                                 : norm::sandwich_bwd_staged_kernel<DT, T2, false, ODD, true, SPLIT>)
-                           : (dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true, ODD, false, SPLIT>
-                                 : norm::sandwich_bwd_staged_kernel<DT, T2, false, ODD, false, SPLIT>);
-          if (smem > 32 * 1024 && !allow_smem(fn, norm::MAX_SMEM)) return (int)NVFP4B200_ERR_CUDA;
-          if (!SPLIT) {
-            fn<<<(unsigned)sp.ctas, T2, smem, st>>>(a, sp.parts_per_group);
-            return launch_status();
-          }
-          cudaLaunchConfig_t cfg = {};
-          cfg.gridDim = dim3((unsigned)(2 * sp.ctas), 1, 1);
-          cfg.blockDim = dim3(T2, 1, 1);
-          cfg.dynamicSmemBytes = smem;
-          cfg.stream = st;
-          cudaLaunchAttribute pair;
-          pair.id = cudaLaunchAttributeClusterDimension;
-          pair.val.clusterDim.x = 2;
-          pair.val.clusterDim.y = pair.val.clusterDim.z = 1;
-          cfg.attrs = &pair;
-          cfg.numAttrs = 1;
-          if (cudaLaunchKernelEx(&cfg, fn, a, sp.parts_per_group) != cudaSuccess) {
-            cudaGetLastError();
-            return (int)NVFP4B200_ERR_LAUNCH;
-          }
+        auto* fn = multi ? (dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true, ODD, true, SPLIT>
+                               : norm::sandwich_bwd_staged_kernel<DT, T2, false, ODD, true, SPLIT>)
+                         : (dn ? norm::sandwich_bwd_staged_kernel<DT, T2, true, ODD, false, SPLIT>
+                               : norm::sandwich_bwd_staged_kernel<DT, T2, false, ODD, false, SPLIT>);
+        if (smem > 32 * 1024 && !allow_smem(fn, norm::MAX_SMEM)) return NVFP4B200_ERR_CUDA;
+        if (!SPLIT) {
+          fn<<<(unsigned)sp.ctas, T2, smem, st>>>(a, sp.parts_per_group);
           return launch_status();
         }
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(2 * sp.ctas), 1, 1);
+        cfg.blockDim = dim3(T2, 1, 1);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cudaLaunchAttribute pair;
+        pair.id = cudaLaunchAttributeClusterDimension;
+        pair.val.clusterDim.x = 2;
+        pair.val.clusterDim.y = pair.val.clusterDim.z = 1;
+        cfg.attrs = &pair;
+        cfg.numAttrs = 1;
+        if (cudaLaunchKernelEx(&cfg, fn, a, sp.parts_per_group) != cudaSuccess) {
+          cudaGetLastError();
+          return NVFP4B200_ERR_LAUNCH;
+        }
+        return launch_status();
+      };
+      if constexpr (!ODD) {
+        return staged();
+      } else {
+        // the ring's copies start on 16-byte boundaries
+        if (aligned(b, 16) && (!dy || aligned(dy, 16)) && (!dn || (aligned(dn, 16) && aligned(y, 16)))) return staged();
+        // 8 columns a thread while 1024 threads cover the row: twice the warps of 16
+        // columns (166 -> 123 us at 2013 x 4971 fp16)
+        constexpr int T2 = T <= 512 ? 2 * T : T, V = T <= 512 ? 1 : norm::VPT;
+        norm::sandwich_bwd_kernel<DT, T2, V><<<(unsigned)sp.ctas, T2, 0, st>>>(a, sp.parts_per_group);
+        return launch_status();
       }
-      // 8 columns a thread while 1024 threads cover the row: twice the warps of 16
-      // columns (166 -> 123 us at 2013 x 4971 fp16)
-      constexpr int T2 = T <= 512 ? 2 * T : T, V = T <= 512 ? 1 : norm::VPT;
-      norm::sandwich_bwd_kernel<DT, decltype(v)::value, T2, V><<<(unsigned)sp.ctas, T2, 0, st>>>(a, sp.parts_per_group);
-      return launch_status();
     });
     if (r) return r;
     if (!dgamma_post && !dgamma_pre && !dgate) return (int)NVFP4B200_OK;
