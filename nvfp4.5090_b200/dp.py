@@ -146,13 +146,12 @@ class ShardedBucketOptimizer:
         gradient norm, which needs every bucket)."""
         if key not in self.rs_works:
             raise RuntimeError(f"bucket {key!r}: no reduce-scatter in flight")
-        w = self.rs_works[key]
-        if w is None:   # waited for already
-            return
-        if timeout_s is None:
-            w.wait()
-        else:
-            w.wait(timeout=datetime.timedelta(seconds=timeout_s))
+        w = self.rs_works.pop(key)   # a wait that raises leaves the bucket free for another exchange
+        if w is not None:            # None: waited for already
+            if timeout_s is None:
+                w.wait()
+            else:
+                w.wait(timeout=datetime.timedelta(seconds=timeout_s))
         self.rs_works[key] = None
 
     def update(self, key: Hashable, param_full: torch.Tensor, update_fn, timeout_s: Optional[float] = None,
