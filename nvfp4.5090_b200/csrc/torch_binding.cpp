@@ -350,9 +350,9 @@ struct MXLinear : public torch::autograd::Function<MXLinear> {
     torch::autograd::variable_list out(5);
     if (!dy.defined()) return out;
     if (need) {
-      auto [dx, dw] = linear_backward(dy, opt(saved[0]), opt(saved[1]), shape, n, need & 1, need & 2, wtype == at::kFloat);
+      auto [dx, dw] = linear_backward(dy, opt(saved[0]), opt(saved[1]), shape, n, need & 1, need & 2, wtype != at::kBFloat16);
       if (dx) out[0] = *dx;
-      if (dw) out[1] = dw->scalar_type() == wtype ? *dw : dw->to(wtype);
+      if (dw) out[1] = dw->scalar_type() == wtype ? *dw : dw->to(wtype);   // fp16: from fp32, one rounding
     }
     if (b >= 0 && ctx->needs_input_grad(2))
       out[2] = dy.reshape({tokens(shape), n}).sum(at::IntArrayRef{0}, false, at::kFloat).to((at::ScalarType)b);
