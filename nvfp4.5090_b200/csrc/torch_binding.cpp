@@ -57,6 +57,12 @@ int64_t operand_bytes(int64_t rows, int64_t k) { return rows * k / 2 + scale_byt
 Tensor bytes(const Tensor& like, c10::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kByte)); }
 Tensor floats(const Tensor& like, c10::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
 
+// Contiguous, on a 16-byte boundary (a slice of a flat parameter buffer may start anywhere): copied otherwise.
+Tensor vector_of(const Tensor& t) {
+  const Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
+}
+
 // ---- MXFP4 -----------------------------------------------------------------
 
 // x as the quantizers read it: 2-D, unit column stride, 16-byte aligned rows;
@@ -108,8 +114,7 @@ std::pair<Pair, Pair> quantize(const Tensor& x_, const OptTensor& row_, const Op
   if (gamma_) {
     TORCH_CHECK(on(*gamma_, x) && gamma_->scalar_type() == at::kBFloat16 && gamma_->numel() == c,
                 "gamma is bf16 [K] on the input's device");
-    gamma = gamma_->contiguous();
-    if (reinterpret_cast<uintptr_t>(gamma->data_ptr()) % 16) gamma = gamma->clone();
+    gamma = vector_of(*gamma_);
   }
   On at_(x);
   Pair a, b;
@@ -155,7 +160,7 @@ OptTensor bias_of(const OptTensor& bias, int64_t n, const Tensor& like) {
   if (!bias) return std::nullopt;
   TORCH_CHECK(on(*bias, like) && bias->scalar_type() == at::kBFloat16 && bias->numel() == n,
               "bias is a CUDA BF16 tensor [n] on the operands' device");
-  return bias->contiguous();
+  return vector_of(*bias);
 }
 
 Tensor mx_gemm(const Tensor& qa, const Tensor& sa, const Tensor& qb, const Tensor& sb, const OptTensor& bias_,
@@ -261,7 +266,7 @@ std::tuple<Tensor, OptTensor, OptTensor> linear_forward(const Tensor& x_, const 
   OptTensor bias;
   if (bias_) {
     TORCH_CHECK(on(*bias_, x_) && bias_->numel() == n, "bias is a tensor [N] on the input's device");
-    bias = bias_->to(at::kBFloat16).contiguous();
+    bias = vector_of(bias_->to(at::kBFloat16));
   }
   On at_(x_);
   const Tensor x = float_matrix(x_.dim() == 2 ? x_ : x_.reshape({-1, k})), w = float_matrix(w_);
