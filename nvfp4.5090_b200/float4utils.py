@@ -416,7 +416,9 @@ class MXFP4Linear(NVFP4Linear):
     ``freeze()`` quantizes the weight once and drops into the serving form
     (``ops.mx_linear``: bf16 inputs, no gradients; the weight is not read again
     until ``thaw()``, a move or a loaded state, after which the layer is no
-    longer frozen); without it every call quantizes the current weight."""
+    longer frozen); without it every call quantizes the current weight.  A call
+    of a frozen layer that would have to give gradients (of the input, the
+    weight or the bias) is refused."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=torch.bfloat16):
         super().__init__(in_features, out_features, bias, device, dtype)
@@ -442,8 +444,9 @@ class MXFP4Linear(NVFP4Linear):
 
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         if self._held is not None:
-            require(not (torch.is_grad_enabled() and input.requires_grad),
-                    "a frozen MXFP4Linear has no gradients: thaw() it, or call it under torch.no_grad()")
+            wanted = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (input, self.weight, self.bias))
+            require(not wanted, "a frozen MXFP4Linear has no gradients: thaw() it, call it under torch.no_grad(), or "
+                                "requires_grad_(False) it")
             return ops.mx_linear(input, *self._held)
         return mxfp4_linear(input, self.weight, self.bias)
 
