@@ -61,11 +61,22 @@ def _scalar_f32(g: Optional[torch.Tensor], device) -> Optional[torch.Tensor]:
 _WS = {}
 
 
+def _capturing(device: torch.device) -> bool:
+    if device.index is None or device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def workspace(device: torch.device) -> torch.Tensor:
     """Zeroed 2-word workspace for the amax reductions, one per (device, stream).
 
     The kernels leave it zero after every call; calls on one stream never
-    overlap, so one workspace per stream is race-free."""
+    overlap, so one workspace per stream is race-free.  A captured call runs
+    whenever its graph does, on any stream: it gets a workspace of its own,
+    zeroed in the graph."""
+    if _capturing(device):
+        return torch.zeros(2, dtype=torch.int32, device=device)
     stream = torch.cuda.current_stream(device).cuda_stream
     key = (device.index, stream)
     ws = _WS.get(key)
