@@ -153,12 +153,13 @@ struct Norm {
 };
 
 // grad_scale * coef; thread `writer` also writes the norm and the coefficient.
-// A NaN norm gives a NaN coefficient, an infinite one 0.
+// A NaN norm gives a NaN coefficient, an infinite one 0, whatever the limit (inf / inf is no factor).
 __device__ __forceinline__ float clip_factor(const Norm& a, bool writer) {
   const double total = a.inf ? total_of<true>(a.partials, a.n) : total_of<false>(a.partials, a.n);
   const double norm = (a.inf ? total : sqrt(total)) * fabs((double)a.grad_scale);
   double c = (double)a.max_norm / (norm + 1e-6);
   if (c > 1.0) c = 1.0;
+  if (norm == INFINITY) c = 0.0;
   if (writer) {
     if (a.norm) *a.norm = (float)norm;
     if (a.coef) *a.coef = (float)c;
