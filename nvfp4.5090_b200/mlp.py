@@ -201,6 +201,8 @@ class SandwichNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, b, x, gamma_post, gate, gamma_pre, residual_scale, branch_scale, eps, pre):
         d = b.shape[-1]
+        if x.shape[-1] != d:
+            raise RuntimeError(f"b and x must match in width: {d} and {x.shape[-1]}")
         b2 = b.reshape(-1, d)
         y, n, inv_b, inv_y = ops.sandwich_norm(b2, x.reshape(-1, d), gamma_post, gate, gamma_pre,
                                                residual_scale=residual_scale, branch_scale=branch_scale, eps=eps,
@@ -209,7 +211,7 @@ class SandwichNormFunction(torch.autograd.Function):
             y, n = (None if t is None else torch.ops.aten._unsafe_view(t, b.shape) for t in (y, n))
         # y as it is returned: a change of it in place before the backward that reads it is refused
         ctx.save_for_backward(b2, y if n is not None else None, inv_b, inv_y, gamma_post, gate, gamma_pre)
-        ctx.scales, ctx.shape = (residual_scale, branch_scale), b.shape
+        ctx.scales, ctx.shape, ctx.x_shape = (residual_scale, branch_scale), b.shape, x.shape
         ctx.set_materialize_grads(False)
         return y if n is None else (y, n)
 
@@ -224,7 +226,7 @@ class SandwichNormFunction(torch.autograd.Function):
         g = ops.sandwich_norm_bwd(flat(dy), b, inv_b, gamma_post, gate, residual_scale=ctx.scales[0],
                                   branch_scale=ctx.scales[1], **more)
         like = lambda v, p: None if p is None or v is None else v.reshape(p.shape).to(p.dtype)
-        return (g["db"].view(ctx.shape), g["dx"].view(ctx.shape), like(g["dgamma_post"], gamma_post),
+        return (g["db"].view(ctx.shape), g["dx"].view(ctx.x_shape), like(g["dgamma_post"], gamma_post),
                 like(g["dgate"], gate), like(g["dgamma_pre"], gamma_pre), None, None, None, None)
 
 
@@ -233,7 +235,8 @@ def sandwich_norm(b: torch.Tensor, x: torch.Tensor, gamma_post: Optional[torch.T
                   residual_scale: float = 1.0, branch_scale: float = 1.0, eps: float = 1e-6,
                   pre: Optional[bool] = None):
     """Differentiable ``ops.sandwich_norm`` on b, x [..., D]: y, or (y, n) when the
-    next block's pre-norm is asked for (``gamma_pre`` given or ``pre=True``).
+    next block's pre-norm is asked for (``gamma_pre`` given or ``pre=True``), in
+    b's shape (x may lay the same rows out in another).
     A gate of shape [B, D] (or [B, 1, D]) goes with x of shape [B, S, D]."""
     return SandwichNormFunction.apply(b, x, gamma_post, gate, gamma_pre, float(residual_scale), float(branch_scale),
                                       float(eps), pre)
