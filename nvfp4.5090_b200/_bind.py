@@ -21,6 +21,10 @@ def load():
     if not os.path.exists(path):
         raise _lib.NVFP4Error(f"torch binding not found at {path}; build it with "
                               "`python -c 'import __graft_entry__ as g; g.build()'` (no fallback exists)")
+    made = _build.binding_built_for()
+    if made and made != _build.binding_target():   # its calls into another PyTorch would crash
+        raise _lib.NVFP4Error(f"the torch binding was built for {made}, this is {_build.binding_target()}: build it again with "
+                              "`python -c 'import __graft_entry__ as g; g.build()'`")
     _lib.load()
     loader = importlib.machinery.ExtensionFileLoader(_build.BINDING_NAME, path)
     module = importlib.util.module_from_spec(importlib.util.spec_from_loader(_build.BINDING_NAME, loader))

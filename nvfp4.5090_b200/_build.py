@@ -23,6 +23,7 @@ LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libnvfp4b200.so")
 BINDING_NAME = "_nvfp4b200_torch"
 BINDING_PATH = os.path.join(LIB_DIR, BINDING_NAME + ".so")
+BINDING_STAMP = os.path.join(LIB_DIR, BINDING_NAME + ".txt")   # what the module was compiled against
 SOURCES = ["quant.cu", "gemm.cu", "train.cu", "noalloc.cu", "mx.cu", "mxlin.cu", "clip.cu", "norm.cu"]
 HEADERS = [os.path.join(CSRC, "common.cuh"), os.path.join(CSRC, "vec.cuh"), os.path.join(CSRC, "bulk.cuh"), os.path.join(CSRC, "mx.cuh"),
            os.path.join(CSRC, "sched_slots.h"), os.path.join(CSRC, "row_stop.h"), os.path.join(REPO_DIR, "include", "nvfp4_b200.h")]
@@ -75,11 +76,26 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB_PATH
 
 
+def binding_target() -> str:
+    """The PyTorch and Python whose binary interfaces the torch extension module is made for."""
+    import torch
+    return f"torch {torch.__version__}, C++11 ABI {int(torch._C._GLIBCXX_USE_CXX11_ABI)}, {sys.implementation.cache_tag}"
+
+
+def binding_built_for() -> str:
+    """``binding_target()`` at the time the module was built; empty where nothing tells."""
+    if not os.path.exists(BINDING_STAMP):
+        return ""
+    with open(BINDING_STAMP) as f:
+        return f.read().strip()
+
+
 def build_binding(force: bool = False, verbose: bool = False) -> str:
-    """Compile (if needed) the torch extension module next to the library."""
+    """Compile (if needed: sources newer, or another PyTorch or Python) the
+    torch extension module next to the library."""
     src = os.path.join(CSRC, "torch_binding.cpp")
     header = os.path.join(REPO_DIR, "include", "nvfp4_b200.h")
-    if not force and not _stale(BINDING_PATH, [src, header]):
+    if not force and not _stale(BINDING_PATH, [src, header]) and binding_built_for() == binding_target():
         return BINDING_PATH
     import sysconfig
 
@@ -104,6 +120,8 @@ def build_binding(force: bool = False, verbose: bool = False) -> str:
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)
     os.replace(tmp, BINDING_PATH)
+    with open(BINDING_STAMP, "w") as f:
+        f.write(binding_target() + "\n")
     return BINDING_PATH
 
 
