@@ -60,8 +60,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if verbose:
         for cmd in todo:
             print(" ".join(cmd), file=sys.stderr)
-    # side by side: norm.cu alone (some 150 kernels) takes about 110 s.  (Not with nvcc's
-    # --split-compile, 50 s: the forward norm at 16384 x 8192 then took 210 us, 190 without.)
+    # side by side: norm.cu alone (360 kernels) takes two to three minutes.  (Not with nvcc's
+    # --split-compile, half of that: the forward norm at 16384 x 8192 then took 210 us, 190 without.)
     with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
         for done in [pool.submit(subprocess.run, cmd, check=True) for cmd in todo]:
             done.result()

@@ -467,12 +467,19 @@ int take_mxlin_device_error() {
 
 using namespace nvfp4b200;
 
-// Whether the 128-row tiles, times blocks of 128 tokens, beat the 256 x 256 pair
-// tiles of the general GEMM: always for one block of tokens, and while there is
-// an SM for each of them.  Against the general GEMM (quantizer included): 256
-// tokens 18.7 / 27.2 us at 4096 x 14336 (64 tiles), 512 tokens 14.2 / 15.1 at 4096
-// x 4096 (128 tiles); 768 tokens 17.5 / 15.7 there (192 tiles), 256 tokens 18.3 /
-// 16.3 at 14336 x 4096 (224 tiles).
+// Whether to take the 128-row tiles, times blocks of 128 tokens, and not the 256 x
+// 256 pair tiles of the general GEMM: for one block of tokens, and while there is
+// an SM for each tile.  Both ways in us (quantizer included, replayed from a graph
+// over weights that come from HBM), weights as n x k:
+//   tokens            16          64          96         128         256
+//   28672 x 4096   16.8/23.8   17.7/23.6   19.4/23.9   19.8/24.6   26.3/26.0 *
+//   14336 x 4096   12.5/14.7   13.7/14.9   14.9/15.2   15.9/15.6   16.4/16.5 *
+//   4096 x 14336   12.6/25.6   14.3/25.9   15.6/26.3   17.7/26.7   18.8/27.3
+//   4096 x 4096     8.3/12.9   10.9/13.3   13.0/13.6   15.1/14.1   12.9/14.1
+//   57344 x 8192   51.0/66.0   51.5/62.5   55.6/64.0   58.0/65.2   68.6/68.6 *
+// (*: the rule takes the general GEMM.)  So the rule costs up to 7% at 97 to 128
+// tokens of a small weight, where K is in four parts.  512 tokens 14.2/15.1 at
+// 4096 x 4096 (128 tiles), 768 tokens 17.5/15.7 there (192 tiles).
 static bool few_tokens(int64_t m, int64_t tiles, int sms) { return m <= 128 || tiles * ceil_div(m, 128) <= sms; }
 
 extern "C" {

@@ -1176,8 +1176,8 @@ int nvfp4b200_sandwich_norm(const void* b, const void* x, const void* gamma_post
       constexpr int T = decltype(tpr)::value, THREADS = norm::threads_of(T), GROUPS = THREADS / T;
       constexpr int DT = decltype(dt)::value;
       constexpr bool VEC = decltype(v)::value;
-      // the staged kernel where its ring fits (all but fp32 rows of more than 8192 columns): 195 -> 168 us
-      // at 16384 x 8192 bf16 with the next norm.  fp32: 8 columns a thread, so that 32 warps share an SM
+      // the staged kernel where its ring fits (all but fp32 rows of more than 8192 columns): 195 us without,
+      // 168 to 187 by the GPU with it, at 16384 x 8192 bf16 with the next norm.  fp32: 8 columns a thread, so that 32 warps share an SM
       // (8192 x 4096: 88 us, 141 with 16 columns; bf16 at 16384 x 4096 93 with 16 columns, 109 with 8)
       constexpr int V = DT == NVFP4B200_F32 && T <= 512 ? 1 : norm::VPT, TV = T * norm::VPT / V;
       constexpr int THREADS_V = norm::threads_of(TV);
@@ -1269,8 +1269,8 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
     const int r = norm::by_width((int)d, [&](auto tpr) {
       constexpr int T = decltype(tpr)::value, DT = decltype(dt)::value;
       constexpr bool ODD = !decltype(v)::value;
-      // the staged kernel: 346 -> 152 us at 16000 x 4096 bf16 with 8 gates and the next norm, 611 -> 246 with a
-      // gate per row
+      // the staged kernel: at 16000 x 4096 bf16 with 8 gates and the next norm 346 us without, 149 to 165 by the
+      // GPU with it; 611 and 246 with a gate per row
       auto staged = [&]() -> int {
         constexpr bool SPLIT = T > 512;
         constexpr int T2 = SPLIT ? T : 2 * T;
@@ -1315,7 +1315,8 @@ int nvfp4b200_sandwich_norm_bwd(const void* dy, const void* dn, const void* b, c
       if constexpr (!ODD) {
         return staged();
       } else {
-        // the ring's copies start on 16-byte boundaries
+        // the ring's copies start on 16-byte boundaries.  (Without the ring 16000 x 4096 bf16 takes 784 us, and
+        // 4096 x 16384, 32 registers for 16 columns a thread, 2099 against 225: such tensors are better copied.)
         if (aligned(b, 16) && (!dy || aligned(dy, 16)) && (!dn || (aligned(dn, 16) && aligned(y, 16)))) return staged();
         // 8 columns a thread while 1024 threads cover the row: twice the warps of 16
         // columns (166 -> 123 us at 2013 x 4971 fp16)

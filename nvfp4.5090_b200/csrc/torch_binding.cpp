@@ -266,7 +266,7 @@ std::tuple<Tensor, OptTensor, OptTensor> linear_forward(const Tensor& x_, const 
   OptTensor bias;
   if (bias_) {
     TORCH_CHECK(on(*bias_, x_) && bias_->numel() == n, "bias is a tensor [N] on the input's device");
-    bias = vector_of(bias_->to(at::kBFloat16));
+    bias = vector_of(bias_->to(at::kBFloat16));   // the type in which the product's epilogue reads it
   }
   On at_(x_);
   const Tensor x = float_matrix(x_.dim() == 2 ? x_ : x_.reshape({-1, k})), w = float_matrix(w_);

@@ -406,7 +406,10 @@ def mxfp4_linear(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     dimension, which takes K % 32 == 0 and, for gradients, N % 32 == 0 (else
     N % 8 == 0); tokens count as filled up with zeros.  Quantization is the
     identity in the backward, which keeps x and the weight in MXFP4 only; there
-    is no second derivative."""
+    is no second derivative.  The bias is rounded to bf16 before it is added,
+    whatever its type (2^-8 of its magnitude at most, less than the 4-bit
+    weights' own rounding); gradients have the types of what they belong to, each rounded
+    once from fp32."""
     return _bind.ext.mxfp4_linear(input, weight, bias)
 
 
