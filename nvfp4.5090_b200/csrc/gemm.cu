@@ -55,6 +55,7 @@
 #include <cstring>
 #include <atomic>
 #include <mutex>
+#include <type_traits>
 
 namespace nvfp4b200 {
 
@@ -1297,7 +1298,8 @@ struct DswigluIn {
 using Slots = SchedSlots<STREAM_SLOTS, GRAPH_SLOTS>;
 
 static Slots& slots_of(int dev) {
-  static Slots* all = new Slots[64];   // never freed: graphs may go after static objects have
+  static Slots all[64];
+  static_assert(std::is_trivially_destructible<Slots>::value, "graphs may go after static objects have");
   return all[dev & 63];
 }
 

@@ -9,12 +9,11 @@
 #pragma once
 
 #include <cstdint>
-#include <deque>
 #include <mutex>
-#include <unordered_map>
 
 namespace nvfp4b200 {
 
+// Plain arrays: nothing here allocates, so nothing throws through a C entry point.
 template <int STREAMS, int GRAPHS>
 class SchedSlots {   // of one device
  public:
@@ -23,34 +22,35 @@ class SchedSlots {   // of one device
   // The counter of a stream, by an id that no other stream ever has.
   int of_stream(uint64_t id) {
     std::lock_guard<std::mutex> lock(mu_);
-    const auto at = streams_.find(id);
-    if (at != streams_.end()) return at->second;
-    if ((int)streams_.size() == STREAMS) return -1;
-    const int slot = (int)streams_.size();
-    streams_.emplace(id, slot);
-    return slot;
+    for (int i = 0; i < streams_; ++i)
+      if (ids_[i] == id) return i;
+    if (streams_ == STREAMS) return -1;
+    ids_[streams_] = id;
+    return streams_++;
   }
 
   // A counter for one captured launch, until give_back.
   int take() {
     std::lock_guard<std::mutex> lock(mu_);
     if (fresh_ < GRAPHS) return STREAMS + fresh_++;
-    if (back_.empty()) return -1;
-    const int slot = back_.front();   // the one that has been back the longest
-    back_.pop_front();
+    if (waiting_ == 0) return -1;
+    const int slot = back_[first_];   // the one that has been back the longest
+    first_ = (first_ + 1) % GRAPHS;
+    --waiting_;
     return slot;
   }
 
-  void give_back(int slot) {
+  void give_back(int slot) {   // one that take() gave: at most GRAPHS are out
     std::lock_guard<std::mutex> lock(mu_);
-    back_.push_back(slot);
+    back_[(first_ + waiting_++) % GRAPHS] = slot;
   }
 
  private:
   std::mutex mu_;
-  std::unordered_map<uint64_t, int> streams_;
-  std::deque<int> back_;
-  int fresh_ = 0;
+  uint64_t ids_[STREAMS] = {};
+  int streams_ = 0, fresh_ = 0;
+  int back_[GRAPHS] = {};   // given back: waiting_ of them from first_ on, around the end
+  int first_ = 0, waiting_ = 0;
 };
 
 }  // namespace nvfp4b200

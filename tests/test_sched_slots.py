@@ -86,3 +86,23 @@ def test_from_many_threads(lib):
     for t in threads:
         t.join()
     assert not bad
+
+
+def test_given_back_many_times(lib):
+    """Around the end of the list of counters given back, in the order they came."""
+    s = lib.make()
+    held = [lib.take(s) for _ in range(GRAPHS)]
+    for i in range(50):
+        out = held[: 1 + i % GRAPHS]
+        for slot in out:
+            lib.give_back(s, slot)
+        again = [lib.take(s) for _ in out]
+        assert again == out and lib.take(s) == -1
+        held = held[len(out):] + again
+    assert sorted(held) == list(range(STREAMS, STREAMS + GRAPHS))
+
+
+def test_nothing_is_allocated():
+    """A C entry point lets no exception through: the header holds no container that can throw."""
+    text = open(HEADER).read()
+    assert not any(w in text for w in ("unordered_map", "deque", "vector", "new "))
