@@ -1177,8 +1177,9 @@ int nvfp4b200_sandwich_norm(const void* b, const void* x, const void* gamma_post
       constexpr int DT = decltype(dt)::value;
       constexpr bool VEC = decltype(v)::value;
       // the staged kernel where its ring fits (all but fp32 rows of more than 8192 columns): 195 us without,
-      // 168 to 187 by the GPU with it, at 16384 x 8192 bf16 with the next norm.  fp32: 8 columns a thread, so that 32 warps share an SM
-      // (8192 x 4096: 88 us, 141 with 16 columns; bf16 at 16384 x 4096 93 with 16 columns, 109 with 8)
+      // 168 to 187 by the GPU with it, at 16384 x 8192 bf16 with the next norm.  fp32: 8 columns a thread,
+      // so that 32 warps share an SM (8192 x 4096: 88 us, 141 with 16 columns; bf16 at 16384 x 4096 93 with
+      // 16 columns, 109 with 8)
       constexpr int V = DT == NVFP4B200_F32 && T <= 512 ? 1 : norm::VPT, TV = T * norm::VPT / V;
       constexpr int THREADS_V = norm::threads_of(TV);
       constexpr int smem = norm::STAGES * 2 * THREADS_V * 8 * V * norm::dtype_size<DT>();

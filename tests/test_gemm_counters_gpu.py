@@ -65,7 +65,7 @@ def test_many_launches_on_several_streams(pkg):
     ops = pkg.ops
     sets = []
     for i in range(4):
-        qa, qb = ops.mx_quantize(rnd((2560 + 256 * i, 512), i)), ops.mx_quantize(rnd((4096, 512), 10 + i))
+        qa, qb = ops.mx_quantize(rnd((2400 + 300 * i, 512), i)), ops.mx_quantize(rnd((4096, 512), 10 + i))
         sets.append((qa, qb, ops.mx_gemm(*qa, *qb)))
     outs = [[torch.zeros_like(r) for _ in range(3)] for _, _, r in sets]
     streams = [torch.cuda.Stream() for _ in sets]
@@ -102,4 +102,41 @@ def test_more_captured_launches_than_counters(pkg):
         assert all(torch.equal(o, ref) for o in outs) and torch.equal(nout, nref)
         assert torch.equal(ops.mx_gemm(*qa, *qb), ref)
         del graph
+    assert ops.device_error() == 0
+
+
+def test_large_products_behind_dependent_launches(pkg):
+    """Captured together: few-token products, which start while the kernel before
+    them still runs, each right before a product of several tiles per CTA pair."""
+    ops = pkg.ops
+    w1, w2 = ops.mx_quantize(rnd((2048, 2048), 1, 0.02)), ops.mx_quantize(rnd((8192, 2048), 2, 0.02))
+    tok, big = rnd((8, 2048), 3), ops.mx_quantize(rnd((2400, 2048), 4))
+    more = rnd((100, 2048), 5)
+
+    def chain():
+        out = []
+        for x in (tok, more):
+            out += [ops.mx_linear(x, *w1), ops.mx_gemm(*big, *w2)]
+        return out
+
+    ref = chain()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(chain())
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for rep in range(10):
+        for o in outs:
+            for v in o:
+                v.zero_()
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for o in outs:
+            assert all(torch.equal(a, b) for a, b in zip(o, ref)), rep
     assert ops.device_error() == 0
